@@ -33,6 +33,11 @@ int suhpe_abi_version(void);
 enum { SUHPE_ACT_NONE = 0, SUHPE_ACT_RELU = 1, SUHPE_ACT_RELU6 = 2, SUHPE_ACT_SILU = 3, SUHPE_ACT_GELU = 4,
        SUHPE_ACT_SIGMOID = 5 };
 
+/* element types of the operators that take fp32, bf16 or fp16 rows (every other entry point is fp32) */
+enum { SUHPE_F32 = 0, SUHPE_BF16 = 1, SUHPE_F16 = 2 };
+/* types of the positions that suhpe_rope_axes takes */
+enum { SUHPE_POS_I32 = 0, SUHPE_POS_I64 = 1, SUHPE_POS_F32 = 2 };
+
 /* ------------------------------------------------------------------ matrix-Fisher rotation head ---------- */
 /* src/fisher/fisher_utils.py:14-36 (vmf_loss / KL_Fisher) + :39-48.  A,R: (n,9).  Writes loss (n), the
  * gradient dloss_i/dA_i (n,9) and the mode rotation Rest (n,9).  Any output pointer may be NULL. */
@@ -564,6 +569,46 @@ int suhpe_window_attn_bwd_rs(const float* qkv, const float* fwd_out, const float
 int64_t suhpe_window_attn_dbias_workspace_bytes(int ws, int heads);
 int suhpe_window_attn_dbias(const float* dS, const int32_t* inv_ptr, const int32_t* inv_list, int B, int H, int W, int ws, int heads,
                             int noff, float* dbias_table, void* workspace, suhpe_stream_t stream);
+
+/* ------------------------------------------------------------------ operators of transformer blocks ------ */
+/* New capability next to src/tiny_vit.py's blocks (LayerNorm, Linear, GELU, bias-table attention, all fp32 there): rotary positions, gated feed-forward,
+ * dropout without a stored mask, 16-bit LayerNorm.  `dtype` is the type of x, y and of everything without another type in its declaration.  Zero rows
+ * are allowed (nothing is read; gradients of weights are then zero).
+ *
+ * Rotary positions with several axes.  x, y: (rows, heads, parts, dh), contiguous; parts 0 .. rotated - 1 of every head are rotated (packed qkv rows of
+ * the windowed attention: parts = 3, rotated = 2), the others and the channels from 2 * pairs on are copied.  Pair p turns by pos[row][axis[p]] *
+ * freq[p] * 2 pi (freq: revolutions per unit of position); its members are channels (p, p + pairs) where halves != 0, else (2 p, 2 p + 1):
+ *   (x1, x2) -> (x1 cos - x2 sin, x1 sin + x2 cos);  inverse != 0 turns back, which is also the gradient.
+ * pos: (rows, naxes) of pos_type, axis entries in 0 .. naxes - 1; angles are exact to fp32 for |pos| < 2^31.  y == x rotates in place (nothing is
+ * copied); other overlaps are not allowed. */
+int suhpe_rope_axes(const void* x, int dtype, int64_t rows, int heads, int parts, int rotated, int dh, const void* pos, int pos_type, int naxes,
+                    const double* freq, const int32_t* axis, int pairs, int halves, int inverse, void* y, suhpe_stream_t stream);
+/* Dropout whose mask is never stored: y[i] = (skip ? skip[i] : 0) + (kept(i) ? x[i] / keep : 0), kept(i) the draw of suhpe_dropout_mask for element i at
+ * host_offset = position (so y equals x * mask [+ skip]; a dropped element is 0 whatever x[i] is).  The gradient of x is the same call on dy with the
+ * same counter and position; (count + 3) / 4 positions are used.  y may be x or skip itself; other overlaps are not allowed. */
+int suhpe_dropout_apply(const void* x, int dtype, int64_t count, float keep, const uint64_t* counter, uint64_t position, const void* skip, void* y,
+                        suhpe_stream_t stream);
+/* counter[1] += by on the device: the last launch of a captured graph that draws, so that its next replay draws fresh numbers */
+int suhpe_dropout_advance(uint64_t* counter, uint64_t by, suhpe_stream_t stream);
+/* LayerNorm of bf16 / fp16 rows with fp32 statistics, parameters and parameter gradients; skip as in suhpe_layernorm_bwd_skip (NULL: none);
+ * dgamma / dbeta may be NULL.  workspace: suhpe_layernorm16_bwd_workspace_bytes(c). */
+int suhpe_layernorm16_fwd(const void* x, int dtype, int64_t rows, int c, float eps, const float* gamma, const float* beta, void* y, float* mean, float* rstd,
+                          suhpe_stream_t stream);
+int64_t suhpe_layernorm16_bwd_workspace_bytes(int c);
+int suhpe_layernorm16_bwd(const void* x, const void* dy, int dtype, int64_t rows, int c, const float* mean, const float* rstd, const float* gamma, const void* skip,
+                          void* dx, float* dgamma, float* dbeta, int accumulate, void* workspace, int64_t workspace_bytes, suhpe_stream_t stream);
+/* Gated feed-forward block: g = x wg^T + bg, u = x wu^T + bu, h = act(g) u, y = h wd^T + bd.  x (m, k), wg / wu (n, k), wd (o, n), y (m, o); biases may be
+ * NULL.  h (m, n) is always written; g and u (m, n) where not NULL (the backward needs all three).  Products are summed in fp32; g, u and h are rounded
+ * to dtype once.  act: any SUHPE_ACT_*.
+ * Backward: dx (NULL: not wanted), dwg / dwu / dwd and dbg / dbu / dbd (NULL: not wanted; the three weights' together) of type grad_dtype (dtype or
+ * SUHPE_F32), added to what they hold where accumulate != 0.  Every sum has a fixed order: results do not vary from call to call. */
+int64_t suhpe_gated_ffn_fwd_workspace_bytes(int dtype, int64_t m, int k, int n, int o);
+int suhpe_gated_ffn_fwd(int dtype, int act, int64_t m, int k, int n, int o, const void* x, const void* wg, const void* wu, const void* wd, const void* bg, const void* bu,
+                        const void* bd, void* g, void* u, void* h, void* y, void* workspace, int64_t workspace_bytes, suhpe_stream_t stream);
+int64_t suhpe_gated_ffn_bwd_workspace_bytes(int dtype, int64_t m, int k, int n, int o);
+int suhpe_gated_ffn_bwd(int dtype, int act, int64_t m, int k, int n, int o, const void* dy, const void* x, const void* wg, const void* wu, const void* wd, const void* g,
+                        const void* u, const void* h, void* dx, void* dwg, void* dwu, void* dwd, void* dbg, void* dbu, void* dbd, int grad_dtype, int accumulate,
+                        void* workspace, int64_t workspace_bytes, suhpe_stream_t stream);
 
 /* ---- data-parallel exchange (new capability: the reference trains on one GPU, train.py:24-25).
  * One communicator per rank (= per process, = per GPU) over RCCL / xGMI; float32 payloads; every call is enqueued on `stream`

@@ -1,0 +1,380 @@
+// Operators on token rows in fp32 / bf16 / fp16: rotary positions with several axes, dropout whose mask is never stored, 16-bit LayerNorm.
+// All three are bound by memory: each element is read once and written once, in 16-byte vectors where sizes and addresses allow.
+#include "lowp.h"
+
+namespace suhpe {
+namespace {
+
+// ------------------------------------------------------------------------------------------ rotary positions
+// Pair p of a head belongs to axis[p] and turns by pos[row][axis[p]] * freq[p] radians.  The angle is formed in 64 bits as REVOLUTIONS (freq holds
+// radians / 2 pi): the whole turns are dropped exactly before the 32-bit sine and cosine, so a position of 10^6 is as exact as one of 10.
+// A block takes R rows: it evaluates sine and cosine of each (row, pair) ONCE into LDS and then streams all heads of those rows past the table
+// (q and k, every head: the evaluation is amortised over heads * rotated vectors).
+template <typename P> __device__ __forceinline__ double pos_of(const P* pos, int64_t i) { return (double)pos[i]; }
+
+struct RopeArgs {
+    int64_t rows;
+    int heads, parts, rotated, dh, naxes, pairs, halves, inverse, copy, rows_per_block;
+    const double* freq;
+    const int32_t* axis;
+};
+
+template <typename T, typename P, int V>
+__global__ __launch_bounds__(256) void rope_axes_kernel(const T* x, T* y, const P* __restrict__ pos, const RopeArgs a) {
+    extern __shared__ __attribute__((aligned(16))) float2 turn[];      // [row][pair] cos, sin
+    const int64_t row0 = (int64_t)blockIdx.x * a.rows_per_block;
+    const int nrows = (int)(a.rows - row0 < a.rows_per_block ? a.rows - row0 : a.rows_per_block);
+    for (int i = threadIdx.x; i < nrows * a.pairs; i += 256) {
+        const int r = i / a.pairs, p = i - r * a.pairs;
+        const double rev = pos_of(pos, (row0 + r) * a.naxes + a.axis[p]) * a.freq[p];
+        float s, c;
+        sincospif(2.f * (float)(rev - rint(rev)), &s, &c);
+        turn[i] = make_float2(c, a.inverse ? -s : s);
+    }
+    __syncthreads();
+    // items of a head: rotated parts first -- `ir` vectors of pairs (halves: the first members, whose partners lie `pairs` further; adjacent: V / 2
+    // pairs a vector; V == 1: one pair an item in both layouts) and `ip` vectors behind the rotated width -- then the parts that stay as they are
+    const bool wide = V > 1 && !a.halves;
+    const int ir = wide ? 2 * a.pairs / V : a.pairs / V, ip = a.copy ? (a.dh - 2 * a.pairs) / V : 0;
+    const int irp = ir + ip, nrot = a.rotated * irp, nh = nrot + (a.copy ? (a.parts - a.rotated) * (a.dh / V) : 0);
+    const int per_row = a.heads * nh, total = nrows * per_row;
+    constexpr int U = 4;
+    for (int i0 = threadIdx.x; i0 < total; i0 += 256 * U) {
+        float v1[U][V], v2[U][V];
+        int64_t at1[U];
+        int at2[U], tab[U];                                            // tab: first pair's place in the table, -1: a plain copy
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + 256 * u;
+            at1[u] = -1;
+            if (i >= total) continue;
+            const int r = i / per_row, rem = i - r * per_row, h = rem / nh, j = rem - h * nh;
+            const int64_t head = ((row0 + r) * a.heads + h) * a.parts * (int64_t)a.dh;
+            at2[u] = -1;
+            if (j < nrot) {
+                const int part = j / irp, q = j - part * irp;
+                if (q < ir) {
+                    const int p = wide ? q * V / 2 : q * V;
+                    tab[u] = r * a.pairs + p;
+                    at1[u] = head + part * a.dh + (a.halves ? p : 2 * p);
+                    if (!wide) at2[u] = a.halves ? a.pairs : 1;
+                } else {
+                    tab[u] = -1;
+                    at1[u] = head + part * a.dh + 2 * a.pairs + (q - ir) * V;
+                }
+            } else {
+                tab[u] = -1;
+                at1[u] = head + a.rotated * a.dh + (int64_t)(j - nrot) * V;
+            }
+            load_n<T, V>(x + at1[u], v1[u]);
+            if (at2[u] >= 0) load_n<T, V>(x + at1[u] + at2[u], v2[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (at1[u] < 0) continue;
+            if (tab[u] >= 0) {
+                if (at2[u] >= 0) {
+                    float o1[V], o2[V];
+#pragma unroll
+                    for (int k = 0; k < V; ++k) {
+                        const float2 t = turn[tab[u] + k];
+                        o1[k] = v1[u][k] * t.x - v2[u][k] * t.y;
+                        o2[k] = v1[u][k] * t.y + v2[u][k] * t.x;
+                    }
+                    store_n<T, V>(y + at1[u], o1);
+                    store_n<T, V>(y + at1[u] + at2[u], o2);
+                } else if constexpr (V > 1) {
+                    float o[V];
+#pragma unroll
+                    for (int k = 0; k < V; k += 2) {
+                        const float2 t = turn[tab[u] + k / 2];
+                        o[k] = v1[u][k] * t.x - v1[u][k + 1] * t.y;
+                        o[k + 1] = v1[u][k] * t.y + v1[u][k + 1] * t.x;
+                    }
+                    store_n<T, V>(y + at1[u], o);
+                }
+            } else {
+                store_n<T, V>(y + at1[u], v1[u]);
+            }
+        }
+    }
+}
+
+template <typename T, typename P>
+int rope_launch(const T* x, T* y, const P* pos, RopeArgs a, hipStream_t st) {
+    constexpr int FULL = 16 / sizeof(T);
+    const int step = a.halves ? a.pairs : 2 * a.pairs;                 // the widths that a vector must divide
+    const auto fits = [&](int v) { return a.dh % v == 0 && step % v == 0 && aligned(x, v * sizeof(T)) && aligned(y, v * sizeof(T)); };
+    // about 2048 elements per thread block keep a few loads of every thread in flight; the table stays under 32 KB
+    const int64_t width = (int64_t)a.heads * a.parts * a.dh;
+    int64_t r = ceil_div(256 * 4 * FULL, width);
+    if (r * a.pairs > 4096) r = 4096 / a.pairs;
+    if (r < 1) r = 1;
+    if (r > a.rows) r = a.rows;
+    a.rows_per_block = (int)r;
+    const dim3 grid((unsigned)ceil_div(a.rows, r));
+    const size_t lds = (size_t)r * a.pairs * sizeof(float2);
+    if (fits(FULL)) hipLaunchKernelGGL((rope_axes_kernel<T, P, FULL>), grid, dim3(256), lds, st, x, y, pos, a);
+    else if (fits(FULL / 2)) hipLaunchKernelGGL((rope_axes_kernel<T, P, FULL / 2>), grid, dim3(256), lds, st, x, y, pos, a);
+    else hipLaunchKernelGGL((rope_axes_kernel<T, P, 1>), grid, dim3(256), lds, st, x, y, pos, a);
+    return check_launch("suhpe_rope_axes");
+}
+
+template <typename T>
+int rope_types(const void* x, void* y, const void* pos, int pos_type, const RopeArgs& a, hipStream_t st) {
+    const T* xt = static_cast<const T*>(x);
+    T* yt = static_cast<T*>(y);
+    if (pos_type == SUHPE_POS_I32) return rope_launch<T, int32_t>(xt, yt, static_cast<const int32_t*>(pos), a, st);
+    if (pos_type == SUHPE_POS_I64) return rope_launch<T, int64_t>(xt, yt, static_cast<const int64_t*>(pos), a, st);
+    return rope_launch<T, float>(xt, yt, static_cast<const float*>(pos), a, st);
+}
+
+// ------------------------------------------------------------------------------------------ dropout without a stored mask
+// y_i = [skip_i +] (r_i < keep ? x_i / keep : 0) with r_i the 24-bit number that suhpe_dropout_mask draws for element i at the same stream position:
+// word i % 4 of Philox call counter[1] + position + i / 4.  The gradient is the same call on dy: nothing is kept between the two.
+// A dropped element is 0 whatever x holds there (also infinities and NaN).
+template <typename T, bool VECTOR>
+__global__ __launch_bounds__(256) void dropout_apply_kernel(const T* x, const T* skip, T* y, int64_t count, uint32_t bound, float scale,
+                                                            const uint64_t* __restrict__ counter, uint64_t position) {
+    constexpr int N = VECTOR ? 16 / sizeof(T) : 4;                      // elements of a thread's turn: one or two calls of the generator
+    const uint64_t seed = counter[0], base = counter[1] + position;
+    const int64_t turns = (count + N - 1) / N, stride = (int64_t)gridDim.x * 256;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < turns; i += stride) {
+        const int64_t e0 = i * N;
+        const int n = count - e0 < N ? (int)(count - e0) : N;
+        float v[N], s[N];
+        if (VECTOR && n == N) {
+            load_n<T, N>(x + e0, v);
+            if (skip) load_n<T, N>(skip + e0, s);
+        } else {
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                v[k] = k < n ? (float)x[e0 + k] : 0.f;
+                s[k] = k < n && skip ? (float)skip[e0 + k] : 0.f;
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < N; q += 4) {
+            uint32_t w[4];
+            philox_words(seed, base + (uint64_t)((e0 + q) >> 2), w);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float d = (w[k] >> 8) < bound ? v[q + k] * scale : 0.f;
+                v[q + k] = skip ? s[q + k] + d : d;
+            }
+        }
+        if (VECTOR && n == N) {
+            store_n<T, N>(y + e0, v);
+        } else {
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+                if (k < n) y[e0 + k] = (T)v[k];
+        }
+    }
+}
+
+__global__ void dropout_advance_kernel(uint64_t* counter, uint64_t by) { counter[1] += by; }
+
+template <typename T>
+int dropout_launch(const void* x, const void* skip, void* y, int64_t count, uint32_t bound, float scale, const uint64_t* counter, uint64_t position, hipStream_t st) {
+    const T *xt = static_cast<const T*>(x), *kt = static_cast<const T*>(skip);
+    T* yt = static_cast<T*>(y);
+    if (aligned(x, 16) && aligned(y, 16) && aligned(skip, 16))
+        hipLaunchKernelGGL((dropout_apply_kernel<T, true>), dim3(grid_for(ceil_div(count, 16 / sizeof(T)), 256)), dim3(256), 0, st, xt, kt, yt, count, bound, scale, counter, position);
+    else
+        hipLaunchKernelGGL((dropout_apply_kernel<T, false>), dim3(grid_for(ceil_div(count, 4), 256)), dim3(256), 0, st, xt, kt, yt, count, bound, scale, counter, position);
+    return check_launch("suhpe_dropout_apply");
+}
+
+// ------------------------------------------------------------------------------------------ LayerNorm of 16-bit rows
+// y = (x - mean) rstd gamma + beta with the statistics, gamma, beta and the parameters' gradients in fp32: only x, y, dy, dx have 16 bits.
+// One wavefront per row, any width.
+template <typename T>
+__global__ __launch_bounds__(256) void layernorm16_fwd_any(const T* __restrict__ x, int64_t rows, int c, float eps, const float* __restrict__ gamma,
+                                                           const float* __restrict__ beta, T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    const T* xr = x + row * c;
+    float s = 0.f;
+    for (int j = lane; j < c; j += 64) s += (float)xr[j];
+    const float m = wave_sum(s) / c;
+    float q = 0.f;
+    for (int j = lane; j < c; j += 64) { const float d = (float)xr[j] - m; q += d * d; }
+    const float rs = 1.f / sqrtf(wave_sum(q) / c + eps);
+    for (int j = lane; j < c; j += 64) y[row * c + j] = (T)(((float)xr[j] - m) * rs * (gamma ? gamma[j] : 1.f) + (beta ? beta[j] : 0.f));
+    if (lane == 0) { mean[row] = m; rstd[row] = rs; }
+}
+
+// dx = rstd (g - mean(g) - xhat mean(g xhat)) [+ skip], g = dy gamma
+template <typename T>
+__global__ __launch_bounds__(256) void layernorm16_bwd_dx_any(const T* __restrict__ x, const T* __restrict__ dy, int64_t rows, int c,
+                                                              const float* __restrict__ mean, const float* __restrict__ rstd, const float* __restrict__ gamma,
+                                                              const T* __restrict__ skip, T* __restrict__ dx) {
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    const float m = mean[row], rs = rstd[row];
+    const int64_t at = row * c;
+    float s0 = 0.f, s1 = 0.f;
+    for (int j = lane; j < c; j += 64) {
+        const float g = (float)dy[at + j] * (gamma ? gamma[j] : 1.f);
+        s0 += g;
+        s1 += g * (((float)x[at + j] - m) * rs);
+    }
+    s0 = wave_sum(s0) / c;
+    s1 = wave_sum(s1) / c;
+    for (int j = lane; j < c; j += 64) {
+        const float g = (float)dy[at + j] * (gamma ? gamma[j] : 1.f), xh = ((float)x[at + j] - m) * rs;
+        dx[at + j] = (T)(rs * (g - s0 - xh * s1) + (skip ? (float)skip[at + j] : 0.f));
+    }
+}
+
+// column sums of dy and dy * xhat over a block's rows: part[block][2][c]
+template <typename T>
+__global__ __launch_bounds__(256) void layernorm16_bwd_cols_any(const T* __restrict__ x, const T* __restrict__ dy, int64_t rows, int c, int64_t rows_per_block,
+                                                                const float* __restrict__ mean, const float* __restrict__ rstd, float* __restrict__ part) {
+    __shared__ float lds[2][4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = blockIdx.y * 64 + lane;
+    const int64_t r0 = (int64_t)blockIdx.x * rows_per_block, r1 = r0 + rows_per_block < rows ? r0 + rows_per_block : rows;
+    float sg = 0.f, sb = 0.f;
+    if (j < c)
+        for (int64_t r = r0 + wave; r < r1; r += 4) {
+            const float d = (float)dy[r * c + j];
+            sb += d;
+            sg += d * (((float)x[r * c + j] - mean[r]) * rstd[r]);
+        }
+    lds[0][wave][lane] = sg;
+    lds[1][wave][lane] = sb;
+    __syncthreads();
+    if (wave == 0 && j < c) {
+        part[((int64_t)blockIdx.x * 2 + 0) * c + j] = (lds[0][0][lane] + lds[0][1][lane]) + (lds[0][2][lane] + lds[0][3][lane]);
+        part[((int64_t)blockIdx.x * 2 + 1) * c + j] = (lds[1][0][lane] + lds[1][1][lane]) + (lds[1][2][lane] + lds[1][3][lane]);
+    }
+}
+
+// the partial sums of `blocks` blocks in a fixed order: 16 columns x 16 slices per block
+__global__ __launch_bounds__(256) void layernorm16_bwd_finish(const float* __restrict__ part, int blocks, int c, float* __restrict__ dgamma, float* __restrict__ dbeta,
+                                                              int accumulate) {
+    __shared__ float lds[16][17];
+    const int col = threadIdx.x & 15, slice = threadIdx.x >> 4, j = blockIdx.x * 16 + col, which = blockIdx.y;
+    float s = 0.f;
+    if (j < c)
+        for (int b = slice; b < blocks; b += 16) s += part[((int64_t)b * 2 + which) * c + j];
+    lds[slice][col] = s;
+    __syncthreads();
+    float* out = which ? dbeta : dgamma;
+    if (slice == 0 && j < c && out) {
+        float t = 0.f;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) t += lds[k][col];
+        out[j] = accumulate ? out[j] + t : t;
+    }
+}
+
+constexpr int kLnBlocks = 512;
+
+template <typename T>
+int ln16_fwd(const void* x, int64_t rows, int c, float eps, const float* gamma, const float* beta, void* y, float* mean, float* rstd, hipStream_t st) {
+    hipLaunchKernelGGL((layernorm16_fwd_any<T>), dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, st, static_cast<const T*>(x), rows, c, eps, gamma, beta,
+                       static_cast<T*>(y), mean, rstd);
+    return check_launch("suhpe_layernorm16_fwd");
+}
+
+template <typename T>
+int ln16_bwd(const void* x, const void* dy, int64_t rows, int c, const float* mean, const float* rstd, const float* gamma, const void* skip, void* dx, float* dgamma,
+             float* dbeta, int accumulate, float* part, hipStream_t st) {
+    const T *xt = static_cast<const T*>(x), *dt = static_cast<const T*>(dy);
+    int blocks = 0;
+    if (rows > 0) {
+        hipLaunchKernelGGL((layernorm16_bwd_dx_any<T>), dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, st, xt, dt, rows, c, mean, rstd, gamma,
+                           static_cast<const T*>(skip), static_cast<T*>(dx));
+        if (dgamma || dbeta) {
+            blocks = (int)(ceil_div(rows, 16) < kLnBlocks ? ceil_div(rows, 16) : kLnBlocks);
+            const int64_t per = ceil_div(rows, blocks);
+            blocks = (int)ceil_div(rows, per);
+            hipLaunchKernelGGL((layernorm16_bwd_cols_any<T>), dim3(blocks, (unsigned)ceil_div(c, 64)), dim3(256), 0, st, xt, dt, rows, c, per, mean, rstd, part);
+        }
+    }
+    if (dgamma || dbeta)
+        hipLaunchKernelGGL(layernorm16_bwd_finish, dim3((unsigned)ceil_div(c, 16), 2), dim3(256), 0, st, part, blocks, c, dgamma, dbeta, accumulate);
+    return check_launch("suhpe_layernorm16_bwd");
+}
+
+}  // namespace
+}  // namespace suhpe
+
+using namespace suhpe;
+
+extern "C" {
+
+int suhpe_rope_axes(const void* x, int dtype, int64_t rows, int heads, int parts, int rotated, int dh, const void* pos, int pos_type, int naxes, const double* freq,
+                    const int32_t* axis, int pairs, int halves, int inverse, void* y, suhpe_stream_t stream) {
+    SUHPE_REQUIRE(dtype_ok(dtype), "suhpe_rope_axes: unknown dtype %d", dtype);
+    SUHPE_REQUIRE(pos_type >= SUHPE_POS_I32 && pos_type <= SUHPE_POS_F32, "suhpe_rope_axes: unknown position type %d", pos_type);
+    SUHPE_REQUIRE(rows >= 0 && heads > 0 && parts > 0 && rotated > 0 && rotated <= parts && dh > 1 && naxes > 0, "suhpe_rope_axes: bad sizes");
+    SUHPE_REQUIRE(pairs > 0 && pairs <= 4096 && 2 * pairs <= dh, "suhpe_rope_axes: %d pairs do not fit heads of %d (at most 4096)", pairs, dh);
+    SUHPE_REQUIRE((int64_t)heads * parts * dh <= (1 << 24), "suhpe_rope_axes: a row of %lld elements is too wide", (long long)heads * parts * dh);
+    SUHPE_REQUIRE(rows <= 0x7fffffff, "suhpe_rope_axes: too many rows");
+    if (rows == 0) return SUHPE_OK;
+    SUHPE_REQUIRE(x && y && pos && freq && axis, "suhpe_rope_axes: null pointer");
+    const RopeArgs a = {rows, heads, parts, rotated, dh, naxes, pairs, halves ? 1 : 0, inverse ? 1 : 0, x != y, 0, freq, axis};
+    hipStream_t st = as_stream(stream);
+    if (dtype == SUHPE_F32) return rope_types<float>(x, y, pos, pos_type, a, st);
+    if (dtype == SUHPE_BF16) return rope_types<bf16>(x, y, pos, pos_type, a, st);
+    return rope_types<f16>(x, y, pos, pos_type, a, st);
+}
+
+int suhpe_dropout_apply(const void* x, int dtype, int64_t count, float keep, const uint64_t* counter, uint64_t position, const void* skip, void* y, suhpe_stream_t stream) {
+    SUHPE_REQUIRE(dtype_ok(dtype), "suhpe_dropout_apply: unknown dtype %d", dtype);
+    SUHPE_REQUIRE(keep >= 0.f && keep <= 1.f, "suhpe_dropout_apply: keep %g outside [0, 1]", (double)keep);
+    SUHPE_REQUIRE(count >= 0, "suhpe_dropout_apply: negative count");
+    if (count == 0) return SUHPE_OK;
+    SUHPE_REQUIRE(x && y && counter, "suhpe_dropout_apply: null pointer");
+    // r < keep for r = k / 2^24, k a 24-bit integer  <=>  k < ceil(keep 2^24): the product is exact in double
+    const double scaled = (double)keep * 16777216.0;
+    uint32_t bound = (uint32_t)scaled;
+    if ((double)bound < scaled) ++bound;
+    const float scale = keep > 0.f ? 1.f / keep : 0.f;
+    hipStream_t st = as_stream(stream);
+    if (dtype == SUHPE_F32) return dropout_launch<float>(x, skip, y, count, bound, scale, counter, position, st);
+    if (dtype == SUHPE_BF16) return dropout_launch<bf16>(x, skip, y, count, bound, scale, counter, position, st);
+    return dropout_launch<f16>(x, skip, y, count, bound, scale, counter, position, st);
+}
+
+int suhpe_dropout_advance(uint64_t* counter, uint64_t by, suhpe_stream_t stream) {
+    SUHPE_REQUIRE(counter, "suhpe_dropout_advance: null pointer");
+    hipLaunchKernelGGL(dropout_advance_kernel, dim3(1), dim3(1), 0, as_stream(stream), counter, by);
+    return check_launch("suhpe_dropout_advance");
+}
+
+int suhpe_layernorm16_fwd(const void* x, int dtype, int64_t rows, int c, float eps, const float* gamma, const float* beta, void* y, float* mean, float* rstd,
+                          suhpe_stream_t stream) {
+    SUHPE_REQUIRE(dtype == SUHPE_BF16 || dtype == SUHPE_F16, "suhpe_layernorm16_fwd: 16-bit rows only (fp32: suhpe_layernorm_fwd)");
+    SUHPE_REQUIRE(rows >= 0 && c > 0 && rows <= 0x7fffffffll, "suhpe_layernorm16_fwd: bad sizes");
+    if (rows == 0) return SUHPE_OK;
+    SUHPE_REQUIRE(x && y && mean && rstd, "suhpe_layernorm16_fwd: null pointer");
+    if (dtype == SUHPE_BF16) return ln16_fwd<bf16>(x, rows, c, eps, gamma, beta, y, mean, rstd, as_stream(stream));
+    return ln16_fwd<f16>(x, rows, c, eps, gamma, beta, y, mean, rstd, as_stream(stream));
+}
+
+int64_t suhpe_layernorm16_bwd_workspace_bytes(int c) { return (int64_t)kLnBlocks * 2 * c * (int64_t)sizeof(float); }
+
+int suhpe_layernorm16_bwd(const void* x, const void* dy, int dtype, int64_t rows, int c, const float* mean, const float* rstd, const float* gamma, const void* skip, void* dx,
+                          float* dgamma, float* dbeta, int accumulate, void* workspace, int64_t workspace_bytes, suhpe_stream_t stream) {
+    SUHPE_REQUIRE(dtype == SUHPE_BF16 || dtype == SUHPE_F16, "suhpe_layernorm16_bwd: 16-bit rows only (fp32: suhpe_layernorm_bwd)");
+    SUHPE_REQUIRE(rows >= 0 && c > 0 && rows <= 0x7fffffffll, "suhpe_layernorm16_bwd: bad sizes");
+    SUHPE_REQUIRE(rows == 0 || (x && dy && dx && mean && rstd), "suhpe_layernorm16_bwd: null pointer");
+    if (dgamma || dbeta) {
+        SUHPE_REQUIRE(workspace, "suhpe_layernorm16_bwd: null workspace");
+        if (workspace_bytes < suhpe_layernorm16_bwd_workspace_bytes(c)) {
+            set_error("suhpe_layernorm16_bwd: workspace of %lld bytes, needs %lld", (long long)workspace_bytes, (long long)suhpe_layernorm16_bwd_workspace_bytes(c));
+            return SUHPE_EWORKSPACE;
+        }
+    }
+    float* part = static_cast<float*>(workspace);
+    if (dtype == SUHPE_BF16) return ln16_bwd<bf16>(x, dy, rows, c, mean, rstd, gamma, skip, dx, dgamma, dbeta, accumulate, part, as_stream(stream));
+    return ln16_bwd<f16>(x, dy, rows, c, mean, rstd, gamma, skip, dx, dgamma, dbeta, accumulate, part, as_stream(stream));
+}
+
+}  // extern "C"

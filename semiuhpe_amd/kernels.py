@@ -7,6 +7,7 @@ Conv filters keep torch's logical shape (Cout, Cin/g, R, S) in channels_last mem
 [Cout][R][S][Cin/g].
 """
 import ctypes
+import math
 import os
 import json
 
@@ -1184,6 +1185,9 @@ def bn_act_bwd(x, dy, c, mean, rstd, gamma, beta, act, train_stats, dgamma=None,
 
 @_memop
 def layernorm_fwd(x, c, eps, gamma, beta):
+    """y (x's type), mean, rstd (fp32) of rows of c; fp32, bf16 or fp16 rows, gamma and beta fp32"""
+    if x.dtype in _LOWP:
+        return _layernorm16_fwd(x, c, eps, gamma, beta)
     _chk(x, "x")
     rows = x.numel() // c
     y = torch.empty_like(x)
@@ -1195,7 +1199,10 @@ def layernorm_fwd(x, c, eps, gamma, beta):
 
 @_memop
 def layernorm_bwd(x, dy, c, mean, rstd, gamma, dgamma=None, dbeta=None, accumulate=False, skip=None):
-    """skip: a tensor of x's shape added to dx (the gradient that bypassed the normalised sub-block through its residual connection)"""
+    """skip: a tensor of x's shape added to dx (the gradient that bypassed the normalised sub-block through its residual connection).
+    x, dy, skip and dx share a type (fp32, bf16 or fp16); gamma, mean, rstd, dgamma and dbeta are fp32"""
+    if x.dtype in _LOWP:
+        return _layernorm16_bwd(x, dy, c, mean, rstd, gamma, dgamma, dbeta, accumulate, skip)
     _chk(x, "x"); _chk(dy, "dy"); _chk(skip, "skip")
     dx = torch.empty_like(x)
     assert skip is None or skip.numel() == x.numel()
@@ -1614,6 +1621,244 @@ def window_attn_bwd_rs(qkv, out, stats, dout, bias_table, bias_idx, B, H, W, ws,
         ws2 = workspace("attn_dbias", lib.suhpe_window_attn_dbias_workspace_bytes(ws, heads), qkv.device)
         call("suhpe_window_attn_dbias", ptr(ws_buf), ptr(inverse[0]), ptr(inverse[1]), B, H, W, ws, heads, noff, ptr(dbias), ptr(ws2))
     return dqkv
+
+
+# ---------------------------------------------------------------------------------------------- operators of transformer blocks
+# Rotary positions, gated feed-forward block, dropout without a stored mask, 16-bit LayerNorm: fp32, bf16 or fp16 tensors (LayerNorm's 16-bit form is
+# reached through layernorm_fwd / layernorm_bwd).  Launches go to the current stream of the TENSORS' device; scratch comes from the caching allocator
+# (inside a graph capture: from that graph's own pool), so calls on several streams and captured graphs share none.
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_LOWP = (torch.bfloat16, torch.float16)
+
+
+def _chk_tok(t, name, dtype=None, device=None, shape=None):
+    """contiguous fp32 / bf16 / fp16 tensor on the HIP device (None passes)"""
+    if t is None:
+        return
+    if not torch.is_tensor(t):
+        raise ValueError(f"{name}: expected a tensor, got {type(t).__name__}")
+    if not t.is_cuda:
+        _lib.require_gpu()
+        raise RuntimeError(f"semiuhpe_amd: {name} must live on the HIP device (got {t.device}); there is no CPU path")
+    if t.dtype not in _DTYPES:
+        raise ValueError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{name}: expected {dtype}, got {t.dtype}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous tensor, got strides {t.stride()} for shape {tuple(t.shape)}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name}: on {t.device}, the other tensors on {device}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+
+
+def _overlap(a, b):
+    """do the two contiguous tensors share memory without being the same range?"""
+    a0, b0, na, nb = a.data_ptr(), b.data_ptr(), a.numel() * a.element_size(), b.numel() * b.element_size()
+    return na > 0 and nb > 0 and a0 < b0 + nb and b0 < a0 + na and (a0, na) != (b0, nb)
+
+
+def _call_on(device, name, *args):
+    """_lib.call with `device` current: the launch goes to that device's current stream"""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return call(name, *args)
+    with torch.cuda.device(device):
+        return call(name, *args)
+
+
+def _scratch(nbytes, device):
+    return torch.empty(int(nbytes), dtype=torch.uint8, device=device) if nbytes > 0 else None
+
+
+def _layernorm16_fwd(x, c, eps, gamma, beta):
+    _chk_tok(x, "x")
+    _chk_tok(gamma, "gamma", torch.float32, x.device, (c,)); _chk_tok(beta, "beta", torch.float32, x.device, (c,))
+    if c < 1 or x.dim() == 0 or x.shape[-1] != c:
+        raise ValueError(f"x: expected rows of {c}, got shape {tuple(x.shape)}")
+    rows = x.numel() // c
+    y = torch.empty_like(x)
+    mean = torch.empty(rows, dtype=torch.float32, device=x.device)
+    rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
+    _call_on(x.device, "suhpe_layernorm16_fwd", ptr(x), _DTYPES[x.dtype], rows, c, float(eps), ptr(gamma), ptr(beta), ptr(y), ptr(mean), ptr(rstd))
+    return y, mean, rstd
+
+
+def _layernorm16_bwd(x, dy, c, mean, rstd, gamma, dgamma, dbeta, accumulate, skip):
+    _chk_tok(x, "x")
+    if c < 1 or x.dim() == 0 or x.shape[-1] != c:
+        raise ValueError(f"x: expected rows of {c}, got shape {tuple(x.shape)}")
+    rows = x.numel() // c
+    _chk_tok(dy, "dy", x.dtype, x.device, x.shape); _chk_tok(skip, "skip", x.dtype, x.device, x.shape)
+    for t, name, n in ((mean, "mean", rows), (rstd, "rstd", rows), (gamma, "gamma", c), (dgamma, "dgamma", c), (dbeta, "dbeta", c)):
+        _chk_tok(t, name, torch.float32, x.device, (n,))
+    dx = torch.empty_like(x)
+    nbytes = _lib.load().suhpe_layernorm16_bwd_workspace_bytes(c) if dgamma is not None or dbeta is not None else 0
+    ws = _scratch(nbytes, x.device)
+    _call_on(x.device, "suhpe_layernorm16_bwd", ptr(x), ptr(dy), _DTYPES[x.dtype], rows, c, ptr(mean), ptr(rstd), ptr(gamma), ptr(skip), ptr(dx), ptr(dgamma),
+             ptr(dbeta), int(accumulate), ptr(ws), nbytes)
+    return dx
+
+
+class RopeAxes:
+    """The plan of rope_axes: `axes` gives the rotated channels of each position axis (even numbers, together at most dh), in the order of the columns of
+    the positions, e.g. (16, 16) for (row, column) of an image's tokens or (32, 48, 48) for (frame, row, column) of a clip's.  Pair j of an axis of width
+    w turns by position * theta^(-2 j / w).  layout "halves": pair p of a head = channels (p, p + pairs), "adjacent": (2 p, 2 p + 1); channels beyond
+    sum(axes) are not rotated."""
+
+    def __init__(self, dh, axes, theta=10000.0, layout="halves", device="cuda"):
+        axes = [int(w) for w in axes]
+        if not axes or any(w < 0 or w % 2 for w in axes) or not 0 < sum(axes) <= dh:
+            raise ValueError(f"axes {axes}: even widths that add up to 2 .. {dh} channels")
+        if layout not in ("halves", "adjacent"):
+            raise ValueError(f"layout {layout!r}: 'halves' or 'adjacent'")
+        if not theta > 0:
+            raise ValueError(f"theta {theta}: a positive number")
+        self.dh, self.axes, self.theta, self.layout, self.pairs = int(dh), tuple(axes), float(theta), layout, sum(axes) // 2
+        turns = [self.theta ** (-2.0 * j / w) / (2.0 * math.pi) for w in axes for j in range(w // 2)]
+        self.freq = torch.tensor(turns, dtype=torch.float64, device=device)          # revolutions per unit of position
+        self.axis = torch.tensor([a for a, w in enumerate(axes) for _ in range(w // 2)], dtype=torch.int32, device=device)
+
+
+_POS_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+
+
+@_memop
+def rope_axes(x, pos, plan, heads, parts=1, rotated=None, inverse=False, out=None):
+    """x (..., heads * parts * dh): every head's parts 0 .. rotated - 1 (default: all) rotated by the positions pos (rows, axes) (int32, int64 or float32); parts=3,
+    rotated=2 for packed qkv rows.  inverse=True turns back: the gradient.  out=x works in place and touches the rotated channels only."""
+    _chk_tok(x, "x")
+    rotated = parts if rotated is None else rotated
+    if heads < 1 or parts < 1 or not 1 <= rotated <= parts:
+        raise ValueError(f"heads {heads}, parts {parts}, rotated {rotated}: 1 <= rotated <= parts")
+    width = heads * parts * plan.dh
+    if x.dim() == 0 or x.shape[-1] != width:
+        raise ValueError(f"x: expected rows of {heads} heads * {parts} parts * {plan.dh} = {width}, got shape {tuple(x.shape)}")
+    rows = x.numel() // width
+    if not torch.is_tensor(pos) or pos.dtype not in _POS_TYPES:
+        raise ValueError("pos: an int32, int64 or float32 tensor")
+    if tuple(pos.shape) != (rows, len(plan.axes)) or not pos.is_contiguous():
+        raise ValueError(f"pos: expected a contiguous tensor of shape {(rows, len(plan.axes))}, got {tuple(pos.shape)}")
+    if pos.device != x.device or plan.freq.device != x.device:
+        raise ValueError(f"x on {x.device}, pos on {pos.device}, plan on {plan.freq.device}")
+    if out is None:
+        out = torch.empty_like(x)
+    else:
+        _chk_tok(out, "out", x.dtype, x.device, x.shape)
+        if _overlap(x, out):
+            raise ValueError("out: x itself or a tensor that shares no memory with it")
+    _call_on(x.device, "suhpe_rope_axes", ptr(x), _DTYPES[x.dtype], rows, heads, parts, rotated, plan.dh, ptr(pos), _POS_TYPES[pos.dtype], len(plan.axes),
+             ptr(plan.freq), ptr(plan.axis), plan.pairs, int(plan.layout == "halves"), int(inverse), ptr(out))
+    return out
+
+
+@_memop
+def dropout_apply(x, keep, counter, position, skip=None, out=None):
+    """[skip +] x / keep where the generator keeps the element, 0 where it drops it: the values of x * mask with the mask that dropout_mask would draw from
+    `counter` (device int64 pair: seed, offset) at `position`, without storing it.  The gradient is dropout_apply(dy, keep, counter, position).
+    Uses (x.numel() + 3) // 4 positions.  out: may be x or skip."""
+    _chk_tok(x, "x")
+    _chk_tok(skip, "skip", x.dtype, x.device, x.shape)
+    if not 0.0 <= keep <= 1.0:
+        raise ValueError(f"keep {keep}: a probability")
+    if not torch.is_tensor(counter) or counter.dtype != torch.int64 or tuple(counter.shape) != (2,) or not counter.is_contiguous() or counter.device != x.device:
+        raise ValueError(f"counter: an int64 pair (seed, offset) on {x.device}")
+    if position < 0:
+        raise ValueError(f"position {position}: not negative")
+    if out is None:
+        out = torch.empty_like(x)
+    else:
+        _chk_tok(out, "out", x.dtype, x.device, x.shape)
+        if _overlap(x, out) or (skip is not None and _overlap(skip, out)):
+            raise ValueError("out: x or skip itself, or a tensor that shares no memory with them")
+    _call_on(x.device, "suhpe_dropout_apply", ptr(x), _DTYPES[x.dtype], x.numel(), float(keep), ptr(counter), int(position), ptr(skip), ptr(out))
+    return out
+
+
+def dropout_fwd(x, keep, skip=None):
+    """dropout_apply at the running position of x.device's generator (the one that dropout_mask draws from) -> (y, draw); dropout_bwd(dy, draw) is the gradient"""
+    _chk_tok(x, "x")
+    ctr = rng_counter(x.device)
+    key = torch.device(x.device)
+    draw = (ctr, _host_offsets[key], float(keep))
+    y = dropout_apply(x, keep, ctr, draw[1], skip=skip)
+    _host_offsets[key] += (x.numel() + 3) // 4
+    return y, draw
+
+
+def dropout_bwd(dy, draw):
+    ctr, position, keep = draw
+    return dropout_apply(dy, keep, ctr, position)
+
+
+def dropout_advance(counter, by):
+    """move `counter` on by `by` positions on the device: at the end of a captured graph that draws, so that every replay draws fresh numbers"""
+    if not torch.is_tensor(counter) or not counter.is_cuda or counter.dtype != torch.int64 or tuple(counter.shape) != (2,) or not counter.is_contiguous():
+        raise ValueError("counter: an int64 pair (seed, offset) on the HIP device")
+    if by < 0:
+        raise ValueError(f"by {by}: not negative")
+    _call_on(counter.device, "suhpe_dropout_advance", ptr(counter), int(by))
+
+
+def _ffn_sizes(x, wg, wu, wd, act):
+    _chk_tok(x, "x")
+    if act not in ACT:
+        raise ValueError(f"act {act!r}: one of {sorted(k for k in ACT if k)}")
+    for t, name in ((wg, "wg"), (wu, "wu"), (wd, "wd")):
+        _chk_tok(t, name, x.dtype, x.device)
+        if t is None or t.dim() != 2:
+            raise ValueError(f"{name}: expected a matrix")
+    n, k = wg.shape
+    o = wd.shape[0]
+    if tuple(wu.shape) != (n, k) or wd.shape[1] != n or min(n, k, o) < 1:
+        raise ValueError(f"wg {tuple(wg.shape)}, wu {tuple(wu.shape)}, wd {tuple(wd.shape)}: expected (n, k), (n, k), (o, n)")
+    if x.dim() == 0 or x.shape[-1] != k:
+        raise ValueError(f"x: expected rows of {k}, got shape {tuple(x.shape)}")
+    return x.numel() // k, k, n, o
+
+
+@_memop
+def gated_ffn_fwd(x, wg, wu, wd, bg=None, bu=None, bd=None, act="silu", save=True):
+    """The gated feed-forward block y = (act(x wg^T + bg) * (x wu^T + bu)) wd^T + bd: x (..., k), wg and wu (n, k), wd (o, n) -> y (..., o) and, with save=True, what
+    gated_ffn_bwd needs (g, u, h: both projections and the product, each rounded to x's type once), else None."""
+    m, k, n, o = _ffn_sizes(x, wg, wu, wd, act)
+    for t, name, c in ((bg, "bg", n), (bu, "bu", n), (bd, "bd", o)):
+        _chk_tok(t, name, x.dtype, x.device, (c,))
+    y = torch.empty(x.shape[:-1] + (o,), dtype=x.dtype, device=x.device)
+    h = torch.empty((m, n), dtype=x.dtype, device=x.device)
+    g, u = (torch.empty_like(h), torch.empty_like(h)) if save else (None, None)
+    nbytes = _lib.load().suhpe_gated_ffn_fwd_workspace_bytes(_DTYPES[x.dtype], m, k, n, o)
+    ws = _scratch(nbytes, x.device)
+    _call_on(x.device, "suhpe_gated_ffn_fwd", _DTYPES[x.dtype], ACT[act], m, k, n, o, ptr(x), ptr(wg), ptr(wu), ptr(wd), ptr(bg), ptr(bu), ptr(bd), ptr(g), ptr(u), ptr(h),
+             ptr(y), ptr(ws), nbytes)
+    return y, ((g, u, h) if save else None)
+
+
+@_memop
+def gated_ffn_bwd(dy, x, wg, wu, wd, saved, act="silu", dwg=None, dwu=None, dwd=None, dbg=None, dbu=None, dbd=None, accumulate=False, need_dx=True):
+    """-> dx (None with need_dx=False); writes the gradients it is given buffers for (added to what they hold with accumulate=True): dwg, dwu, dwd together, each of
+    dbg, dbu, dbd by itself, all of x's type or all fp32.  `saved`: what gated_ffn_fwd(save=True) returned for this x."""
+    m, k, n, o = _ffn_sizes(x, wg, wu, wd, act)
+    _chk_tok(dy, "dy", x.dtype, x.device, x.shape[:-1] + (o,))
+    if saved is None:
+        raise ValueError("saved: the forward ran with save=False")
+    for t, name in zip(saved, ("g", "u", "h")):
+        _chk_tok(t, name, x.dtype, x.device, (m, n))
+    if len({t is None for t in (dwg, dwu, dwd)}) != 1:
+        raise ValueError("dwg, dwu, dwd: all three or none")
+    grads = [(dwg, "dwg", (n, k)), (dwu, "dwu", (n, k)), (dwd, "dwd", (o, n)), (dbg, "dbg", (n,)), (dbu, "dbu", (n,)), (dbd, "dbd", (o,))]
+    types = {t.dtype for t, _, _ in grads if t is not None} or {x.dtype}
+    gtype = next(iter(types))
+    if len(types) != 1 or gtype not in (x.dtype, torch.float32):
+        raise ValueError(f"gradients: all {x.dtype} or all float32")
+    for t, name, shape in grads:
+        _chk_tok(t, name, gtype, x.device, shape)
+    dx = torch.empty_like(x) if need_dx else None
+    nbytes = _lib.load().suhpe_gated_ffn_bwd_workspace_bytes(_DTYPES[x.dtype], m, k, n, o)
+    ws = _scratch(nbytes, x.device)
+    g, u, h = saved
+    _call_on(x.device, "suhpe_gated_ffn_bwd", _DTYPES[x.dtype], ACT[act], m, k, n, o, ptr(dy), ptr(x), ptr(wg), ptr(wu), ptr(wd), ptr(g), ptr(u), ptr(h), ptr(dx),
+             ptr(dwg), ptr(dwu), ptr(dwd), ptr(dbg), ptr(dbu), ptr(dbd), _DTYPES[gtype], int(accumulate), ptr(ws), nbytes)
+    return dx
 
 
 # ---------------------------------------------------------------------------------------------- optimiser
