@@ -1,118 +1,312 @@
 // Gated feed-forward block (forward and backward) in fp32 / bf16 / fp16:
 //   g = x Wg^T + bg, u = x Wu^T + bu, h = act(g) u, y = h Wd^T + bd
 //   dh = dy Wd, dg = dh u act'(g), du = dh act(g), dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, dWd = dy^T h, db = column sums
+//
+// Forward, two products: [g | u] with the activation and the product in the epilogue (a tile takes the SAME columns of Wg and Wu, so both factors of an
+// output element meet in one lane's registers), then y.  Backward, four: dh whose epilogue turns it into dg and du at once (dh itself is never stored),
+// dx as one product over two ranges of n, dWg and dWu in one launch, dWd.  g, u and h are rounded to the tensors' type once on their way to memory (they are
+// operands of 16-bit matrix instructions next); every sum runs in fp32.
 #include "lowp.h"
+#include "gemm_lowp.inl"
 
 namespace suhpe {
 namespace {
 
-// One operand of a product over k: element (row, k) at p[row * rs + k * ks]
-struct View { const void* p; int64_t rs, ks; };
+// ------------------------------------------------------------------------------------------ few rows (serving)
+// At most 16 MT rows: the weights are the traffic, each is read once, straight from memory into the matrix instructions' registers.  A workgroup takes 16 rows of the
+// weights (GATE: of both) and its W wavefronts split k; their sums meet in LDS in a fixed order.  Rows may start at any element: 16-byte loads from any
+// address, and the end of a row whose length no vector divides is read element by element.
+template <typename T> __device__ __forceinline__ i32x4 load_k(const T* row, int64_t k, int64_t K) {
+    constexpr int CH = 16 / sizeof(T);
+    i32x4 v = {0, 0, 0, 0};
+    if (k + CH <= K) {
+        __builtin_memcpy(&v, row + k, 16);
+    } else if (k < K) {
+        T e[CH];
+#pragma unroll
+        for (int i = 0; i < CH; ++i) e[i] = k + i < K ? row[k + i] : (T)0.f;
+        __builtin_memcpy(&v, e, 16);
+    }
+    return v;
+}
 
-// out[m][j] = sum_k A[m][k] B[j][k], 64 x 64 outputs per block, 4 x 4 per thread, sums in fp32
-enum { EPI_STORE = 0, EPI_GATE = 1, EPI_GATE_BWD = 2 };
-template <typename T, typename O, int EPI>
-__global__ __launch_bounds__(256) void ffn_product_simple(View a, View b, View a2, View b2, int64_t M, int N, int64_t K, int64_t K2, const T* bias, const T* bias2, int act,
-                                                          const T* gin, const T* uin, T* gout, T* uout, O* out, int accumulate) {
-    __shared__ float As[16][65], Bs[16][65], Cs[EPI == EPI_GATE ? 16 : 1][65];
-    const int t = threadIdx.x, tm = t & 15, tn = t >> 4;
-    const int64_t m0 = (int64_t)blockIdx.x * 64;
-    const int n0 = blockIdx.y * 64;
-    float acc[4][4] = {}, acc2[4][4] = {};
-    const int64_t kpad = (K + 15) / 16 * 16;
-    for (int64_t k0 = 0; k0 < kpad + K2; k0 += 16) {
-        const bool second = k0 >= kpad;
-        const View& A = second ? a2 : a;
-        const View& B = second ? b2 : b;
-        const int64_t kb = second ? k0 - kpad : k0, ke = second ? K2 : K;
+template <typename T, int MT, int W, bool GATE>
+__global__ __launch_bounds__(64 * W) void ffn_few_rows(const T* __restrict__ x, int M, int64_t K, const T* __restrict__ w, const T* __restrict__ w2, int N, const T* __restrict__ bias,
+                                                       const T* __restrict__ bias2, int act, T* __restrict__ gout, T* __restrict__ uout, T* __restrict__ out) {
+    constexpr int KE = 64 / (int)sizeof(T), CH = 16 / (int)sizeof(T), S = GATE ? 2 : 1;      // k of one matrix step
+    __shared__ f32x4 sums[W][S][MT][64];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, t = lane & 15, g = lane >> 4;
+    const int n0 = blockIdx.x * 16, nr = n0 + t < N ? n0 + t : N - 1;
+    const T *r1 = w + nr * K, *r2 = GATE ? w2 + nr * K : nullptr;
+    const T* xr[MT];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int e = t + 256 * i, kk = e & 15, r = e >> 4;
-            const int64_t k = kb + kk;
-            As[kk][r] = (m0 + r < M && k < ke) ? (float)static_cast<const T*>(A.p)[(m0 + r) * A.rs + k * A.ks] : 0.f;
-            Bs[kk][r] = (n0 + r < N && k < ke) ? (float)static_cast<const T*>(B.p)[(n0 + r) * B.rs + k * B.ks] : 0.f;
-            if (EPI == EPI_GATE) Cs[kk][r] = (n0 + r < N && k < ke) ? (float)static_cast<const T*>(b2.p)[(n0 + r) * b2.rs + k * b2.ks] : 0.f;
+    for (int i = 0; i < MT; ++i) xr[i] = x + (int64_t)(16 * i + t < M ? 16 * i + t : M - 1) * K;
+    const int64_t steps = (K + KE - 1) / KE, lo = steps * wave / W, hi = steps * (wave + 1) / W;
+    f32x4 acc[S][MT];
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[s][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    constexpr int U = MT > 2 ? 2 : 4;
+    for (int64_t q = lo; q < hi; q += U) {
+        i32x4 a[U][S], b[U][MT];
+#pragma unroll
+        for (int v = 0; v < U; ++v) {
+            const int64_t k = q + v < hi ? (q + v) * KE + g * CH : K;      // (steps past the slice read nothing: zeros)
+            a[v][0] = load_k(r1, k, K);
+            if constexpr (GATE) a[v][1] = load_k(r2, k, K);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) b[v][i] = load_k(xr[i], k, K);
         }
-        __syncthreads();
-        for (int kk = 0; kk < 16; ++kk)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+        for (int v = 0; v < U; ++v)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    acc[i][j] += As[kk][tm + 16 * i] * Bs[kk][tn + 16 * j];
-                    if (EPI == EPI_GATE) acc2[i][j] += As[kk][tm + 16 * i] * Cs[kk][tn + 16 * j];
-                }
-        __syncthreads();
+            for (int s = 0; s < S; ++s)
+#pragma unroll
+                for (int i = 0; i < MT; ++i) acc[s][i] = Mfma<T>::run(a[v][s], b[v][i], acc[s][i]);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int s = 0; s < S; ++s)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t m = m0 + tm + 16 * i;
-            const int n = n0 + tn + 16 * j;
-            if (m >= M || n >= N) continue;
-            const int64_t at = m * N + n;
-            if constexpr (EPI == EPI_GATE) {
-                const float g = acc[i][j] + (bias ? (float)bias[n] : 0.f), u = acc2[i][j] + (bias2 ? (float)bias2[n] : 0.f);
-                if (gout) { gout[at] = (T)g; uout[at] = (T)u; }
-                out[at] = (O)(act_apply(g, act) * u);
-            } else if constexpr (EPI == EPI_GATE_BWD) {
-                const float g = (float)gin[at], u = (float)uin[at];
-                gout[at] = (T)(acc[i][j] * u * act_grad(g, act));
-                uout[at] = (T)(acc[i][j] * act_apply(g, act));
-            } else {
-                float v = acc[i][j] + (bias ? (float)bias[n] : 0.f);
-                if (accumulate) v += (float)out[at];
-                out[at] = (O)v;
-            }
+        for (int i = 0; i < MT; ++i) sums[wave][s][i][lane] = acc[s][i];
+    __syncthreads();
+    if (wave >= MT) return;
+    f32x4 total[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        total[s] = sums[0][s][wave][lane];
+#pragma unroll
+        for (int v = 1; v < W; ++v) total[s] += sums[v][s][wave][lane];
+    }
+    const int m = 16 * wave + t, n = n0 + 4 * g;
+    if (m >= M) return;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        if (n + r >= N) break;
+        const int64_t at = (int64_t)m * N + n + r;
+        const float v = total[0][r] + (bias ? (float)bias[n + r] : 0.f);
+        if constexpr (GATE) {
+            const float u = total[1][r] + (bias2 ? (float)bias2[n + r] : 0.f);
+            if (gout) { gout[at] = (T)v; uout[at] = (T)u; }
+            out[at] = (T)(act_apply(v, act) * u);
+        } else {
+            out[at] = (T)v;
         }
+    }
 }
 
-template <typename T, typename O>
-__global__ __launch_bounds__(256) void ffn_column_sum_simple(const T* x, int64_t rows, int c, O* out, int accumulate) {
-    const int j = blockIdx.x * 256 + threadIdx.x;
-    if (j >= c) return;
-    float s = 0.f;
-    for (int64_t r = 0; r < rows; ++r) s += (float)x[r * c + j];
-    out[j] = (O)(accumulate ? (float)out[j] + s : s);
+constexpr int kFewRows = 32;
+
+template <typename T, bool GATE>
+void few_rows(const T* x, int M, int64_t K, const T* w, const T* w2, int N, const T* bias, const T* bias2, int act, T* g, T* u, T* out, hipStream_t st) {
+    const dim3 grid((unsigned)ceil_div(N, 16));
+    constexpr int W = GATE ? 8 : 16;                                   // (both weights in flight need the registers of 8 wavefronts)
+    if (M <= 16) hipLaunchKernelGGL((ffn_few_rows<T, 1, W, GATE>), grid, dim3(64 * W), 0, st, x, M, K, w, w2, N, bias, bias2, act, g, u, out);
+    else hipLaunchKernelGGL((ffn_few_rows<T, 2, W, GATE>), grid, dim3(64 * W), 0, st, x, M, K, w, w2, N, bias, bias2, act, g, u, out);
 }
 
-inline dim3 tiles(int64_t M, int N) { return dim3((unsigned)ceil_div(M, 64), (unsigned)ceil_div(N, 64)); }
+// ------------------------------------------------------------------------------------------ column sums (bias gradients)
+// up to three matrices in one launch (grid z); part: [job][row block][columns], finished in a fixed order
+struct ColumnJobs { const void* x[3]; int64_t ld[3]; int c[3]; void* out[3]; float* part[3]; int jobs; };
+constexpr int kColBlocks = 256;
 
 template <typename T>
-int ffn_fwd(int act, int64_t m, int k, int n, int o, const void* x, const void* wg, const void* wu, const void* wd, const void* bg, const void* bu, const void* bd, void* g,
-            void* u, void* h, void* y, hipStream_t st) {
+__global__ __launch_bounds__(256) void column_sums(const ColumnJobs q, int64_t rows, int64_t rows_per_block) {
+    __shared__ float lds[4][256];
+    const int job = blockIdx.z, c = q.c[job], lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = blockIdx.y * 256 + lane * 4;
+    if ((int)blockIdx.y * 256 >= c) return;
+    const T* x = static_cast<const T*>(q.x[job]);
+    const int64_t ld = q.ld[job], r0 = (int64_t)blockIdx.x * rows_per_block, r1 = r0 + rows_per_block < rows ? r0 + rows_per_block : rows;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    const bool vec = (ld & 3) == 0 && j + 4 <= c && (reinterpret_cast<uintptr_t>(x) & (4 * sizeof(T) - 1)) == 0;
+    for (int64_t r = r0 + wave; r < r1; r += 4) {
+        float v[4];
+        if (vec) load_n<T, 4>(x + r * ld + j, v);
+        else
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = j + e < c ? (float)x[r * ld + j + e] : 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] += v[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) lds[wave][lane * 4 + e] = s[e];
+    __syncthreads();
+    const int jj = blockIdx.y * 256 + threadIdx.x;
+    if (jj < c) q.part[job][(int64_t)blockIdx.x * c + jj] = (lds[0][threadIdx.x] + lds[1][threadIdx.x]) + (lds[2][threadIdx.x] + lds[3][threadIdx.x]);
+}
+
+template <typename O>
+__global__ __launch_bounds__(256) void column_sums_finish(const ColumnJobs q, int blocks, int accumulate) {
+    __shared__ float lds[16][17];
+    const int job = blockIdx.z, c = q.c[job], col = threadIdx.x & 15, slice = threadIdx.x >> 4, j = blockIdx.x * 16 + col;
+    if ((int)blockIdx.x * 16 >= c) return;
+    float s = 0.f;
+    if (j < c)
+        for (int b = slice; b < blocks; b += 16) s += q.part[job][(int64_t)b * c + j];
+    lds[slice][col] = s;
+    __syncthreads();
+    if (slice == 0 && j < c) {
+        float t = 0.f;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) t += lds[k][col];
+        O* out = static_cast<O*>(q.out[job]);
+        out[j] = (O)(accumulate ? (float)out[j] + t : t);
+    }
+}
+
+// ------------------------------------------------------------------------------------------ workspaces
+// Pieces of a call's workspace, laid out in one order by the size query and by the call
+struct Space {
+    char* base;
+    int64_t used = 0;
+    void* take(int64_t bytes) {
+        void* p = base ? base + used : nullptr;
+        used += ceil_div(bytes, 256) * 256;
+        return p;
+    }
+};
+struct Dims {
+    int64_t m;
+    int k, n, o, es;
+    int ch() const { return 16 / es; }
+    int pad(int c) const { return (int)ceil_div(c, ch()) * ch(); }
+    bool odd(int c) const { return c % ch() != 0; }
+    int64_t steps(int64_t c) const { return ceil_div(c, 128 / es); }
+    void* copy(Space& s, int64_t rows, int c) const { return odd(c) ? s.take(rows * pad(c) * es) : nullptr; }
+};
+inline int64_t part_bytes(const Plan& q, int64_t M, int64_t N, int problems) { return q.splits > 1 ? (int64_t)q.splits * M * N * 4 * problems : 0; }
+
+struct FwdSpace {
+    void *xp, *gp, *up, *hp, *dp;
+    float* part;
+    Plan gate, down;
+    FwdSpace(const Dims& d, Space& s) : gate(plan_gemm(d.m, 2 * (int64_t)d.n, d.steps(d.k), 1, false)), down(plan_gemm(d.m, d.o, d.steps(d.n), 1, true)) {
+        xp = d.copy(s, d.m, d.k); gp = d.copy(s, d.n, d.k); up = d.copy(s, d.n, d.k); hp = d.copy(s, d.m, d.n); dp = d.copy(s, d.o, d.n);
+        part = static_cast<float*>(s.take(part_bytes(down, d.m, d.o, 1)));
+    }
+};
+struct BwdSpace {
+    void *dg, *du, *xp, *gp, *up, *hp, *dp, *yp;
+    float *part, *cols[3];
+    Plan gate, dx, dw, dwd;
+    BwdSpace(const Dims& d, Space& s)
+        : gate(plan_gemm(d.m, d.n, d.steps(d.o), 1, false)), dx(plan_gemm(d.m, d.k, 2 * d.steps(d.n), 1, true)), dw(plan_gemm(d.n, d.k, d.steps(d.m), 2, true)),
+          dwd(plan_gemm(d.o, d.n, d.steps(d.m), 1, true)) {
+        dg = s.take(d.m * d.pad(d.n) * d.es);
+        du = s.take(d.m * d.pad(d.n) * d.es);
+        xp = d.copy(s, d.m, d.k); gp = d.copy(s, d.n, d.k); up = d.copy(s, d.n, d.k); hp = d.copy(s, d.m, d.n); dp = d.copy(s, d.o, d.n); yp = d.copy(s, d.m, d.o);
+        int64_t most = part_bytes(dx, d.m, d.k, 1);
+        if (part_bytes(dw, d.n, d.k, 2) > most) most = part_bytes(dw, d.n, d.k, 2);
+        if (part_bytes(dwd, d.o, d.n, 1) > most) most = part_bytes(dwd, d.o, d.n, 1);
+        part = static_cast<float*>(s.take(most));
+        for (int i = 0; i < 3; ++i) cols[i] = static_cast<float*>(s.take((int64_t)kColBlocks * (i < 2 ? d.n : d.o) * 4));
+    }
+};
+
+// the operand itself, or its copy with rows of whole 16-byte chunks
+template <typename T> const char* rows_of(const void* p, void* copy, int64_t rows, int c, const Dims& d, hipStream_t st) {
+    if (!copy) return static_cast<const char*>(p);
+    const int cp = d.pad(c);
+    hipLaunchKernelGGL((pad_rows<T>), dim3(grid_for(rows * (cp / d.ch()), 256)), dim3(256), 0, st, static_cast<const T*>(p), rows, c, cp, static_cast<T*>(copy));
+    return static_cast<const char*>(copy);
+}
+
+template <typename O> __global__ __launch_bounds__(256) void ffn_zero(O* p, int64_t count) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) p[i] = (O)0.f;
+}
+
+template <typename T>
+int ffn_fwd(int act, const Dims& d, const void* x, const void* wg, const void* wu, const void* wd, const void* bg, const void* bu, const void* bd, void* g, void* u, void* h,
+            void* y, void* workspace, hipStream_t st) {
     auto c = [](const void* p) { return static_cast<const T*>(p); };
     auto w = [](void* p) { return static_cast<T*>(p); };
-    hipLaunchKernelGGL((ffn_product_simple<T, T, EPI_GATE>), tiles(m, n), dim3(256), 0, st, View{x, k, 1}, View{wg, k, 1}, View{}, View{wu, k, 1}, m, n, (int64_t)k, (int64_t)0,
-                       c(bg), c(bu), act, nullptr, nullptr, w(g), w(u), w(h), 0);
-    hipLaunchKernelGGL((ffn_product_simple<T, T, EPI_STORE>), tiles(m, o), dim3(256), 0, st, View{h, n, 1}, View{wd, n, 1}, View{}, View{}, m, o, (int64_t)n, (int64_t)0, c(bd),
-                       nullptr, 0, nullptr, nullptr, nullptr, nullptr, w(y), 0);
-    return check_launch("suhpe_gated_ffn_fwd");
+    if (d.m <= kFewRows) {
+        few_rows<T, true>(c(x), (int)d.m, d.k, c(wg), c(wu), d.n, c(bg), c(bu), act, w(g), w(u), w(h), st);
+        few_rows<T, false>(c(h), (int)d.m, d.n, c(wd), nullptr, d.o, c(bd), nullptr, 0, nullptr, nullptr, w(y), st);
+        return check_launch("suhpe_gated_ffn_fwd");
+    }
+    Space space{static_cast<char*>(workspace)};
+    const FwdSpace s(d, space);
+    GemmArgs a{};
+    a.a = {{rows_of<T>(x, s.xp, d.m, d.k, d, st), nullptr}, (int64_t)d.pad(d.k) * d.es, d.m};
+    a.b = {{rows_of<T>(wg, s.gp, d.n, d.k, d, st), rows_of<T>(wu, s.up, d.n, d.k, d, st)}, (int64_t)d.pad(d.k) * d.es, d.n};
+    a.M = d.m; a.N = d.n; a.K = d.pad(d.k); a.nseg = 1; a.problems = 1; a.ldo = d.n;
+    a.bias = bg; a.bias2 = bu; a.gout = g; a.uout = u; a.out[0] = h; a.act = act;
+    a.vec = d.n % 4 == 0 && aligned(h, 4 * d.es) && aligned(g, 4 * d.es) && aligned(u, 4 * d.es);
+    if (int rc = gemm_launch<T, T, false, false, EPI_GATE>(a, s.gate, st)) return rc;
+    a = GemmArgs{};
+    a.a = {{rows_of<T>(h, s.hp, d.m, d.n, d, st), nullptr}, (int64_t)d.pad(d.n) * d.es, d.m};
+    a.b = {{rows_of<T>(wd, s.dp, d.o, d.n, d, st), nullptr}, (int64_t)d.pad(d.n) * d.es, d.o};
+    a.M = d.m; a.N = d.o; a.K = d.pad(d.n); a.nseg = 1; a.problems = 1; a.ldo = d.o;
+    a.bias = bd; a.out[0] = y; a.part = s.part;
+    a.vec = d.o % 4 == 0 && aligned(y, 4 * d.es);
+    return gemm_launch<T, T, false, false, EPI_STORE>(a, s.down, st);
 }
 
 template <typename T, typename O>
-int ffn_bwd(int act, int64_t m, int k, int n, int o, const void* dy, const void* x, const void* wg, const void* wu, const void* wd, const void* g, const void* u, const void* h,
-            void* dx, void* dwg, void* dwu, void* dwd, void* dbg, void* dbu, void* dbd, int accumulate, void* dg, void* du, hipStream_t st) {
-    auto c = [](const void* p) { return static_cast<const T*>(p); };
-    auto w = [](void* p) { return static_cast<T*>(p); };
-    auto q = [](void* p) { return static_cast<O*>(p); };
-    if (m > 0) {
-        hipLaunchKernelGGL((ffn_product_simple<T, T, EPI_GATE_BWD>), tiles(m, n), dim3(256), 0, st, View{dy, o, 1}, View{wd, 1, n}, View{}, View{}, m, n, (int64_t)o, (int64_t)0,
-                           nullptr, nullptr, act, c(g), c(u), w(dg), w(du), static_cast<T*>(nullptr), 0);
-        if (dx)
-            hipLaunchKernelGGL((ffn_product_simple<T, T, EPI_STORE>), tiles(m, k), dim3(256), 0, st, View{dg, n, 1}, View{wg, 1, k}, View{du, n, 1}, View{wu, 1, k}, m, k,
-                               (int64_t)n, (int64_t)n, nullptr, nullptr, 0, nullptr, nullptr, nullptr, nullptr, w(dx), 0);
+int ffn_bwd(int act, const Dims& d, const void* dy, const void* x, const void* wg, const void* wu, const void* wd, const void* g, const void* u, const void* h, void* dx, void* dwg,
+            void* dwu, void* dwd, void* dbg, void* dbu, void* dbd, int accumulate, void* workspace, hipStream_t st) {
+    Space space{static_cast<char*>(workspace)};
+    const BwdSpace s(d, space);
+    const int np = d.pad(d.n), kp = d.pad(d.k), op = d.pad(d.o);
+    const int64_t es = d.es;
+    if (d.m > 0) {
+        const char* dyr = rows_of<T>(dy, s.yp, d.m, d.o, d, st);
+        GemmArgs a{};
+        a.a = {{dyr, nullptr}, op * es, d.m};
+        a.b = {{rows_of<T>(wd, s.dp, d.o, d.n, d, st), nullptr}, np * es, d.n};
+        a.M = d.m; a.N = d.n; a.K = d.o; a.nseg = 1; a.problems = 1; a.ldo = np;
+        a.gin = g; a.uin = u; a.gout = s.dg; a.uout = s.du; a.act = act;
+        a.vec = d.n % 4 == 0 && aligned(g, 4 * es) && aligned(u, 4 * es);
+        // (k of dy's rows ends at the padded width: zeros there; rows of wd end at o)
+        if (int rc = gemm_launch<T, T, false, true, EPI_GATE_BWD>(a, s.gate, st)) return rc;
+        if (dx) {
+            a = GemmArgs{};
+            a.a = {{static_cast<const char*>(s.dg), static_cast<const char*>(s.du)}, np * es, d.m};
+            a.b = {{rows_of<T>(wg, s.gp, d.n, d.k, d, st), rows_of<T>(wu, s.up, d.n, d.k, d, st)}, kp * es, d.k};
+            a.M = d.m; a.N = d.k; a.K = d.n; a.nseg = 2; a.problems = 1; a.ldo = d.k;
+            a.out[0] = dx; a.part = s.part;
+            a.vec = d.k % 4 == 0 && aligned(dx, 4 * es);
+            if (int rc = gemm_launch<T, T, false, true, EPI_STORE>(a, s.dx, st)) return rc;
+        }
+        if (dwg) {
+            a = GemmArgs{};
+            a.a = {{static_cast<const char*>(s.dg), static_cast<const char*>(s.du)}, np * es, d.n};
+            const char* xr = rows_of<T>(x, s.xp, d.m, d.k, d, st);
+            a.b = {{xr, xr}, kp * es, d.k};
+            a.M = d.n; a.N = d.k; a.K = d.m; a.nseg = 1; a.problems = 2; a.ldo = d.k;
+            a.out[0] = dwg; a.out[1] = dwu; a.part = s.part; a.accumulate = accumulate;
+            a.vec = d.k % 4 == 0 && aligned(dwg, 4 * sizeof(O)) && aligned(dwu, 4 * sizeof(O));
+            if (int rc = gemm_launch<T, O, true, true, EPI_STORE>(a, s.dw, st)) return rc;
+            a = GemmArgs{};
+            a.a = {{dyr, nullptr}, op * es, d.o};
+            a.b = {{rows_of<T>(h, s.hp, d.m, d.n, d, st), nullptr}, np * es, d.n};
+            a.M = d.o; a.N = d.n; a.K = d.m; a.nseg = 1; a.problems = 1; a.ldo = d.n;
+            a.out[0] = dwd; a.part = s.part; a.accumulate = accumulate;
+            a.vec = d.n % 4 == 0 && aligned(dwd, 4 * sizeof(O));
+            if (int rc = gemm_launch<T, O, true, true, EPI_STORE>(a, s.dwd, st)) return rc;
+        }
+    } else if (!accumulate) {                                          // no rows: the gradients are zero
+        auto zero = [&](void* p, int64_t count) {
+            if (p) hipLaunchKernelGGL((ffn_zero<O>), dim3(grid_for(count, 256)), dim3(256), 0, st, static_cast<O*>(p), count);
+        };
+        zero(dwg, (int64_t)d.n * d.k); zero(dwu, (int64_t)d.n * d.k); zero(dwd, (int64_t)d.o * d.n);
+        zero(dbg, d.n); zero(dbu, d.n); zero(dbd, d.o);
     }
-    auto weight = [&](const void* left, int rows, const void* right, int cols, void* out) {
-        hipLaunchKernelGGL((ffn_product_simple<T, O, EPI_STORE>), tiles(rows, cols), dim3(256), 0, st, View{left, 1, rows}, View{right, 1, cols}, View{}, View{}, (int64_t)rows, cols, m,
-                           (int64_t)0, nullptr, nullptr, 0, nullptr, nullptr, nullptr, nullptr, q(out), accumulate);
-    };
-    if (dwg) { weight(dg, n, x, k, dwg); weight(du, n, x, k, dwu); weight(dy, o, h, n, dwd); }
-    auto bias = [&](const void* v, int cols, void* out) {
-        if (out) hipLaunchKernelGGL((ffn_column_sum_simple<T, O>), dim3((unsigned)ceil_div(cols, 256)), dim3(256), 0, st, c(v), m, cols, q(out), accumulate);
-    };
-    bias(dg, n, dbg); bias(du, n, dbu); bias(dy, o, dbd);
+    if (d.m > 0 && (dbg || dbu || dbd)) {
+        ColumnJobs q{};
+        int widest = 0;
+        auto add = [&](const void* v, int64_t ld, int c, void* out, float* part) {
+            if (!out) return;
+            q.x[q.jobs] = v; q.ld[q.jobs] = ld; q.c[q.jobs] = c; q.out[q.jobs] = out; q.part[q.jobs++] = part;
+            widest = c > widest ? c : widest;
+        };
+        add(s.dg, np, d.n, dbg, s.cols[0]); add(s.du, np, d.n, dbu, s.cols[1]); add(dy, d.o, d.o, dbd, s.cols[2]);
+        const int64_t per = ceil_div(d.m, ceil_div(d.m, 32) < kColBlocks ? ceil_div(d.m, 32) : kColBlocks);
+        const int blocks = (int)ceil_div(d.m, per);
+        hipLaunchKernelGGL((column_sums<T>), dim3(blocks, (unsigned)ceil_div(widest, 256), q.jobs), dim3(256), 0, st, q, d.m, per);
+        hipLaunchKernelGGL((column_sums_finish<O>), dim3((unsigned)ceil_div(widest, 16), 1, q.jobs), dim3(256), 0, st, q, blocks, accumulate);
+    }
     return check_launch("suhpe_gated_ffn_bwd");
 }
 
@@ -123,6 +317,11 @@ int ffn_sizes(const char* who, int dtype, int act, int64_t m, int k, int n, int 
     SUHPE_REQUIRE(k <= (1 << 20) && n <= (1 << 20) && o <= (1 << 20), "%s: widths up to 2^20", who);
     return SUHPE_OK;
 }
+int space_short(const char* who, const void* workspace, int64_t have, int64_t need) {
+    if (need == 0 || (workspace && have >= need && aligned(workspace, 256))) return SUHPE_OK;
+    set_error("%s: workspace of %lld bytes at %p, needs %lld on a 256-byte boundary", who, (long long)have, workspace, (long long)need);
+    return SUHPE_EWORKSPACE;
+}
 
 }  // namespace
 }  // namespace suhpe
@@ -131,7 +330,12 @@ using namespace suhpe;
 
 extern "C" {
 
-int64_t suhpe_gated_ffn_fwd_workspace_bytes(int dtype, int64_t m, int k, int n, int o) { return 0; }
+int64_t suhpe_gated_ffn_fwd_workspace_bytes(int dtype, int64_t m, int k, int n, int o) {
+    if (ffn_sizes("suhpe_gated_ffn_fwd_workspace_bytes", dtype, 0, m, k, n, o) || m <= kFewRows) return 0;
+    Space space{nullptr};
+    const FwdSpace s(Dims{m, k, n, o, dtype_size(dtype)}, space);
+    return space.used;
+}
 
 int suhpe_gated_ffn_fwd(int dtype, int act, int64_t m, int k, int n, int o, const void* x, const void* wg, const void* wu, const void* wd, const void* bg, const void* bu,
                         const void* bd, void* g, void* u, void* h, void* y, void* workspace, int64_t workspace_bytes, suhpe_stream_t stream) {
@@ -139,13 +343,23 @@ int suhpe_gated_ffn_fwd(int dtype, int act, int64_t m, int k, int n, int o, cons
     SUHPE_REQUIRE((g == nullptr) == (u == nullptr), "suhpe_gated_ffn_fwd: g and u are kept together or not at all");
     if (m == 0) return SUHPE_OK;
     SUHPE_REQUIRE(x && wg && wu && wd && h && y, "suhpe_gated_ffn_fwd: null pointer");
+    const Dims d{m, k, n, o, dtype_size(dtype)};
+    if (m > kFewRows)
+        SUHPE_REQUIRE((d.odd(k) || (aligned(x, 16) && aligned(wg, 16) && aligned(wu, 16))) && (d.odd(n) || (aligned(h, 16) && aligned(wd, 16))),
+                      "suhpe_gated_ffn_fwd: x, wg, wu, wd and h start on 16-byte boundaries");
+    if (int rc = space_short("suhpe_gated_ffn_fwd", workspace, workspace_bytes, suhpe_gated_ffn_fwd_workspace_bytes(dtype, m, k, n, o))) return rc;
     hipStream_t st = as_stream(stream);
-    if (dtype == SUHPE_F32) return ffn_fwd<float>(act, m, k, n, o, x, wg, wu, wd, bg, bu, bd, g, u, h, y, st);
-    if (dtype == SUHPE_BF16) return ffn_fwd<bf16>(act, m, k, n, o, x, wg, wu, wd, bg, bu, bd, g, u, h, y, st);
-    return ffn_fwd<f16>(act, m, k, n, o, x, wg, wu, wd, bg, bu, bd, g, u, h, y, st);
+    if (dtype == SUHPE_F32) return ffn_fwd<float>(act, d, x, wg, wu, wd, bg, bu, bd, g, u, h, y, workspace, st);
+    if (dtype == SUHPE_BF16) return ffn_fwd<bf16>(act, d, x, wg, wu, wd, bg, bu, bd, g, u, h, y, workspace, st);
+    return ffn_fwd<f16>(act, d, x, wg, wu, wd, bg, bu, bd, g, u, h, y, workspace, st);
 }
 
-int64_t suhpe_gated_ffn_bwd_workspace_bytes(int dtype, int64_t m, int k, int n, int o) { return 2 * ceil_div(m * n * dtype_size(dtype), 256) * 256; }
+int64_t suhpe_gated_ffn_bwd_workspace_bytes(int dtype, int64_t m, int k, int n, int o) {
+    if (m == 0 || ffn_sizes("suhpe_gated_ffn_bwd_workspace_bytes", dtype, 0, m, k, n, o)) return 0;
+    Space space{nullptr};
+    const BwdSpace s(Dims{m, k, n, o, dtype_size(dtype)}, space);
+    return space.used;
+}
 
 int suhpe_gated_ffn_bwd(int dtype, int act, int64_t m, int k, int n, int o, const void* dy, const void* x, const void* wg, const void* wu, const void* wd, const void* g,
                         const void* u, const void* h, void* dx, void* dwg, void* dwu, void* dwd, void* dbg, void* dbu, void* dbd, int grad_dtype, int accumulate,
@@ -154,14 +368,14 @@ int suhpe_gated_ffn_bwd(int dtype, int act, int64_t m, int k, int n, int o, cons
     SUHPE_REQUIRE(grad_dtype == dtype || grad_dtype == SUHPE_F32, "suhpe_gated_ffn_bwd: gradients have the weights' type or fp32");
     SUHPE_REQUIRE((dwg != nullptr) == (dwu != nullptr) && (dwg != nullptr) == (dwd != nullptr), "suhpe_gated_ffn_bwd: the three weights' gradients are wanted together or not at all");
     SUHPE_REQUIRE(m == 0 || (dy && x && wg && wu && wd && g && u && h), "suhpe_gated_ffn_bwd: null pointer");
-    const int64_t need = suhpe_gated_ffn_bwd_workspace_bytes(dtype, m, k, n, o);
-    if (need > 0 && (!workspace || workspace_bytes < need)) {
-        set_error("suhpe_gated_ffn_bwd: workspace of %lld bytes, needs %lld", (long long)workspace_bytes, (long long)need);
-        return SUHPE_EWORKSPACE;
-    }
-    void *dg = workspace, *du = static_cast<char*>(workspace) + need / 2;
+    if (m == 0 && (accumulate || !(dwg || dbg || dbu || dbd))) return SUHPE_OK;      // nothing to write
+    const Dims d{m, k, n, o, dtype_size(dtype)};
+    if (m > 0)
+        SUHPE_REQUIRE((d.odd(k) || (aligned(x, 16) && aligned(wg, 16) && aligned(wu, 16))) && (d.odd(n) || (aligned(h, 16) && aligned(wd, 16))) && (d.odd(o) || aligned(dy, 16)),
+                      "suhpe_gated_ffn_bwd: dy, x, wg, wu, wd and h start on 16-byte boundaries");
+    if (int rc = space_short("suhpe_gated_ffn_bwd", workspace, workspace_bytes, suhpe_gated_ffn_bwd_workspace_bytes(dtype, m, k, n, o))) return rc;
     hipStream_t st = as_stream(stream);
-#define FFN_BWD(T, O) ffn_bwd<T, O>(act, m, k, n, o, dy, x, wg, wu, wd, g, u, h, dx, dwg, dwu, dwd, dbg, dbu, dbd, accumulate, dg, du, st)
+#define FFN_BWD(T, O) ffn_bwd<T, O>(act, d, dy, x, wg, wu, wd, g, u, h, dx, dwg, dwu, dwd, dbg, dbu, dbd, accumulate, workspace, st)
     if (dtype == SUHPE_F32) return FFN_BWD(float, float);
     if (dtype == SUHPE_BF16) return grad_dtype == SUHPE_F32 ? FFN_BWD(bf16, float) : FFN_BWD(bf16, bf16);
     return grad_dtype == SUHPE_F32 ? FFN_BWD(f16, float) : FFN_BWD(f16, f16);

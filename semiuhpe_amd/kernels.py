@@ -1670,6 +1670,11 @@ def _scratch(nbytes, device):
     return torch.empty(int(nbytes), dtype=torch.uint8, device=device) if nbytes > 0 else None
 
 
+def _on_16_bytes(t):
+    """the tensor, or a copy of one that starts off a 16-byte boundary (a view into another tensor)"""
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _layernorm16_fwd(x, c, eps, gamma, beta):
     _chk_tok(x, "x")
     _chk_tok(gamma, "gamma", torch.float32, x.device, (c,)); _chk_tok(beta, "beta", torch.float32, x.device, (c,))
@@ -1821,6 +1826,7 @@ def gated_ffn_fwd(x, wg, wu, wd, bg=None, bu=None, bd=None, act="silu", save=Tru
     """The gated feed-forward block y = (act(x wg^T + bg) * (x wu^T + bu)) wd^T + bd: x (..., k), wg and wu (n, k), wd (o, n) -> y (..., o) and, with save=True, what
     gated_ffn_bwd needs (g, u, h: both projections and the product, each rounded to x's type once), else None."""
     m, k, n, o = _ffn_sizes(x, wg, wu, wd, act)
+    x, wg, wu, wd = (_on_16_bytes(t) for t in (x, wg, wu, wd))
     for t, name, c in ((bg, "bg", n), (bu, "bu", n), (bd, "bd", o)):
         _chk_tok(t, name, x.dtype, x.device, (c,))
     y = torch.empty(x.shape[:-1] + (o,), dtype=x.dtype, device=x.device)
@@ -1853,9 +1859,10 @@ def gated_ffn_bwd(dy, x, wg, wu, wd, saved, act="silu", dwg=None, dwu=None, dwd=
     for t, name, shape in grads:
         _chk_tok(t, name, gtype, x.device, shape)
     dx = torch.empty_like(x) if need_dx else None
+    dy, x, wg, wu, wd = (_on_16_bytes(t) for t in (dy, x, wg, wu, wd))
     nbytes = _lib.load().suhpe_gated_ffn_bwd_workspace_bytes(_DTYPES[x.dtype], m, k, n, o)
     ws = _scratch(nbytes, x.device)
-    g, u, h = saved
+    g, u, h = (_on_16_bytes(t) for t in saved)
     _call_on(x.device, "suhpe_gated_ffn_bwd", _DTYPES[x.dtype], ACT[act], m, k, n, o, ptr(dy), ptr(x), ptr(wg), ptr(wu), ptr(wd), ptr(g), ptr(u), ptr(h), ptr(dx),
              ptr(dwg), ptr(dwu), ptr(dwd), ptr(dbg), ptr(dbu), ptr(dbd), _DTYPES[gtype], int(accumulate), ptr(ws), nbytes)
     return dx

@@ -79,6 +79,22 @@ def test_gated_ffn(K, cfg, dtype):
     assert all(torch.equal(p, q) for p, q in zip(before, dw))              # (the same bits again)
 
 
+@pytest.mark.parametrize("cfg", [(4100, 3080, 3336, 3600, "bf16"), (2300, 1000, 2504, 1000, "fp16"), (2100, 520, 1304, 520, "fp32"), (1500, 1003, 1503, 1005, "bf16"),
+                                 (20000, 96, 136, 96, "bf16")], ids=str)
+def test_large_sizes(K, cfg):
+    """the large tiles, reductions split over many workgroups and rows of no whole vector, against 64-bit products"""
+    m, k, n, o, dtype = cfg
+    x, w, b, dy = block(m, k, n, o, dtype, m % 200 == 100)
+    ref = R.gated_ffn(x, *w, *b, dy, "silu", device="cuda")
+    got, _ = run(K, x, w, b, dy, "silu")
+    for key, (value, bound) in ref.items():
+        if got[key] is not None:
+            R.within(got[key], value, bound, key)
+            off = (got[key].double() - value).norm() / value.norm()
+            # random roundings add up as squares: a few half steps of the type (fp32: of its sums of up to 20000 terms) in the 2-norm
+            assert float(off) < (6 * R.half(x.dtype) if dtype != "fp32" else 1e-5), (key, float(off))
+
+
 @pytest.mark.parametrize("act", ["silu", "gelu", "sigmoid", "none"])
 def test_activations(K, act):
     x, w, b, dy = block(40, 48, 56, 32, "fp32", True)

@@ -62,6 +62,8 @@ def test_gated_ffn_refusals(lib):
     for bad in (dict(grad=F16), dict(grad=4), dict(dy=None), dict(dwg=None), dict(dwd=None)):
         assert bwd(**bad) == -1, bad
         assert b"suhpe_gated_ffn_bwd" in lib.suhpe_last_error()
+    assert lib.suhpe_gated_ffn_bwd(BF16, 3, 0, 16, 24, 16, None, None, None, None, None, None, None, None, None, None, None, None, None, None, None, BF16, 0, None, 0, None) == 0
+    assert lib.suhpe_gated_ffn_bwd_workspace_bytes(BF16, 0, 16, 24, 16) == 0
     assert bwd(nbytes=need - 1) == -3
     assert bwd(ws=None) == -3
 

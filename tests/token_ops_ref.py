@@ -16,7 +16,7 @@ def half(t):
 
 def within(got, ref, bound, what=""):
     """every element finite where the reference is, and within its bound"""
-    got = got.detach().cpu().double()
+    got = got.detach().to(ref.device).double()
     assert got.shape == ref.shape, (what, got.shape, ref.shape)
     off = (got - ref).abs()
     bad = ~(off <= bound)
@@ -127,15 +127,15 @@ def act(g, name):
     raise ValueError(name)
 
 
-def gated_ffn(x, wg, wu, wd, bg, bu, bd, dy, name, grad_type=None):
-    """dict of (value, bound): y and, with dy, dx, dwg, dwu, dwd, dbg, dbu, dbd"""
+def gated_ffn(x, wg, wu, wd, bg, bu, bd, dy, name, grad_type=None, device="cpu"):
+    """dict of (value, bound): y and, with dy, dx, dwg, dwu, dwd, dbg, dbu, dbd (64-bit products on `device`)"""
     t = x.dtype
     r = half(t) * 1.001
     tiny = 2.0 ** -24 if t == torch.float16 else 0.0                    # (half a step of fp16's subnormals)
-    f = lambda v: v.detach().cpu().double()  # noqa: E731
+    f = lambda v: v.detach().to(device).double()  # noqa: E731
     X, G, W, D = f(x).reshape(-1, x.shape[-1]), f(wg), f(wu), f(wd)
     k, n, o = G.shape[1], G.shape[0], D.shape[0]
-    zero = lambda c: torch.zeros(c, dtype=torch.float64)  # noqa: E731
+    zero = lambda c: torch.zeros(c, dtype=torch.float64, device=device)  # noqa: E731
     Bg, Bu, Bd = (f(b) if b is not None else zero(c) for b, c in ((bg, n), (bu, n), (bd, o)))
     g, u = X @ G.t() + Bg, X @ W.t() + Bu
     e_g = (k + 2) * U * (X.abs() @ G.abs().t() + Bg.abs())
