@@ -188,7 +188,223 @@ int dropout_launch(const void* x, const void* skip, void* y, int64_t count, uint
 
 // ------------------------------------------------------------------------------------------ LayerNorm of 16-bit rows
 // y = (x - mean) rstd gamma + beta with the statistics, gamma, beta and the parameters' gradients in fp32: only x, y, dy, dx have 16 bits.
-// One wavefront per row, any width.
+// LPR lanes share a row (8 .. 64, or the 256 of a block), each holding NV vectors of 8 elements in registers between the statistics and the result: one pass
+// over memory.  Blocks are persistent: gamma and beta (8 bytes an element, twice what x and y take together) are loaded once per lane, not once per row, and
+// the next row's loads are issued before this row's sums.  Any width >= 8 runs on full vectors: a row's last vector starts at c - 8 and leaves out of the sums
+// what the vector before it holds (both write the same bits there), and 16-byte accesses may start at any element.
+template <typename T, int LPR, int NV> struct LnRow {
+    typename Vec<T, 8>::type v[NV];
+    __device__ __forceinline__ void load(const T* row, const int (&at)[NV]) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+            if (at[k] >= 0) __builtin_memcpy(&v[k], row + at[k], 16);
+    }
+};
+
+// sum over the LPR lanes of a row (lds: 2 x 4 floats, two places used in turn)
+template <int LPR> __device__ __forceinline__ float row_sum(float v, float* lds, int& turn) {
+    constexpr int S = LPR < 64 ? LPR : 64;
+#pragma unroll
+    for (int o = S / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    if constexpr (LPR == 256) {
+        float* at = lds + turn * 4;
+        if ((threadIdx.x & 63) == 0) at[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = (at[0] + at[1]) + (at[2] + at[3]);
+        turn ^= 1;
+    }
+    return v;
+}
+
+// element offset of this lane's vectors in a row (-1: none), and how many leading elements of the last one the vector before it owns
+template <int LPR, int NV> __device__ __forceinline__ void ln_places(int c, int (&at)[NV], int (&skip)[NV]) {
+    const int sub = threadIdx.x % LPR;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int e = (sub + LPR * k) * 8;
+        at[k] = e >= c ? -1 : e + 8 <= c ? e : c - 8;
+        skip[k] = e >= c ? 8 : e - at[k];
+    }
+}
+
+// this lane's columns of gamma or beta, in 16-byte loads (32 four-byte ones per lane took 20 us of a 27 us launch over 4 099 rows of 1 357)
+template <int NV> __device__ __forceinline__ void ln_param(const float* p, const int (&at)[NV], float without, float (&v)[NV][8]) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[k][e] = without;
+        if (p && at[k] >= 0) {
+            float4 lo, hi;
+            __builtin_memcpy(&lo, p + at[k], 16);
+            __builtin_memcpy(&hi, p + at[k] + 4, 16);
+            v[k][0] = lo.x; v[k][1] = lo.y; v[k][2] = lo.z; v[k][3] = lo.w;
+            v[k][4] = hi.x; v[k][5] = hi.y; v[k][6] = hi.z; v[k][7] = hi.w;
+        }
+    }
+}
+
+template <typename T, int LPR, int NV>
+__global__ __launch_bounds__(256) void layernorm16_fwd_kernel(const T* __restrict__ x, int64_t rows, int c, float eps, const float* __restrict__ gamma,
+                                                              const float* __restrict__ beta, T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
+    __shared__ float lds[8];
+    int turn = 0;
+    constexpr int RPB = 256 / LPR;
+    int at[NV], skip[NV];
+    ln_places<LPR, NV>(c, at, skip);
+    float ga[NV][8], be[NV][8];
+    ln_param<NV>(gamma, at, 1.f, ga);
+    ln_param<NV>(beta, at, 0.f, be);
+    const float inv = 1.f / c;
+    const int64_t first = (int64_t)blockIdx.x * RPB, stride = (int64_t)gridDim.x * RPB;
+    const int mine = threadIdx.x / LPR;
+    LnRow<T, LPR, NV> cur, next;
+    if (first + mine < rows) cur.load(x + (first + mine) * c, at);
+    for (int64_t r0 = first; r0 < rows; r0 += stride) {
+        const int64_t row = r0 + mine;
+        if (row + stride < rows) next.load(x + (row + stride) * c, at);
+        float v[NV][8], s = 0.f, q = 0.f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[k][e] = (float)cur.v[k][e];
+                s += e >= skip[k] ? v[k][e] : 0.f;
+            }
+        const float m = row_sum<LPR>(s, lds, turn) * inv;
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[k][e] -= m;
+                q += e >= skip[k] ? v[k][e] * v[k][e] : 0.f;
+            }
+        const float rs = 1.f / sqrtf(row_sum<LPR>(q, lds, turn) * inv + eps);
+        if (row < rows) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k)
+                if (at[k] >= 0) {
+                    typename Vec<T, 8>::type o;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) o[e] = (T)(v[k][e] * rs * ga[k][e] + be[k][e]);
+                    __builtin_memcpy(y + row * c + at[k], &o, 16);
+                }
+            if (threadIdx.x % LPR == 0) { mean[row] = m; rstd[row] = rs; }
+        }
+        cur = next;
+    }
+}
+
+// dx = rstd (g - mean(g) - xhat mean(g xhat)) [+ skip], g = dy gamma, and the block's column sums of dy xhat and dy: part[block][2][c].  x and dy are read once.
+template <typename T, int LPR, int NV, bool COLS>
+__global__ __launch_bounds__(256) void layernorm16_bwd_kernel(const T* __restrict__ x, const T* __restrict__ dy, int64_t rows, int c, const float* __restrict__ mean,
+                                                              const float* __restrict__ rstd, const float* __restrict__ gamma, const T* __restrict__ bypass,
+                                                              T* __restrict__ dx, float* __restrict__ part) {
+    __shared__ float lds[8];
+    extern __shared__ float cols[];                                    // [wavefront][2][c]
+    int turn = 0;
+    constexpr int RPB = 256 / LPR;
+    int at[NV], skip[NV];
+    ln_places<LPR, NV>(c, at, skip);
+    float ga[NV][8], sg[NV][8], sb[NV][8];
+    ln_param<NV>(gamma, at, 1.f, ga);
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sg[k][e] = sb[k][e] = 0.f;
+    const float inv = 1.f / c;
+    const int64_t first = (int64_t)blockIdx.x * RPB, stride = (int64_t)gridDim.x * RPB;
+    const int mine = threadIdx.x / LPR;
+    LnRow<T, LPR, NV> cx, cd, nx, nd;
+    float m = 0.f, rs = 0.f, nm = 0.f, nrs = 0.f;
+    if (first + mine < rows) {
+        cx.load(x + (first + mine) * c, at);
+        cd.load(dy + (first + mine) * c, at);
+        m = mean[first + mine];
+        rs = rstd[first + mine];
+    }
+    for (int64_t r0 = first; r0 < rows; r0 += stride) {
+        const int64_t row = r0 + mine;
+        if (row + stride < rows) {
+            nx.load(x + (row + stride) * c, at);
+            nd.load(dy + (row + stride) * c, at);
+            nm = mean[row + stride];
+            nrs = rstd[row + stride];
+        }
+        const bool live = row < rows;
+        float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const bool own = live && e >= skip[k];
+                const float d = (float)cd.v[k][e], xh = ((float)cx.v[k][e] - m) * rs, g = d * ga[k][e];
+                s0 += own ? g : 0.f;
+                s1 += own ? g * xh : 0.f;
+                if constexpr (COLS) {
+                    sg[k][e] += own ? d * xh : 0.f;
+                    sb[k][e] += own ? d : 0.f;
+                }
+            }
+        s0 = row_sum<LPR>(s0, lds, turn) * inv;
+        s1 = row_sum<LPR>(s1, lds, turn) * inv;
+        if (live) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k)
+                if (at[k] >= 0) {
+                    typename Vec<T, 8>::type o, b;
+                    if (bypass) __builtin_memcpy(&b, bypass + row * c + at[k], 16);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {                      // (xhat and g again from the 16-bit rows: cheaper than the registers that would hold them)
+                        const float xh = ((float)cx.v[k][e] - m) * rs, g = (float)cd.v[k][e] * ga[k][e];
+                        const float d = rs * (g - s0 - xh * s1);
+                        o[e] = (T)(bypass ? d + (float)b[e] : d);
+                    }
+                    __builtin_memcpy(dx + row * c + at[k], &o, 16);
+                }
+        }
+        cx = nx; cd = nd; m = nm; rs = nrs;
+    }
+    if constexpr (COLS) {
+        // rows of one wavefront first (lanes LPR, 2 LPR, ... apart), then the four wavefronts
+        if constexpr (LPR < 64)
+#pragma unroll
+            for (int k = 0; k < NV; ++k)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+#pragma unroll
+                    for (int o = LPR; o < 64; o <<= 1) {
+                        sg[k][e] += __shfl_xor(sg[k][e], o, 64);
+                        sb[k][e] += __shfl_xor(sb[k][e], o, 64);
+                    }
+        float* const mine_part = part + (int64_t)blockIdx.x * 2 * c;
+        if constexpr (LPR == 256) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (e >= skip[k]) {                                // (one lane owns a column)
+                        mine_part[at[k] + e] = sg[k][e];
+                        mine_part[c + at[k] + e] = sb[k][e];
+                    }
+            return;
+        }
+        if ((int)(threadIdx.x & 63) < LPR) {
+            float* at_wave = cols + (threadIdx.x >> 6) * 2 * c;
+#pragma unroll
+            for (int k = 0; k < NV; ++k)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (e >= skip[k]) {
+                        at_wave[at[k] + e] = sg[k][e];
+                        at_wave[c + at[k] + e] = sb[k][e];
+                    }
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < 2 * c; i += 256) mine_part[i] = (cols[i] + cols[2 * c + i]) + (cols[4 * c + i] + cols[6 * c + i]);
+    }
+}
+
+// Widths under 8 and over 8192: one wavefront per row, element by element
 template <typename T>
 __global__ __launch_bounds__(256) void layernorm16_fwd_any(const T* __restrict__ x, int64_t rows, int c, float eps, const float* __restrict__ gamma,
                                                            const float* __restrict__ beta, T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
@@ -253,53 +469,101 @@ __global__ __launch_bounds__(256) void layernorm16_bwd_cols_any(const T* __restr
     }
 }
 
-// the partial sums of `blocks` blocks in a fixed order: 16 columns x 16 slices per block
-__global__ __launch_bounds__(256) void layernorm16_bwd_finish(const float* __restrict__ part, int blocks, int c, float* __restrict__ dgamma, float* __restrict__ dbeta,
-                                                              int accumulate) {
-    __shared__ float lds[16][17];
+// the partial sums of `blocks` blocks in a fixed order: 16 columns x 64 slices per block, 8 loads of a thread in flight together
+__global__ __launch_bounds__(1024) void layernorm16_bwd_finish(const float* __restrict__ part, int blocks, int c, float* __restrict__ dgamma, float* __restrict__ dbeta,
+                                                               int accumulate) {
+    __shared__ float lds[64][17];
     const int col = threadIdx.x & 15, slice = threadIdx.x >> 4, j = blockIdx.x * 16 + col, which = blockIdx.y;
     float s = 0.f;
     if (j < c)
-        for (int b = slice; b < blocks; b += 16) s += part[((int64_t)b * 2 + which) * c + j];
+        for (int b0 = slice; b0 < blocks; b0 += 512) {
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = b0 + 64 * u < blocks ? part[((int64_t)(b0 + 64 * u) * 2 + which) * c + j] : 0.f;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s += v[u];
+        }
     lds[slice][col] = s;
     __syncthreads();
     float* out = which ? dbeta : dgamma;
     if (slice == 0 && j < c && out) {
         float t = 0.f;
 #pragma unroll
-        for (int k = 0; k < 16; ++k) t += lds[k][col];
+        for (int k = 0; k < 64; ++k) t += lds[k][col];
         out[j] = accumulate ? out[j] + t : t;
     }
 }
 
 constexpr int kLnBlocks = 512;
 
+// lanes per row and vectors per lane for a width: as few lanes as hold the row in at most 3 vectors each (the sums cross few lanes and the parameters' registers
+// stay few), then the whole block
+#define LN16_WIDTHS(CALL)                                \
+    const int nv = (c + 7) / 8;                          \
+    if (nv <= 8) CALL(8, 1);                             \
+    else if (nv <= 16) CALL(8, 2);                       \
+    else if (nv <= 24) CALL(8, 3);                       \
+    else if (nv <= 32) CALL(16, 2);                      \
+    else if (nv <= 48) CALL(16, 3);                      \
+    else if (nv <= 64) CALL(32, 2);                      \
+    else if (nv <= 96) CALL(32, 3);                      \
+    else if (nv <= 128) CALL(64, 2);                     \
+    else if (nv <= 192) CALL(64, 3);                     \
+    else if (nv <= 256) CALL(256, 1);                    \
+    else if (nv <= 512) CALL(256, 2);                    \
+    else CALL(256, 4);
+
 template <typename T>
 int ln16_fwd(const void* x, int64_t rows, int c, float eps, const float* gamma, const float* beta, void* y, float* mean, float* rstd, hipStream_t st) {
-    hipLaunchKernelGGL((layernorm16_fwd_any<T>), dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, st, static_cast<const T*>(x), rows, c, eps, gamma, beta,
-                       static_cast<T*>(y), mean, rstd);
+    const T* xt = static_cast<const T*>(x);
+    T* yt = static_cast<T*>(y);
+    if (c < 8 || c > 8192) {
+        hipLaunchKernelGGL((layernorm16_fwd_any<T>), dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, st, xt, rows, c, eps, gamma, beta, yt, mean, rstd);
+    } else {
+#define LN16_FWD(L, V)                                                                                                                                           \
+    do {                                                                                                                                                         \
+        const int64_t need = ceil_div(rows, 256 / L);                                                                                                            \
+        hipLaunchKernelGGL((layernorm16_fwd_kernel<T, L, V>), dim3((unsigned)(need < 2048 ? need : 2048)), dim3(256), 0, st, xt, rows, c, eps, gamma, beta, yt, mean, rstd); \
+    } while (0)
+        LN16_WIDTHS(LN16_FWD)
+#undef LN16_FWD
+    }
     return check_launch("suhpe_layernorm16_fwd");
 }
 
 template <typename T>
 int ln16_bwd(const void* x, const void* dy, int64_t rows, int c, const float* mean, const float* rstd, const float* gamma, const void* skip, void* dx, float* dgamma,
              float* dbeta, int accumulate, float* part, hipStream_t st) {
-    const T *xt = static_cast<const T*>(x), *dt = static_cast<const T*>(dy);
+    const T *xt = static_cast<const T*>(x), *dt = static_cast<const T*>(dy), *kt = static_cast<const T*>(skip);
+    T* ot = static_cast<T*>(dx);
+    const bool want = dgamma || dbeta;
     int blocks = 0;
-    if (rows > 0) {
-        hipLaunchKernelGGL((layernorm16_bwd_dx_any<T>), dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, st, xt, dt, rows, c, mean, rstd, gamma,
-                           static_cast<const T*>(skip), static_cast<T*>(dx));
-        if (dgamma || dbeta) {
+    if (rows > 0 && (c < 8 || c > 8192)) {
+        hipLaunchKernelGGL((layernorm16_bwd_dx_any<T>), dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, st, xt, dt, rows, c, mean, rstd, gamma, kt, ot);
+        if (want) {
             blocks = (int)(ceil_div(rows, 16) < kLnBlocks ? ceil_div(rows, 16) : kLnBlocks);
             const int64_t per = ceil_div(rows, blocks);
             blocks = (int)ceil_div(rows, per);
             hipLaunchKernelGGL((layernorm16_bwd_cols_any<T>), dim3(blocks, (unsigned)ceil_div(c, 64)), dim3(256), 0, st, xt, dt, rows, c, per, mean, rstd, part);
         }
+    } else if (rows > 0) {
+#define LN16_BWD(L, V)                                                                                                                                           \
+    do {                                                                                                                                                         \
+        const int64_t need = ceil_div(rows, 256 / L);                                                                                                            \
+        blocks = (int)(need < 256 ? need : need < 1024 ? 256 : need < 2048 ? need / 4 : kLnBlocks);                                                              \
+        if (want)                                                                                                                                                \
+            hipLaunchKernelGGL((layernorm16_bwd_kernel<T, L, V, true>), dim3(blocks), dim3(256), L == 256 ? 0 : 8 * c * sizeof(float), st, xt, dt, rows, c, mean, rstd, gamma, kt, ot, part); \
+        else                                                                                                                                                     \
+            hipLaunchKernelGGL((layernorm16_bwd_kernel<T, L, V, false>), dim3((unsigned)(need < 2048 ? need : 2048)), dim3(256), 0, st, xt, dt, rows, c, mean, rstd, gamma, kt, ot, part); \
+    } while (0)
+        LN16_WIDTHS(LN16_BWD)
+#undef LN16_BWD
     }
-    if (dgamma || dbeta)
-        hipLaunchKernelGGL(layernorm16_bwd_finish, dim3((unsigned)ceil_div(c, 16), 2), dim3(256), 0, st, part, blocks, c, dgamma, dbeta, accumulate);
+    if (want)
+        hipLaunchKernelGGL(layernorm16_bwd_finish, dim3((unsigned)ceil_div(c, 16), 2), dim3(1024), 0, st, part, blocks, c, dgamma, dbeta, accumulate);
     return check_launch("suhpe_layernorm16_bwd");
 }
+#undef LN16_WIDTHS
 
 }  // namespace
 }  // namespace suhpe

@@ -205,7 +205,8 @@ def test_dropout_refusals(K):
 
 
 # ------------------------------------------------------------------------------------------------ 16-bit LayerNorm
-LN = [(1, 1), (1, 8), (3, 5), (4, 64), (17, 192), (33, 384), (5, 576), (2, 1357), (9, 2048), (300, 96), (1, 5000), (3, 4096), (70, 40), (129, 1001)]
+LN = [(1, 1), (1, 8), (3, 5), (4, 64), (17, 192), (33, 384), (5, 576), (2, 1357), (9, 2048), (300, 96), (1, 5000), (3, 4096), (70, 40), (129, 1001),
+      (5000, 192), (2100, 33), (3000, 517), (1, 9), (7, 7), (50, 127), (40, 250), (20, 380), (20, 770), (3, 1537), (700, 2051), (3, 8192), (2, 8200), (600, 4099)]
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
