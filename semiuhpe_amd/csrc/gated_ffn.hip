@@ -106,49 +106,50 @@ void few_rows(const T* x, int M, int64_t K, const T* w, const T* w2, int N, cons
 }
 
 // ------------------------------------------------------------------------------------------ column sums (bias gradients)
-// up to three matrices in one launch (grid z); part: [job][row block][columns], finished in a fixed order
-struct ColumnJobs { const void* x[3]; int64_t ld[3]; int c[3]; void* out[3]; float* part[3]; int jobs; };
+// dg's and du's come from the tiles of the product that makes them, dy's from a pass of its own: [row block][columns] each, finished in a fixed order
 constexpr int kColBlocks = 256;
 
 template <typename T>
-__global__ __launch_bounds__(256) void column_sums(const ColumnJobs q, int64_t rows, int64_t rows_per_block) {
-    __shared__ float lds[4][256];
-    const int job = blockIdx.z, c = q.c[job], lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = blockIdx.y * 256 + lane * 4;
-    if ((int)blockIdx.y * 256 >= c) return;
-    const T* x = static_cast<const T*>(q.x[job]);
-    const int64_t ld = q.ld[job], r0 = (int64_t)blockIdx.x * rows_per_block, r1 = r0 + rows_per_block < rows ? r0 + rows_per_block : rows;
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
-    const bool vec = (ld & 3) == 0 && j + 4 <= c && (reinterpret_cast<uintptr_t>(x) & (4 * sizeof(T) - 1)) == 0;
-    for (int64_t r = r0 + wave; r < r1; r += 4) {
-        float v[4];
-        if (vec) load_n<T, 4>(x + r * ld + j, v);
-        else
+__global__ __launch_bounds__(256) void column_sums(const T* __restrict__ x, int64_t rows, int c, int64_t rows_per_block, float* __restrict__ part) {
+    __shared__ float lds[8][256];
+    const int cg = threadIdx.x & 31, sub = threadIdx.x >> 5, n = blockIdx.y * 256 + cg * 8;
+    const int64_t r0 = (int64_t)blockIdx.x * rows_per_block, r1 = r0 + rows_per_block < rows ? r0 + rows_per_block : rows;
+    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (n < c)
+        for (int64_t r = r0 + sub; r < r1; r += 8) {
+            float v[8];
+            load8(x + r * c + n, n, c, v);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = j + e < c ? (float)x[r * ld + j + e] : 0.f;
+            for (int e = 0; e < 8; ++e) s[e] += v[e];
+        }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[e] += v[e];
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) lds[wave][lane * 4 + e] = s[e];
+    for (int e = 0; e < 8; ++e) lds[sub][cg * 8 + e] = s[e];
     __syncthreads();
-    const int jj = blockIdx.y * 256 + threadIdx.x;
-    if (jj < c) q.part[job][(int64_t)blockIdx.x * c + jj] = (lds[0][threadIdx.x] + lds[1][threadIdx.x]) + (lds[2][threadIdx.x] + lds[3][threadIdx.x]);
+    const int j = blockIdx.y * 256 + threadIdx.x;
+    if (j < c) {
+        float t = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) t += lds[k][threadIdx.x];
+        part[(int64_t)blockIdx.x * c + j] = t;
+    }
 }
 
+struct ColumnJobs { const float* part[3]; int blocks[3], c[3]; void* out[3]; int jobs; };
+
 template <typename O>
-__global__ __launch_bounds__(256) void column_sums_finish(const ColumnJobs q, int blocks, int accumulate) {
-    __shared__ float lds[16][17];
-    const int job = blockIdx.z, c = q.c[job], col = threadIdx.x & 15, slice = threadIdx.x >> 4, j = blockIdx.x * 16 + col;
+__global__ __launch_bounds__(1024) void column_sums_finish(const ColumnJobs q, int accumulate) {
+    __shared__ float lds[64][17];
+    const int job = blockIdx.z, c = q.c[job], blocks = q.blocks[job], col = threadIdx.x & 15, slice = threadIdx.x >> 4, j = blockIdx.x * 16 + col;
     if ((int)blockIdx.x * 16 >= c) return;
     float s = 0.f;
     if (j < c)
-        for (int b = slice; b < blocks; b += 16) s += q.part[job][(int64_t)b * c + j];
+        for (int b = slice; b < blocks; b += 64) s += q.part[job][(int64_t)b * c + j];
     lds[slice][col] = s;
     __syncthreads();
     if (slice == 0 && j < c) {
         float t = 0.f;
 #pragma unroll
-        for (int k = 0; k < 16; ++k) t += lds[k][col];
+        for (int k = 0; k < 64; ++k) t += lds[k][col];
         O* out = static_cast<O*>(q.out[job]);
         out[j] = (O)(accumulate ? (float)out[j] + t : t);
     }
@@ -174,7 +175,6 @@ struct Dims {
     int64_t steps(int64_t c) const { return ceil_div(c, 128 / es); }
     void* copy(Space& s, int64_t rows, int c) const { return odd(c) ? s.take(rows * pad(c) * es) : nullptr; }
 };
-inline int64_t part_bytes(const Plan& q, int64_t M, int64_t N, int problems) { return q.splits > 1 ? (int64_t)q.splits * M * N * 4 * problems : 0; }
 
 struct FwdSpace {
     void *xp, *gp, *up, *hp, *dp;
@@ -182,7 +182,7 @@ struct FwdSpace {
     Plan gate, down;
     FwdSpace(const Dims& d, Space& s) : gate(plan_gemm(d.m, 2 * (int64_t)d.n, d.steps(d.k), 1, false)), down(plan_gemm(d.m, d.o, d.steps(d.n), 1, true)) {
         xp = d.copy(s, d.m, d.k); gp = d.copy(s, d.n, d.k); up = d.copy(s, d.n, d.k); hp = d.copy(s, d.m, d.n); dp = d.copy(s, d.o, d.n);
-        part = static_cast<float*>(s.take(part_bytes(down, d.m, d.o, 1)));
+        part = static_cast<float*>(s.take(down.part_bytes()));
     }
 };
 struct BwdSpace {
@@ -190,16 +190,16 @@ struct BwdSpace {
     float *part, *cols[3];
     Plan gate, dx, dw, dwd;
     BwdSpace(const Dims& d, Space& s)
-        : gate(plan_gemm(d.m, d.n, d.steps(d.o), 1, false)), dx(plan_gemm(d.m, d.k, 2 * d.steps(d.n), 1, true)), dw(plan_gemm(d.n, d.k, d.steps(d.m), 2, true)),
+        : gate(plan_gemm(d.m, d.pad(d.n), d.steps(d.o), 1, false)), dx(plan_gemm(d.m, d.k, 2 * d.steps(d.n), 1, true)), dw(plan_gemm(d.n, d.k, d.steps(d.m), 2, true)),
           dwd(plan_gemm(d.o, d.n, d.steps(d.m), 1, true)) {
         dg = s.take(d.m * d.pad(d.n) * d.es);
         du = s.take(d.m * d.pad(d.n) * d.es);
         xp = d.copy(s, d.m, d.k); gp = d.copy(s, d.n, d.k); up = d.copy(s, d.n, d.k); hp = d.copy(s, d.m, d.n); dp = d.copy(s, d.o, d.n); yp = d.copy(s, d.m, d.o);
-        int64_t most = part_bytes(dx, d.m, d.k, 1);
-        if (part_bytes(dw, d.n, d.k, 2) > most) most = part_bytes(dw, d.n, d.k, 2);
-        if (part_bytes(dwd, d.o, d.n, 1) > most) most = part_bytes(dwd, d.o, d.n, 1);
+        int64_t most = dx.part_bytes();
+        if (dw.part_bytes() > most) most = dw.part_bytes();
+        if (dwd.part_bytes() > most) most = dwd.part_bytes();
         part = static_cast<float*>(s.take(most));
-        for (int i = 0; i < 3; ++i) cols[i] = static_cast<float*>(s.take((int64_t)kColBlocks * (i < 2 ? d.n : d.o) * 4));
+        for (int i = 0; i < 3; ++i) cols[i] = static_cast<float*>(s.take(i < 2 ? gate.tiles_m * d.n * 4 : (int64_t)kColBlocks * d.o * 4));
     }
 };
 
@@ -232,14 +232,12 @@ int ffn_fwd(int act, const Dims& d, const void* x, const void* wg, const void* w
     a.b = {{rows_of<T>(wg, s.gp, d.n, d.k, d, st), rows_of<T>(wu, s.up, d.n, d.k, d, st)}, (int64_t)d.pad(d.k) * d.es, d.n};
     a.M = d.m; a.N = d.n; a.K = d.pad(d.k); a.nseg = 1; a.problems = 1; a.ldo = d.n;
     a.bias = bg; a.bias2 = bu; a.gout = g; a.uout = u; a.out[0] = h; a.act = act;
-    a.vec = d.n % 4 == 0 && aligned(h, 4 * d.es) && aligned(g, 4 * d.es) && aligned(u, 4 * d.es);
     if (int rc = gemm_launch<T, T, false, false, EPI_GATE>(a, s.gate, st)) return rc;
     a = GemmArgs{};
     a.a = {{rows_of<T>(h, s.hp, d.m, d.n, d, st), nullptr}, (int64_t)d.pad(d.n) * d.es, d.m};
     a.b = {{rows_of<T>(wd, s.dp, d.o, d.n, d, st), nullptr}, (int64_t)d.pad(d.n) * d.es, d.o};
     a.M = d.m; a.N = d.o; a.K = d.pad(d.n); a.nseg = 1; a.problems = 1; a.ldo = d.o;
     a.bias = bd; a.out[0] = y; a.part = s.part;
-    a.vec = d.o % 4 == 0 && aligned(y, 4 * d.es);
     return gemm_launch<T, T, false, false, EPI_STORE>(a, s.down, st);
 }
 
@@ -257,7 +255,7 @@ int ffn_bwd(int act, const Dims& d, const void* dy, const void* x, const void* w
         a.b = {{rows_of<T>(wd, s.dp, d.o, d.n, d, st), nullptr}, np * es, d.n};
         a.M = d.m; a.N = d.n; a.K = d.o; a.nseg = 1; a.problems = 1; a.ldo = np;
         a.gin = g; a.uin = u; a.gout = s.dg; a.uout = s.du; a.act = act;
-        a.vec = d.n % 4 == 0 && aligned(g, 4 * es) && aligned(u, 4 * es);
+        if (dbg || dbu) { a.cols = s.cols[0]; a.cols2 = s.cols[1]; }
         // (k of dy's rows ends at the padded width: zeros there; rows of wd end at o)
         if (int rc = gemm_launch<T, T, false, true, EPI_GATE_BWD>(a, s.gate, st)) return rc;
         if (dx) {
@@ -266,7 +264,6 @@ int ffn_bwd(int act, const Dims& d, const void* dy, const void* x, const void* w
             a.b = {{rows_of<T>(wg, s.gp, d.n, d.k, d, st), rows_of<T>(wu, s.up, d.n, d.k, d, st)}, kp * es, d.k};
             a.M = d.m; a.N = d.k; a.K = d.n; a.nseg = 2; a.problems = 1; a.ldo = d.k;
             a.out[0] = dx; a.part = s.part;
-            a.vec = d.k % 4 == 0 && aligned(dx, 4 * es);
             if (int rc = gemm_launch<T, T, false, true, EPI_STORE>(a, s.dx, st)) return rc;
         }
         if (dwg) {
@@ -276,14 +273,12 @@ int ffn_bwd(int act, const Dims& d, const void* dy, const void* x, const void* w
             a.b = {{xr, xr}, kp * es, d.k};
             a.M = d.n; a.N = d.k; a.K = d.m; a.nseg = 1; a.problems = 2; a.ldo = d.k;
             a.out[0] = dwg; a.out[1] = dwu; a.part = s.part; a.accumulate = accumulate;
-            a.vec = d.k % 4 == 0 && aligned(dwg, 4 * sizeof(O)) && aligned(dwu, 4 * sizeof(O));
             if (int rc = gemm_launch<T, O, true, true, EPI_STORE>(a, s.dw, st)) return rc;
             a = GemmArgs{};
             a.a = {{dyr, nullptr}, op * es, d.o};
             a.b = {{rows_of<T>(h, s.hp, d.m, d.n, d, st), nullptr}, np * es, d.n};
             a.M = d.o; a.N = d.n; a.K = d.m; a.nseg = 1; a.problems = 1; a.ldo = d.n;
             a.out[0] = dwd; a.part = s.part; a.accumulate = accumulate;
-            a.vec = d.n % 4 == 0 && aligned(dwd, 4 * sizeof(O));
             if (int rc = gemm_launch<T, O, true, true, EPI_STORE>(a, s.dwd, st)) return rc;
         }
     } else if (!accumulate) {                                          // no rows: the gradients are zero
@@ -296,16 +291,20 @@ int ffn_bwd(int act, const Dims& d, const void* dy, const void* x, const void* w
     if (d.m > 0 && (dbg || dbu || dbd)) {
         ColumnJobs q{};
         int widest = 0;
-        auto add = [&](const void* v, int64_t ld, int c, void* out, float* part) {
+        auto add = [&](int c, void* out, const float* part, int blocks) {
             if (!out) return;
-            q.x[q.jobs] = v; q.ld[q.jobs] = ld; q.c[q.jobs] = c; q.out[q.jobs] = out; q.part[q.jobs++] = part;
+            q.c[q.jobs] = c; q.out[q.jobs] = out; q.part[q.jobs] = part; q.blocks[q.jobs++] = blocks;
             widest = c > widest ? c : widest;
         };
-        add(s.dg, np, d.n, dbg, s.cols[0]); add(s.du, np, d.n, dbu, s.cols[1]); add(dy, d.o, d.o, dbd, s.cols[2]);
-        const int64_t per = ceil_div(d.m, ceil_div(d.m, 32) < kColBlocks ? ceil_div(d.m, 32) : kColBlocks);
-        const int blocks = (int)ceil_div(d.m, per);
-        hipLaunchKernelGGL((column_sums<T>), dim3(blocks, (unsigned)ceil_div(widest, 256), q.jobs), dim3(256), 0, st, q, d.m, per);
-        hipLaunchKernelGGL((column_sums_finish<O>), dim3((unsigned)ceil_div(widest, 16), 1, q.jobs), dim3(256), 0, st, q, blocks, accumulate);
+        add(d.n, dbg, s.cols[0], (int)s.gate.tiles_m);
+        add(d.n, dbu, s.cols[1], (int)s.gate.tiles_m);
+        if (dbd) {
+            const int64_t per = ceil_div(d.m, ceil_div(d.m, 32) < kColBlocks ? ceil_div(d.m, 32) : kColBlocks);
+            const int blocks = (int)ceil_div(d.m, per);
+            hipLaunchKernelGGL((column_sums<T>), dim3(blocks, (unsigned)ceil_div(d.o, 256)), dim3(256), 0, st, static_cast<const T*>(dy), d.m, d.o, per, s.cols[2]);
+            add(d.o, dbd, s.cols[2], blocks);
+        }
+        hipLaunchKernelGGL((column_sums_finish<O>), dim3((unsigned)ceil_div(widest, 16), 1, q.jobs), dim3(1024), 0, st, q, accumulate);
     }
     return check_launch("suhpe_gated_ffn_bwd");
 }

@@ -13,6 +13,8 @@
 // Fragment order of k is the same for every layout (lane group g of 16 takes k = 8 g .. 8 g + 7 of 32, fp32: 4 g + e of 16), so results do not depend on it.
 // The weights' side is the FIRST matrix operand: a lane then holds 4 consecutive output columns of one row, stored as one vector.
 
+#include <type_traits>
+
 namespace suhpe {
 namespace {
 
@@ -33,14 +35,19 @@ struct GemmArgs {
     int64_t M;                                                         // output rows
     int N;                                                             // output columns (EPI_GATE: of g, u, h)
     int64_t K;                                                         // reduction of ONE segment
-    int nk, nseg, splits, problems;                                    // steps of a segment; segments; ways the steps are split; independent products
+    int nk, nseg, problems;                                            // steps of a segment; segments; independent products
     int tiles_m, tiles_n;
+    int whole, streams;                                                // tiles that one workgroup reduces alone; workgroups that share the others' steps
     const void *bias, *bias2, *gin, *uin;
     void *out[2], *gout, *uout;                                        // EPI_GATE: out = h; EPI_GATE_BWD: gout = dg, uout = du
     int ldo;                                                           // columns from row to row of what is written (>= N; EPI_GATE_BWD: zeros behind N)
-    int act, accumulate, vec;                                          // vec: rows and pointers allow 4-column vectors
-    float* part;                                                       // splits > 1: [problem][split][M][N]
+    int act, accumulate;
+    float* part;                                                       // streams > 0: [2 streams][BM][BN]
+    float *cols, *cols2;                                               // EPI_GATE_BWD: column sums of dg and du, [row tile][N], or null
 };
+
+// Steps first .. of the shared tiles that stream w takes (the shared tiles' steps, laid end to end, in equal parts)
+__host__ __device__ __forceinline__ int64_t stream_start(int64_t total, int streams, int64_t w) { return total * w / streams; }
 
 template <typename T> struct Mfma;
 template <> struct Mfma<bf16> {
@@ -138,9 +145,34 @@ __device__ __forceinline__ int xcd_order(int bid, int total) {
     return xcd * per + (xcd < extra ? xcd : extra) + i;
 }
 
+// 8 consecutive columns from / to memory (any element address); columns from `limit` on are zeros / left alone
+template <typename T> __device__ __forceinline__ void load8(const T* p, int n, int limit, float (&v)[8]) {
+    if (n + 8 <= limit) {
+        T t[8];
+        __builtin_memcpy(t, p, sizeof t);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (float)t[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = n + e < limit ? (float)p[e] : 0.f;
+    }
+}
+template <typename T> __device__ __forceinline__ void store8(T* p, int n, int limit, const float (&v)[8]) {
+    if (n + 8 <= limit) {
+        T t[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t[e] = (T)v[e];
+        __builtin_memcpy(p, t, sizeof t);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (n + e < limit) p[e] = (T)v[e];
+    }
+}
+
 template <typename T, typename O, int TM, int TN, int WM, int WN, bool AKM, bool BKM, int EPI>
 __global__ __launch_bounds__(64 * WM * WN) void gemm_lowp(const GemmArgs p) {
-    constexpr int BM = 16 * TM * WM, BN = 16 * TN * WN, NW = WM * WN;
+    constexpr int BM = 16 * TM * WM, BN = 16 * TN * WN, NW = WM * WN, NT = 64 * NW;
     using SA = Side<T, BM, AKM>;
     using SB = Side<T, BN, BKM>;
     constexpr int BKE = SA::BKE, CH = SA::CH, KG = 2;                   // k-groups of a step: 2 x 32 (fp32: 2 x 16)
@@ -148,240 +180,310 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_lowp(const GemmArgs p) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
     const int wm = wave / WN, wn = wave % WN;
-
-    // work item: [problem][split][tile group of 8 row tiles x all column tiles]
-    int item = xcd_order(blockIdx.x, gridDim.x);
-    const int tiles = p.tiles_m * p.tiles_n;
-    const int prob = item / (tiles * p.splits);
-    item -= prob * tiles * p.splits;
-    const int split = item / tiles;
-    item -= split * tiles;
-    constexpr int GROUP = 8;
-    const int group = item / (GROUP * p.tiles_n), gm0 = group * GROUP, gsize = p.tiles_m - gm0 < GROUP ? p.tiles_m - gm0 : GROUP;
-    item -= group * GROUP * p.tiles_n;
-    const int64_t m0 = (int64_t)(gm0 + item % gsize) * BM;
-    const int n0 = (item / gsize) * (EPI == EPI_GATE ? BN / 2 : BN);
-    const int steps = p.nk * p.nseg;
-    const int s0 = (int)((int64_t)steps * split / p.splits), s1 = (int)((int64_t)steps * (split + 1) / p.splits);
-
-    // this lane's pieces: byte offset within the step's source rows, and the first k of its chunk (k-major: its row of k) for the tail of the reduction
-    unsigned offa[PA], offb[PB];
-    int ka[PA], kb[PB];
-#pragma unroll
-    for (int i = 0; i < PA; ++i) {
-        int row, chunk;
-        SA::place(wave * PA + i, lane, &row, &chunk);
-        if constexpr (!AKM) {
-            const int64_t r = m0 + row < p.a.rows ? row : p.a.rows - 1 - m0;                    // rows beyond the last repeat it: never stored
-            offa[i] = (unsigned)(r * p.a.ld + chunk * 16);
-            ka[i] = chunk * CH;
-        } else {
-            offa[i] = m0 + chunk * CH < p.a.rows ? (unsigned)(row * p.a.ld + chunk * 16) : kOob;
-            ka[i] = row;
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < PB; ++i) {
-        int row, chunk;
-        SB::place(wave * PB + i, lane, &row, &chunk);
-        if constexpr (!BKM) {
-            if constexpr (EPI == EPI_GATE) row = (row >> 5) * 16 + (row & 15);                  // 16 gate rows, 16 up rows, ...
-            const int64_t r = n0 + row < p.b.rows ? row : p.b.rows - 1 - n0;
-            offb[i] = (unsigned)(r * p.b.ld + chunk * 16);
-            kb[i] = chunk * CH;
-        } else {
-            offb[i] = n0 + chunk * CH < p.b.rows ? (unsigned)(row * p.b.ld + chunk * 16) : kOob;
-            kb[i] = row;
-        }
-    }
     const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
-    auto issue = [&](int s, int stage) __attribute__((always_inline)) {
-        const int seg = s >= p.nk ? 1 : 0, kt = s - seg * p.nk, which = seg + prob;
-        const int64_t k0 = (int64_t)kt * BKE;
-        const int left = (int)(p.K - k0 < BKE ? p.K - k0 : BKE);                                // elements of k in this step
-        const char* pa = p.a.p[which] + (AKM ? k0 * p.a.ld + m0 * SA::ES : m0 * p.a.ld + k0 * SA::ES);
-        unsigned oa[PA], ob[PB];
-#pragma unroll
-        for (int i = 0; i < PA; ++i) oa[i] = ka[i] < left ? offa[i] : kOob;
-#pragma unroll
-        for (int i = 0; i < PB; ++i) ob[i] = kb[i] < left ? offb[i] : kOob;
-        const unsigned la = __builtin_amdgcn_readfirstlane(lds0 + stage * STAGE + wave * PA * 1024);
-        const unsigned lb = __builtin_amdgcn_readfirstlane(lds0 + stage * STAGE + BM * 128 + wave * PB * 1024);
-        dma<PA>(oa, pa, la);
-        if constexpr (EPI == EPI_GATE) {                               // pieces 4 q, 4 q + 1: gate rows; 4 q + 2, 4 q + 3: up rows
-            static_assert(PB == 4 && !BKM, "a wavefront fills whole blocks of 16 gate and 16 up rows");
-            const int64_t at = n0 * p.b.ld + k0 * SB::ES;
-            const unsigned g[2] = {ob[0], ob[1]}, u[2] = {ob[2], ob[3]};
-            dma<2>(g, p.b.p[0] + at, lb);
-            dma<2>(u, p.b.p[1] + at, lb + 2048);
-        } else {
-            const char* pb = p.b.p[which] + (BKM ? k0 * p.b.ld + (int64_t)n0 * SB::ES : n0 * p.b.ld + k0 * SB::ES);
-            dma<PB>(ob, pb, lb);
-        }
-    };
-
-    f32x4 acc[TM][TN];
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     const int basea = SA::lane_base(lane), baseb = SB::lane_base(lane);
-    if (s0 < s1) issue(s0, 0);
-    for (int s = s0; s < s1; ++s) {
-        const int stage = (s - s0) & 1;
-        // this wavefront's DMA of step s has landed and its reads of the other buffer are done; after the barrier that holds for all of them
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (s + 1 < s1) issue(s + 1, stage ^ 1);
-        const char *ta = smem + stage * STAGE, *tb = ta + BM * 128;
-#pragma unroll
-        for (int kk = 0; kk < KG; ++kk) {
-            i32x4 fa[TM], fb[TN];
-#pragma unroll
-            for (int j = 0; j < TN; ++j) fb[j] = SB::read(tb, baseb, lane, wn * TN + j, kk);
-#pragma unroll
-            for (int i = 0; i < TM; ++i) fa[i] = SA::read(ta, basea, lane, wm * TM + i, kk);
-#pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int j = 0; j < TN; ++j) acc[i][j] = Mfma<T>::run(fb[j], fa[i], acc[i][j]);
-        }
-    }
+    const int steps = p.nk * p.nseg, tiles = p.tiles_m * p.tiles_n;
 
-    // ---- epilogue: lane (t, g) holds columns 16 (wn TN + j) + 4 g .. + 3 of row 16 (wm TM + i) + t
-    const int t = lane & 15, g4 = (lane >> 4) * 4;
-    if constexpr (EPI == EPI_GATE) {
+    // this workgroup's share: one whole tile, or a range of the shared tiles' steps (pieces of at most two tiles and whole ones between them)
+    int64_t at, end;
+    int stream = -1;
+    if ((int)blockIdx.x < p.whole) {
+        at = (int64_t)xcd_order(blockIdx.x, p.whole) * steps;
+        end = at + steps;
+    } else {
+        const int64_t total = ((int64_t)tiles * p.problems - p.whole) * steps;
+        stream = xcd_order(blockIdx.x - p.whole, p.streams);
+        at = (int64_t)p.whole * steps + stream_start(total, p.streams, stream);
+        end = (int64_t)p.whole * steps + stream_start(total, p.streams, stream + 1);
+    }
+    for (int piece = 0; at < end; piece = 1) {
+        int item = (int)(at / steps);
+        const int s0 = (int)(at - (int64_t)item * steps), s1 = (int)(end - at < steps - s0 ? s0 + (end - at) : steps);
+        at += s1 - s0;
+        const bool complete = s0 == 0 && s1 == steps;
+        const int prob = item / tiles;
+        item -= prob * tiles;
+        // tiles in groups of 8 rows of tiles x all columns: neighbours in the order share operands in L2
+        constexpr int GROUP = 8;
+        const int group = item / (GROUP * p.tiles_n), gm0 = group * GROUP, gsize = p.tiles_m - gm0 < GROUP ? p.tiles_m - gm0 : GROUP;
+        item -= group * GROUP * p.tiles_n;
+        const int tile_m = gm0 + item % gsize;
+        const int64_t m0 = (int64_t)tile_m * BM;
+        const int n0 = (item / gsize) * (EPI == EPI_GATE ? BN / 2 : BN);
+
+        // this lane's pieces: byte offset within the step's source rows, and the first k of its chunk (k-major: its row of k) for the tail of the reduction
+        unsigned offa[PA], offb[PB];
+        int ka[PA], kb[PB];
 #pragma unroll
-        for (int j = 0; j < TN; j += 2) {
-            const int n = n0 + (wn * TN + j) * 8 + g4;
-            float bg[4], bu[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const bool ok = n + r < p.N;
-                bg[r] = ok && p.bias ? (float)static_cast<const T*>(p.bias)[n + r] : 0.f;
-                bu[r] = ok && p.bias2 ? (float)static_cast<const T*>(p.bias2)[n + r] : 0.f;
-            }
-#pragma unroll
-            for (int i = 0; i < TM; ++i) {
-                const int64_t m = m0 + (wm * TM + i) * 16 + t;
-                if (m >= p.M || n >= p.N) continue;
-                float gv[4], uv[4], hv[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    gv[r] = acc[i][j][r] + bg[r];
-                    uv[r] = acc[i][j + 1][r] + bu[r];
-                    hv[r] = act_apply(gv[r], p.act) * uv[r];
-                }
-                const int64_t at = m * p.ldo + n;
-                T *go = static_cast<T*>(p.gout), *uo = static_cast<T*>(p.uout), *ho = static_cast<T*>(p.out[0]);
-                if (p.vec) {
-                    if (go) { store_n<T, 4>(go + at, gv); store_n<T, 4>(uo + at, uv); }
-                    store_n<T, 4>(ho + at, hv);
-                } else {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (n + r < p.N) {
-                            if (go) { go[at + r] = (T)gv[r]; uo[at + r] = (T)uv[r]; }
-                            ho[at + r] = (T)hv[r];
-                        }
-                }
+        for (int i = 0; i < PA; ++i) {
+            int row, chunk;
+            SA::place(wave * PA + i, lane, &row, &chunk);
+            if constexpr (!AKM) {
+                const int64_t r = m0 + row < p.a.rows ? row : p.a.rows - 1 - m0;                // rows beyond the last repeat it: never stored
+                offa[i] = (unsigned)(r * p.a.ld + chunk * 16);
+                ka[i] = chunk * CH;
+            } else {
+                offa[i] = m0 + chunk * CH < p.a.rows ? (unsigned)(row * p.a.ld + chunk * 16) : kOob;
+                ka[i] = row;
             }
         }
-    } else if constexpr (EPI == EPI_GATE_BWD) {
 #pragma unroll
-        for (int j = 0; j < TN; ++j) {
-            const int n = n0 + (wn * TN + j) * 16 + g4;
+        for (int i = 0; i < PB; ++i) {
+            int row, chunk;
+            SB::place(wave * PB + i, lane, &row, &chunk);
+            if constexpr (!BKM) {
+                if constexpr (EPI == EPI_GATE) row = (row >> 5) * 16 + (row & 15);              // 16 gate rows, 16 up rows, ...
+                const int64_t r = n0 + row < p.b.rows ? row : p.b.rows - 1 - n0;
+                offb[i] = (unsigned)(r * p.b.ld + chunk * 16);
+                kb[i] = chunk * CH;
+            } else {
+                offb[i] = n0 + chunk * CH < p.b.rows ? (unsigned)(row * p.b.ld + chunk * 16) : kOob;
+                kb[i] = row;
+            }
+        }
+        auto issue = [&](int s, int stage) __attribute__((always_inline)) {
+            const int seg = s >= p.nk ? 1 : 0, kt = s - seg * p.nk, which = seg + prob;
+            const int64_t k0 = (int64_t)kt * BKE;
+            const int left = (int)(p.K - k0 < BKE ? p.K - k0 : BKE);                            // elements of k in this step
+            const char* pa = p.a.p[which] + (AKM ? k0 * p.a.ld + m0 * SA::ES : m0 * p.a.ld + k0 * SA::ES);
+            unsigned oa[PA], ob[PB];
 #pragma unroll
-            for (int i = 0; i < TM; ++i) {
-                const int64_t m = m0 + (wm * TM + i) * 16 + t;
-                if (m >= p.M || n >= p.ldo) continue;
-                float gv[4], uv[4], dg[4], du[4];
-                const T *gi = static_cast<const T*>(p.gin) + m * p.N + n, *ui = static_cast<const T*>(p.uin) + m * p.N + n;
-                if (p.vec) {
-                    load_n<T, 4>(gi, gv);
-                    load_n<T, 4>(ui, uv);
-                } else {
+            for (int i = 0; i < PA; ++i) oa[i] = ka[i] < left ? offa[i] : kOob;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        gv[r] = n + r < p.N ? (float)gi[r] : 0.f;
-                        uv[r] = n + r < p.N ? (float)ui[r] : 0.f;
+            for (int i = 0; i < PB; ++i) ob[i] = kb[i] < left ? offb[i] : kOob;
+            const unsigned la = __builtin_amdgcn_readfirstlane(lds0 + stage * STAGE + wave * PA * 1024);
+            const unsigned lb = __builtin_amdgcn_readfirstlane(lds0 + stage * STAGE + BM * 128 + wave * PB * 1024);
+            dma<PA>(oa, pa, la);
+            if constexpr (EPI == EPI_GATE) {                           // pieces 4 q, 4 q + 1: gate rows; 4 q + 2, 4 q + 3: up rows
+                static_assert(PB == 4 && !BKM, "a wavefront fills whole blocks of 16 gate and 16 up rows");
+                const int64_t off = n0 * p.b.ld + k0 * SB::ES;
+                const unsigned g[2] = {ob[0], ob[1]}, u[2] = {ob[2], ob[3]};
+                dma<2>(g, p.b.p[0] + off, lb);
+                dma<2>(u, p.b.p[1] + off, lb + 2048);
+            } else {
+                const char* pb = p.b.p[which] + (BKM ? k0 * p.b.ld + (int64_t)n0 * SB::ES : n0 * p.b.ld + k0 * SB::ES);
+                dma<PB>(ob, pb, lb);
+            }
+        };
+
+        f32x4 acc[TM][TN];
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (piece) __syncthreads();                                    // the previous piece's results have left LDS
+        issue(s0, 0);
+        for (int s = s0; s < s1; ++s) {
+            const int stage = (s - s0) & 1;
+            // this wavefront's DMA of step s has landed and its reads of the other buffer are done; after the barrier that holds for all of them
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (s + 1 < s1) issue(s + 1, stage ^ 1);
+            const char *ta = smem + stage * STAGE, *tb = ta + BM * 128;
+#pragma unroll
+            for (int kk = 0; kk < KG; ++kk) {
+                i32x4 fa[TM], fb[TN];
+#pragma unroll
+                for (int j = 0; j < TN; ++j) fb[j] = SB::read(tb, baseb, lane, wn * TN + j, kk);
+#pragma unroll
+                for (int i = 0; i < TM; ++i) fa[i] = SA::read(ta, basea, lane, wm * TM + i, kk);
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) acc[i][j] = Mfma<T>::run(fb[j], fa[i], acc[i][j]);
+            }
+        }
+
+        // ---- epilogue.  A lane holds 4 columns of a row (8 bytes of a 16-bit row): the sums go through LDS, 64 rows of each row of wavefronts at a time, and come
+        // back as 8 columns of one row per thread, neighbouring threads side by side: whole 128-byte lines to memory.  16-byte chunk c of a staged row lies at
+        // c ^ (row & 15): the 16 rows of a write pass and the 2 rows of a read pass cover the banks once.
+        constexpr int CHUNKS = TM / 4, ROWS = 64 * WM, PITCH = BN * 4;
+        static_assert(TM % 4 == 0 && ROWS * PITCH <= 2 * STAGE, "a chunk fits the two stages");
+        const int t = lane & 15, g4 = lane >> 4;
+        constexpr int WIDE = EPI == EPI_GATE ? BN / 2 : BN, LANES = WIDE / 8, RPP = NT / LANES, PASSES = ROWS / RPP;
+        const int cg = threadIdx.x % LANES, r0 = threadIdx.x / LANES, n = n0 + cg * 8;
+        const int limit = EPI == EPI_GATE_BWD ? p.ldo : p.N;
+        float b1[8], b2[8], c1[8], c2[8];
+        if constexpr (EPI == EPI_GATE_BWD) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) c1[e] = c2[e] = 0.f;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) b1[e] = b2[e] = 0.f;
+            if (p.bias && n < limit) load8(static_cast<const T*>(p.bias) + n, n, limit, b1);
+            if (EPI == EPI_GATE && p.bias2 && n < limit) load8(static_cast<const T*>(p.bias2) + n, n, limit, b2);
+        }
+        auto finish = [&](auto which_chunk) __attribute__((always_inline)) {
+            constexpr int chunk = decltype(which_chunk)::value;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) {
+                    const int c = (wn * TN + j) * 4 + g4;
+                    *reinterpret_cast<f32x4*>(smem + (wm * 64 + i * 16 + t) * PITCH + ((c ^ t) << 4)) = acc[chunk * 4 + i][j];
+                }
+            __syncthreads();
+            auto staged = [&](int r, int col, float (&v)[8]) __attribute__((always_inline)) {
+                const char* row = smem + r * PITCH;
+                const int c = col >> 2;
+                const f32x4 lo = *reinterpret_cast<const f32x4*>(row + ((c ^ (r & 15)) << 4)), hi = *reinterpret_cast<const f32x4*>(row + (((c + 1) ^ (r & 15)) << 4));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { v[e] = lo[e]; v[4 + e] = hi[e]; }
+            };
+            auto row_of = [&](int r) { return m0 + (r >> 6) * (16 * TM) + chunk * 64 + (r & 63); };
+            if constexpr (EPI == EPI_GATE) {
+#pragma unroll
+                for (int q = 0; q < PASSES; ++q) {
+                    const int r = r0 + q * RPP;
+                    const int64_t m = row_of(r);
+                    if (m >= p.M || n >= limit) continue;
+                    float gv[8], uv[8], hv[8];
+                    const int col = (cg >> 1) * 32 + (cg & 1) * 8;     // 16 gate columns, 16 up columns, ...
+                    staged(r, col, gv);
+                    staged(r, col + 16, uv);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        gv[e] += b1[e];
+                        uv[e] += b2[e];
+                        hv[e] = act_apply(gv[e], p.act) * uv[e];
+                    }
+                    const int64_t o = m * p.ldo + n;
+                    if (p.gout) {
+                        store8(static_cast<T*>(p.gout) + o, n, limit, gv);
+                        store8(static_cast<T*>(p.uout) + o, n, limit, uv);
+                    }
+                    store8(static_cast<T*>(p.out[0]) + o, n, limit, hv);
+                }
+            } else if constexpr (EPI == EPI_GATE_BWD) {
+                constexpr int BATCH = 16 / (int)sizeof(T) / 2;          // rows whose g and u are in flight together
+                static_assert(PASSES % BATCH == 0, "");
+#pragma unroll 1
+                for (int q0 = 0; q0 < PASSES; q0 += BATCH) {
+                    T gr[BATCH][8], ur[BATCH][8];
+#pragma unroll
+                    for (int q = 0; q < BATCH; ++q) {
+                        const int64_t m = row_of(r0 + (q0 + q) * RPP), o = m * p.N + n;
+                        const T *gi = static_cast<const T*>(p.gin) + o, *ui = static_cast<const T*>(p.uin) + o;
+                        if (m < p.M && n + 8 <= p.N) {
+                            __builtin_memcpy(gr[q], gi, sizeof gr[q]);
+                            __builtin_memcpy(ur[q], ui, sizeof ur[q]);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const bool ok = m < p.M && n + e < p.N;
+                                gr[q][e] = ok ? gi[e] : (T)0.f;
+                                ur[q][e] = ok ? ui[e] : (T)0.f;
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int q = 0; q < BATCH; ++q) {
+                        const int r = r0 + (q0 + q) * RPP;
+                        const int64_t m = row_of(r);
+                        if (m >= p.M || n >= limit) continue;
+                        float dh[8], dg[8], du[8];
+                        staged(r, cg * 8, dh);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const float gv = (float)gr[q][e], uv = (float)ur[q][e];
+                            const bool ok = n + e < p.N;               // (columns of padding are written as zeros)
+                            dg[e] = ok ? dh[e] * uv * act_grad(gv, p.act) : 0.f;
+                            du[e] = ok ? dh[e] * act_apply(gv, p.act) : 0.f;
+                            c1[e] += dg[e];
+                            c2[e] += du[e];
+                        }
+                        const int64_t o = m * p.ldo + n;
+                        store8(static_cast<T*>(p.gout) + o, n, limit, dg);
+                        store8(static_cast<T*>(p.uout) + o, n, limit, du);
                     }
                 }
+            } else {
+#pragma unroll 2
+                for (int q = 0; q < PASSES; ++q) {
+                    const int r = r0 + q * RPP;
+                    float v[8];
+                    staged(r, cg * 8, v);
+                    if (!complete) {                                    // a shared tile's piece: the first tile of the stream in slot 2 w, the last in 2 w + 1
+                        float* o = p.part + ((int64_t)(2 * stream + piece) * BM + (r >> 6) * (16 * TM) + chunk * 64 + (r & 63)) * BN + cg * 8;
+                        __builtin_memcpy(o, v, sizeof v);
+                        continue;
+                    }
+                    const int64_t m = row_of(r);
+                    if (m >= p.M || n >= limit) continue;
+                    O* o = static_cast<O*>(p.out[prob]) + m * p.ldo + n;
+                    float old[8];
+                    if (p.accumulate) load8(o, n, limit, old);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const bool ok = n + r < p.N;                       // (columns of padding are written as zeros)
-                    dg[r] = ok ? acc[i][j][r] * uv[r] * act_grad(gv[r], p.act) : 0.f;
-                    du[r] = ok ? acc[i][j][r] * act_apply(gv[r], p.act) : 0.f;
-                }
-                const int64_t at = m * p.ldo + n;                      // (ldo is a multiple of 4)
-                store_n<T, 4>(static_cast<T*>(p.gout) + at, dg);
-                store_n<T, 4>(static_cast<T*>(p.uout) + at, du);
-            }
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < TN; ++j) {
-            const int n = n0 + (wn * TN + j) * 16 + g4;
-            float b[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) b[r] = p.bias && n + r < p.N ? (float)static_cast<const T*>(p.bias)[n + r] : 0.f;
-#pragma unroll
-            for (int i = 0; i < TM; ++i) {
-                const int64_t m = m0 + (wm * TM + i) * 16 + t;
-                if (m >= p.M || n >= p.N) continue;
-                float v[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] = acc[i][j][r];
-                if (p.splits > 1) {
-                    float* o = p.part + (((int64_t)prob * p.splits + split) * p.M + m) * p.N + n;
-                    if ((p.N & 3) == 0) store_n<float, 4>(o, v);
-                    else
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (n + r < p.N) o[r] = v[r];
-                    continue;
-                }
-                O* o = static_cast<O*>(p.out[prob]) + m * p.ldo + n;
-                if (p.vec) {
-                    float old[4];
-                    if (p.accumulate) load_n<O, 4>(o, old);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) v[r] += p.accumulate ? old[r] : b[r];
-                    store_n<O, 4>(o, v);
-                } else {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (n + r < p.N) o[r] = (O)(p.accumulate ? (float)o[r] + v[r] : v[r] + b[r]);
+                    for (int e = 0; e < 8; ++e) v[e] += p.accumulate ? old[e] : b1[e];
+                    store8(o, n, limit, v);
                 }
             }
-        }
+        };
+        finish(std::integral_constant<int, 0>{});
+        if constexpr (CHUNKS == 2) finish(std::integral_constant<int, 1>{});
+        static_assert(CHUNKS <= 2, "");
+        if constexpr (EPI == EPI_GATE_BWD)
+            if (p.cols) {                                               // the tile's column sums of dg and du: RPP partial sums per column, in order
+                float* red = reinterpret_cast<float*>(smem);
+                __syncthreads();
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    red[r0 * BN + cg * 8 + e] = c1[e];
+                    red[(RPP + r0) * BN + cg * 8 + e] = c2[e];
+                }
+                __syncthreads();
+                for (int i = threadIdx.x; i < 2 * BN; i += NT) {
+                    const int which = i / BN, c = i - which * BN;
+                    float sum = 0.f;
+#pragma unroll
+                    for (int r = 0; r < RPP; ++r) sum += red[(which * RPP + r) * BN + c];
+                    if (n0 + c < p.N) (which ? p.cols2 : p.cols)[(int64_t)tile_m * p.N + n0 + c] = sum;
+                }
+            }
     }
 }
 
-// out[m][n] = sum over the splits, in order [+ bias[n]] [+ out]
-template <typename T, typename O, int V>
-__global__ __launch_bounds__(256) void gemm_lowp_join(const float* __restrict__ part, int splits, int64_t M, int N, const T* __restrict__ bias, O* out0, O* out1, int accumulate) {
-    const int64_t total = M * N;
-    const float* src = part + (int64_t)blockIdx.y * splits * total;
-    O* out = blockIdx.y ? out1 : out0;
-    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V; i < total; i += (int64_t)gridDim.x * 256 * V) {
-        float s[V], v[V];
-        load_n<float, V>(src + i, s);
-        for (int z = 1; z < splits; ++z) {
-            load_n<float, V>(src + z * total + i, v);
+// The shared tiles: out[m][n] = sum of the pieces, in the order of k [+ bias[n]] [+ out].  Grid: (shared tiles, slices of a tile's rows)
+template <typename T, typename O, int BM, int BN>
+__global__ __launch_bounds__(256) void gemm_lowp_join(const GemmArgs p) {
+    const int steps = p.nk * p.nseg, tiles = p.tiles_m * p.tiles_n;
+    const int64_t total = ((int64_t)tiles * p.problems - p.whole) * steps, lo = (int64_t)blockIdx.x * steps, hi = lo + steps;
+    int64_t w0 = lo * p.streams / total;                                // the stream that holds step lo
+    while (w0 > 0 && stream_start(total, p.streams, w0) > lo) --w0;
+    while (stream_start(total, p.streams, w0 + 1) <= lo) ++w0;
+    if (stream_start(total, p.streams, w0) <= lo && stream_start(total, p.streams, w0 + 1) >= hi) return;      // one stream had it all
+    int item = (int)blockIdx.x + p.whole;
+    const int prob = item / tiles;
+    item -= prob * tiles;
+    constexpr int GROUP = 8, LANES = BN / 8, RPP = 256 / LANES;
+    const int group = item / (GROUP * p.tiles_n), gm0 = group * GROUP, gsize = p.tiles_m - gm0 < GROUP ? p.tiles_m - gm0 : GROUP;
+    item -= group * GROUP * p.tiles_n;
+    const int64_t m0 = (int64_t)(gm0 + item % gsize) * BM;
+    const int n0 = (item / gsize) * BN, cg = threadIdx.x % LANES, n = n0 + cg * 8;
+    if (n >= p.N) return;
+    const int rows = BM / gridDim.y;
+    for (int r = blockIdx.y * rows + threadIdx.x / LANES; r < (int)(blockIdx.y + 1) * rows; r += RPP) {
+        const int64_t m = m0 + r;
+        if (m >= p.M) return;
+        float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, v[8];
+        for (int64_t w = w0; w < p.streams && stream_start(total, p.streams, w) < hi; ++w) {
+            const bool first = stream_start(total, p.streams, w) / steps == (int64_t)blockIdx.x;
+            __builtin_memcpy(v, p.part + ((2 * w + (first ? 0 : 1)) * BM + r) * BN + cg * 8, sizeof v);
 #pragma unroll
-            for (int r = 0; r < V; ++r) s[r] += v[r];
+            for (int e = 0; e < 8; ++e) s[e] += v[e];
         }
-        if (bias) {
-            const int n = (int)(i % N);
+        if (p.bias) {
+            load8(static_cast<const T*>(p.bias) + n, n, p.N, v);
 #pragma unroll
-            for (int r = 0; r < V; ++r) s[r] += (float)bias[n + r];
+            for (int e = 0; e < 8; ++e) s[e] += v[e];
         }
-        if (accumulate) {
-            load_n<O, V>(out + i, v);
+        O* o = static_cast<O*>(p.out[prob]) + m * p.ldo + n;
+        if (p.accumulate) {
+            load8(o, n, p.N, v);
 #pragma unroll
-            for (int r = 0; r < V; ++r) s[r] = v[r] + s[r];
+            for (int e = 0; e < 8; ++e) s[e] += v[e];
         }
-        store_n<O, V>(out + i, s);
+        store8(o, n, p.N, s);
     }
 }
 
@@ -401,53 +503,67 @@ __global__ __launch_bounds__(256) void pad_rows(const T* __restrict__ src, int64
 }
 
 // ------------------------------------------------------------------------------------------ host side
-struct Plan { int big, splits; };                                      // tile 256 x 256 or 128 x 128; ways the reduction is split
+struct Plan {
+    int big, whole, streams;
+    int64_t tiles_m, tiles_n;
+    int64_t part_bytes() const { return streams ? (int64_t)2 * streams * (big ? 256 * 256 : 128 * 128) * 4 : 0; }
+};
 
-// 256 x 256 tiles keep the matrix units fed from LDS best but leave one workgroup per CU: taken where there are enough of them for the 256 CUs and the
-// reduction is long enough to pay for filling and draining one.  Few tiles: the reduction is split so that about two workgroups per CU run.
-inline Plan plan_gemm(int64_t M, int64_t N, int64_t steps, int problems, bool splittable) {
-    Plan q{0, 1};
-    if (M == 0) return q;
-    const int64_t big = ceil_div(M, 256) * ceil_div(N, 256) * problems;
-    const int64_t small = ceil_div(M, 128) * ceil_div(N, 128) * problems;
-    if (big >= 200 && steps >= 16) q.big = 1;
-    else if (splittable && small < 384) {
-        int64_t s = 512 / small;
-        if (s > steps / 8) s = steps / 8;
-        if (s > 64) s = 64;
-        q.splits = s < 1 ? 1 : (int)s;
+// Tile: 256 x 256 (one workgroup of 8 wavefronts per CU) or 128 x 128 (4 wavefronts, two workgroups per CU).  A step of a large tile takes about 1.9 us on the
+// full chip, a step of two small ones 1.1 us for half the work; filling the pipeline and storing costs about 6 and 3 us.  Whichever the sizes make cheaper by
+// that count, padding of the last tiles and the last round of workgroups included, is taken.
+// Shared tiles (products whose epilogue is linear): the tiles beyond the last full round are cut along k, their steps laid end to end and dealt out evenly, at
+// least 8 to a workgroup; the pieces are summed by a second launch in the order of k.  2 x 5632 x 2048 weight gradients over 16384 rows: 352 tiles take 2 rounds of
+// 256 (31 % idle), shared 1.375.
+inline Plan plan_gemm(int64_t M, int64_t N, int64_t steps, int problems, bool share) {
+    Plan best{};
+    if (M == 0) return best;
+    double best_us = 0.;
+    for (int big = 0; big < 2; ++big) {
+        const int64_t b = big ? 256 : 128, slots = big ? 256 : 512;
+        Plan q{big, 0, 0, ceil_div(M, b), ceil_div(N, b)};
+        const int64_t tiles = q.tiles_m * q.tiles_n * problems, rounds = tiles / slots, rest = tiles - rounds * slots;
+        const double step = big ? 1.9 : 1.1, ends = big ? 6. : 3.;
+        double us = (double)rounds * ((double)steps * step + ends);
+        // alone, the rest runs as long as a full round (the two small tiles of a CU at least share it); shared, its part plus the pieces' way through memory
+        const double alone = (double)steps * step * (big || rest > slots / 2 ? 1. : 0.6) + ends;
+        int64_t w = rest * steps / 8;
+        if (w > slots) w = slots;
+        const double shared = w > 0 ? (double)(rest * steps) / (double)w * step + 2 * ends + (double)w * 2 * (big ? 0.262 : 0.0655) * 2 / 4. : 1e30;
+        if (rest == 0) q.whole = (int)tiles;
+        else if (share && w > rest && shared < alone) { q.whole = (int)(rounds * slots); q.streams = (int)w; us += shared; }
+        else { q.whole = (int)tiles; us += alone; }
+        if (!big || us < best_us) { best = q; best_us = us; }
     }
-    return q;
+    return best;
 }
 
 template <typename T, typename O, bool AKM, bool BKM, int EPI>
-int gemm_launch(GemmArgs a, Plan q, hipStream_t st) {
-    const int bm = q.big ? 256 : 128, bn = EPI == EPI_GATE ? bm / 2 : bm;
-    a.tiles_m = (int)ceil_div(a.M, bm);
-    a.tiles_n = (int)ceil_div(EPI == EPI_GATE_BWD ? a.ldo : a.N, bn);
-    a.splits = q.splits;
+int gemm_launch(GemmArgs a, const Plan& q, hipStream_t st) {
+    const int bm = q.big ? 256 : 128;
+    a.tiles_m = (int)q.tiles_m;
+    a.tiles_n = (int)q.tiles_n;
+    a.whole = q.whole;
+    a.streams = q.streams;
     a.nk = (int)ceil_div(a.K, 128 / (int)sizeof(T));
-    const int64_t grid = (int64_t)a.tiles_m * a.tiles_n * a.splits * a.problems;
-    SUHPE_REQUIRE(grid < 0x7fffffff, "gated_ffn: too many tiles");
+    SUHPE_REQUIRE(q.tiles_m * q.tiles_n * a.problems < 0x7fffffff, "gated_ffn: too many tiles");
     const int lds = 2 * (bm + bm) * 128;                               // two stages of 128 bytes per row of either side
+    const dim3 grid((unsigned)(q.whole + q.streams));
     if (q.big) {
         auto k = gemm_lowp<T, O, 8, 4, 2, 4, AKM, BKM, EPI>;
         (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-        hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(512), lds, st, a);
+        hipLaunchKernelGGL(k, grid, dim3(512), lds, st, a);
     } else {
         auto k = gemm_lowp<T, O, 4, 4, 2, 2, AKM, BKM, EPI>;
         (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-        hipLaunchKernelGGL(k, dim3((unsigned)grid), dim3(256), lds, st, a);
+        hipLaunchKernelGGL(k, grid, dim3(256), lds, st, a);
     }
-    if (q.splits > 1) {
-        const int64_t total = a.M * a.N;
-        const bool v4 = (a.N & 3) == 0 && aligned(a.out[0], 4 * sizeof(O)) && aligned(a.out[1], 4 * sizeof(O));
-        const dim3 g(grid_for(ceil_div(total, v4 ? 4 : 1), 256), a.problems);
-        if (v4) hipLaunchKernelGGL((gemm_lowp_join<T, O, 4>), g, dim3(256), 0, st, a.part, q.splits, a.M, a.N, static_cast<const T*>(a.bias), static_cast<O*>(a.out[0]),
-                                   static_cast<O*>(a.out[1]), a.accumulate);
-        else hipLaunchKernelGGL((gemm_lowp_join<T, O, 1>), g, dim3(256), 0, st, a.part, q.splits, a.M, a.N, static_cast<const T*>(a.bias), static_cast<O*>(a.out[0]),
-                                static_cast<O*>(a.out[1]), a.accumulate);
-    }
+    if constexpr (EPI == EPI_STORE)
+        if (q.streams) {
+            const unsigned rest = (unsigned)(q.tiles_m * q.tiles_n * a.problems - q.whole);
+            if (q.big) hipLaunchKernelGGL((gemm_lowp_join<T, O, 256, 256>), dim3(rest, 16), dim3(256), 0, st, a);
+            else hipLaunchKernelGGL((gemm_lowp_join<T, O, 128, 128>), dim3(rest, 8), dim3(256), 0, st, a);
+        }
     return check_launch("gated_ffn: product");
 }
 
