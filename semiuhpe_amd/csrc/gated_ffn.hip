@@ -180,7 +180,7 @@ struct FwdSpace {
     void *xp, *gp, *up, *hp, *dp;
     float* part;
     Plan gate, down;
-    FwdSpace(const Dims& d, Space& s) : gate(plan_gemm(d.m, 2 * (int64_t)d.n, d.steps(d.k), 1, false)), down(plan_gemm(d.m, d.o, d.steps(d.n), 1, true)) {
+    FwdSpace(const Dims& d, Space& s) : gate(plan_gemm(d.m, 2 * (int64_t)d.n, d.steps(d.k), false)), down(plan_gemm(d.m, d.o, d.steps(d.n), true)) {
         xp = d.copy(s, d.m, d.k); gp = d.copy(s, d.n, d.k); up = d.copy(s, d.n, d.k); hp = d.copy(s, d.m, d.n); dp = d.copy(s, d.o, d.n);
         part = static_cast<float*>(s.take(down.part_bytes()));
     }
@@ -188,18 +188,16 @@ struct FwdSpace {
 struct BwdSpace {
     void *dg, *du, *xp, *gp, *up, *hp, *dp, *yp;
     float *part, *cols[3];
-    Plan gate, dx, dw, dwd;
-    BwdSpace(const Dims& d, Space& s)
-        : gate(plan_gemm(d.m, d.pad(d.n), d.steps(d.o), 1, false)), dx(plan_gemm(d.m, d.k, 2 * d.steps(d.n), 1, true)), dw(plan_gemm(d.n, d.k, d.steps(d.m), 2, true)),
-          dwd(plan_gemm(d.o, d.n, d.steps(d.m), 1, true)) {
+    Plan gate, dx, dw;
+    int64_t gate_rows(const Dims& d) const { return ceil_div(d.m, gate.big ? 256 : 128); }
+    BwdSpace(const Dims& d, Space& s) : gate(plan_gemm(d.m, d.pad(d.n), d.steps(d.o), false)), dx(plan_gemm(d.m, d.k, 2 * d.steps(d.n), true)) {
+        const int64_t mn[3][2] = {{d.n, d.k}, {d.n, d.k}, {d.o, d.n}};
+        dw = plan_gemm(3, mn, d.steps(d.m), true);
         dg = s.take(d.m * d.pad(d.n) * d.es);
         du = s.take(d.m * d.pad(d.n) * d.es);
         xp = d.copy(s, d.m, d.k); gp = d.copy(s, d.n, d.k); up = d.copy(s, d.n, d.k); hp = d.copy(s, d.m, d.n); dp = d.copy(s, d.o, d.n); yp = d.copy(s, d.m, d.o);
-        int64_t most = dx.part_bytes();
-        if (dw.part_bytes() > most) most = dw.part_bytes();
-        if (dwd.part_bytes() > most) most = dwd.part_bytes();
-        part = static_cast<float*>(s.take(most));
-        for (int i = 0; i < 3; ++i) cols[i] = static_cast<float*>(s.take(i < 2 ? gate.tiles_m * d.n * 4 : (int64_t)kColBlocks * d.o * 4));
+        part = static_cast<float*>(s.take(dx.part_bytes() > dw.part_bytes() ? dx.part_bytes() : dw.part_bytes()));
+        for (int i = 0; i < 3; ++i) cols[i] = static_cast<float*>(s.take(i < 2 ? gate_rows(d) * d.n * 4 : (int64_t)kColBlocks * d.o * 4));
     }
 };
 
@@ -227,18 +225,17 @@ int ffn_fwd(int act, const Dims& d, const void* x, const void* wg, const void* w
     }
     Space space{static_cast<char*>(workspace)};
     const FwdSpace s(d, space);
+    const int64_t kp = (int64_t)d.pad(d.k) * d.es, np = (int64_t)d.pad(d.n) * d.es;
     GemmArgs a{};
-    a.a = {{rows_of<T>(x, s.xp, d.m, d.k, d, st), nullptr}, (int64_t)d.pad(d.k) * d.es, d.m};
-    a.b = {{rows_of<T>(wg, s.gp, d.n, d.k, d, st), rows_of<T>(wu, s.up, d.n, d.k, d, st)}, (int64_t)d.pad(d.k) * d.es, d.n};
-    a.M = d.m; a.N = d.n; a.K = d.pad(d.k); a.nseg = 1; a.problems = 1; a.ldo = d.n;
-    a.bias = bg; a.bias2 = bu; a.gout = g; a.uout = u; a.out[0] = h; a.act = act;
-    if (int rc = gemm_launch<T, T, false, false, EPI_GATE>(a, s.gate, st)) return rc;
+    a.pr[0] = {{rows_of<T>(x, s.xp, d.m, d.k, d, st), nullptr}, {rows_of<T>(wg, s.gp, d.n, d.k, d, st), rows_of<T>(wu, s.up, d.n, d.k, d, st)}, kp, kp, d.m, d.n, d.n, h, 0, 0};
+    a.K = d.pad(d.k); a.nseg = 1;
+    a.bias = bg; a.bias2 = bu; a.gout = g; a.uout = u; a.act = act;
+    if (int rc = gemm_launch<T, T, false, false, EPI_GATE>(a, 1, s.gate, st)) return rc;
     a = GemmArgs{};
-    a.a = {{rows_of<T>(h, s.hp, d.m, d.n, d, st), nullptr}, (int64_t)d.pad(d.n) * d.es, d.m};
-    a.b = {{rows_of<T>(wd, s.dp, d.o, d.n, d, st), nullptr}, (int64_t)d.pad(d.n) * d.es, d.o};
-    a.M = d.m; a.N = d.o; a.K = d.pad(d.n); a.nseg = 1; a.problems = 1; a.ldo = d.o;
-    a.bias = bd; a.out[0] = y; a.part = s.part;
-    return gemm_launch<T, T, false, false, EPI_STORE>(a, s.down, st);
+    a.pr[0] = {{rows_of<T>(h, s.hp, d.m, d.n, d, st), nullptr}, {rows_of<T>(wd, s.dp, d.o, d.n, d, st), nullptr}, np, np, d.m, d.o, d.o, y, 0, 0};
+    a.K = d.pad(d.n); a.nseg = 1;
+    a.bias = bd; a.part = s.part;
+    return gemm_launch<T, T, false, false, EPI_STORE>(a, 1, s.down, st);
 }
 
 template <typename T, typename O>
@@ -246,40 +243,29 @@ int ffn_bwd(int act, const Dims& d, const void* dy, const void* x, const void* w
             void* dwu, void* dwd, void* dbg, void* dbu, void* dbd, int accumulate, void* workspace, hipStream_t st) {
     Space space{static_cast<char*>(workspace)};
     const BwdSpace s(d, space);
-    const int np = d.pad(d.n), kp = d.pad(d.k), op = d.pad(d.o);
-    const int64_t es = d.es;
+    const int64_t np = (int64_t)d.pad(d.n) * d.es, kp = (int64_t)d.pad(d.k) * d.es, op = (int64_t)d.pad(d.o) * d.es;
     if (d.m > 0) {
-        const char* dyr = rows_of<T>(dy, s.yp, d.m, d.o, d, st);
+        const char *dyr = rows_of<T>(dy, s.yp, d.m, d.o, d, st), *dg = static_cast<const char*>(s.dg), *du = static_cast<const char*>(s.du);
         GemmArgs a{};
-        a.a = {{dyr, nullptr}, op * es, d.m};
-        a.b = {{rows_of<T>(wd, s.dp, d.o, d.n, d, st), nullptr}, np * es, d.n};
-        a.M = d.m; a.N = d.n; a.K = d.o; a.nseg = 1; a.problems = 1; a.ldo = np;
-        a.gin = g; a.uin = u; a.gout = s.dg; a.uout = s.du; a.act = act;
+        a.pr[0] = {{dyr, nullptr}, {rows_of<T>(wd, s.dp, d.o, d.n, d, st), nullptr}, op, np, d.m, d.n, d.pad(d.n), s.dg, 0, 0};
+        a.K = d.o; a.nseg = 1;
+        a.gin = g; a.uin = u; a.uout = s.du; a.act = act;
         if (dbg || dbu) { a.cols = s.cols[0]; a.cols2 = s.cols[1]; }
-        // (k of dy's rows ends at the padded width: zeros there; rows of wd end at o)
-        if (int rc = gemm_launch<T, T, false, true, EPI_GATE_BWD>(a, s.gate, st)) return rc;
+        if (int rc = gemm_launch<T, T, false, true, EPI_GATE_BWD>(a, 1, s.gate, st)) return rc;
         if (dx) {
             a = GemmArgs{};
-            a.a = {{static_cast<const char*>(s.dg), static_cast<const char*>(s.du)}, np * es, d.m};
-            a.b = {{rows_of<T>(wg, s.gp, d.n, d.k, d, st), rows_of<T>(wu, s.up, d.n, d.k, d, st)}, kp * es, d.k};
-            a.M = d.m; a.N = d.k; a.K = d.n; a.nseg = 2; a.problems = 1; a.ldo = d.k;
-            a.out[0] = dx; a.part = s.part;
-            if (int rc = gemm_launch<T, T, false, true, EPI_STORE>(a, s.dx, st)) return rc;
+            a.pr[0] = {{dg, du}, {rows_of<T>(wg, s.gp, d.n, d.k, d, st), rows_of<T>(wu, s.up, d.n, d.k, d, st)}, np, kp, d.m, d.k, d.k, dx, 0, 0};
+            a.K = d.n; a.nseg = 2; a.part = s.part;
+            if (int rc = gemm_launch<T, T, false, true, EPI_STORE>(a, 1, s.dx, st)) return rc;
         }
         if (dwg) {
             a = GemmArgs{};
-            a.a = {{static_cast<const char*>(s.dg), static_cast<const char*>(s.du)}, np * es, d.n};
             const char* xr = rows_of<T>(x, s.xp, d.m, d.k, d, st);
-            a.b = {{xr, xr}, kp * es, d.k};
-            a.M = d.n; a.N = d.k; a.K = d.m; a.nseg = 1; a.problems = 2; a.ldo = d.k;
-            a.out[0] = dwg; a.out[1] = dwu; a.part = s.part; a.accumulate = accumulate;
-            if (int rc = gemm_launch<T, O, true, true, EPI_STORE>(a, s.dw, st)) return rc;
-            a = GemmArgs{};
-            a.a = {{dyr, nullptr}, op * es, d.o};
-            a.b = {{rows_of<T>(h, s.hp, d.m, d.n, d, st), nullptr}, np * es, d.n};
-            a.M = d.o; a.N = d.n; a.K = d.m; a.nseg = 1; a.problems = 1; a.ldo = d.n;
-            a.out[0] = dwd; a.part = s.part; a.accumulate = accumulate;
-            if (int rc = gemm_launch<T, O, true, true, EPI_STORE>(a, s.dwd, st)) return rc;
+            a.pr[0] = {{dg, nullptr}, {xr, nullptr}, np, kp, d.n, d.k, d.k, dwg, 0, 0};
+            a.pr[1] = {{du, nullptr}, {xr, nullptr}, np, kp, d.n, d.k, d.k, dwu, 0, 0};
+            a.pr[2] = {{dyr, nullptr}, {rows_of<T>(h, s.hp, d.m, d.n, d, st), nullptr}, op, np, d.o, d.n, d.n, dwd, 0, 0};
+            a.K = d.m; a.nseg = 1; a.part = s.part; a.accumulate = accumulate;
+            if (int rc = gemm_launch<T, O, true, true, EPI_STORE>(a, 3, s.dw, st)) return rc;
         }
     } else if (!accumulate) {                                          // no rows: the gradients are zero
         auto zero = [&](void* p, int64_t count) {
@@ -296,8 +282,8 @@ int ffn_bwd(int act, const Dims& d, const void* dy, const void* x, const void* w
             q.c[q.jobs] = c; q.out[q.jobs] = out; q.part[q.jobs] = part; q.blocks[q.jobs++] = blocks;
             widest = c > widest ? c : widest;
         };
-        add(d.n, dbg, s.cols[0], (int)s.gate.tiles_m);
-        add(d.n, dbu, s.cols[1], (int)s.gate.tiles_m);
+        add(d.n, dbg, s.cols[0], (int)s.gate_rows(d));
+        add(d.n, dbu, s.cols[1], (int)s.gate_rows(d));
         if (dbd) {
             const int64_t per = ceil_div(d.m, ceil_div(d.m, 32) < kColBlocks ? ceil_div(d.m, 32) : kColBlocks);
             const int blocks = (int)ceil_div(d.m, per);

@@ -24,30 +24,62 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 enum { EPI_STORE = 0, EPI_GATE = 1, EPI_GATE_BWD = 2 };
 
-struct Operand {
-    const char* p[2];                                                  // by segment / problem, or (EPI_GATE's B) gate and up weights
-    int64_t ld;                                                        // bytes from row to row
-    int64_t rows;                                                      // extent of the axis that is not k
+// One product: A (M rows), B (N rows), out (M, N) with ldo columns from row to row
+struct Product {
+    const char *a[2], *b[2];                                           // by segment of the reduction, or (EPI_GATE's b) gate and up weights
+    int64_t lda, ldb;                                                  // bytes from row to row
+    int64_t M;
+    int N, ldo;                                                        // EPI_GATE: columns of g, u, h; EPI_GATE_BWD: ldo >= N, zeros behind N
+    void* out;                                                         // EPI_GATE: h; EPI_GATE_BWD: dg
+    int tiles_m, tiles_n;
 };
 
 struct GemmArgs {
-    Operand a, b;
-    int64_t M;                                                         // output rows
-    int N;                                                             // output columns (EPI_GATE: of g, u, h)
+    Product pr[3];                                                     // independent products over the same k in one launch
     int64_t K;                                                         // reduction of ONE segment
-    int nk, nseg, problems;                                            // steps of a segment; segments; independent products
-    int tiles_m, tiles_n;
-    int whole, streams;                                                // tiles that one workgroup reduces alone; workgroups that share the others' steps
+    int nk, nseg;                                                      // steps of a segment; segments
+    int tiles, whole, splits;                                          // all tiles; the first `whole` reduced by one workgroup each, the others by `splits` in equal parts
     const void *bias, *bias2, *gin, *uin;
-    void *out[2], *gout, *uout;                                        // EPI_GATE: out = h; EPI_GATE_BWD: gout = dg, uout = du
-    int ldo;                                                           // columns from row to row of what is written (>= N; EPI_GATE_BWD: zeros behind N)
+    void *gout, *uout;                                                 // EPI_GATE: g, u or null; EPI_GATE_BWD: uout = du
     int act, accumulate;
-    float* part;                                                       // streams > 0: [2 streams][BM][BN]
+    float* part;                                                       // [tile behind `whole`][split][BM][BN]
     float *cols, *cols2;                                               // EPI_GATE_BWD: column sums of dg and du, [row tile][N], or null
 };
 
-// Steps first .. of the shared tiles that stream w takes (the shared tiles' steps, laid end to end, in equal parts)
-__host__ __device__ __forceinline__ int64_t stream_start(int64_t total, int streams, int64_t w) { return total * w / streams; }
+// tile number -> product, row tile, column tile: groups of 8 rows of tiles x all columns, so that neighbours in the order share operands in L2
+__device__ __forceinline__ Product tile_of(const GemmArgs& p, int item, int* tile_m, int* tile_n) {
+    Product pr = p.pr[0];
+#pragma unroll
+    for (int q = 1; q < 3; ++q) {
+        const int before = pr.tiles_m * pr.tiles_n;
+        if (item < before) break;
+        item -= before;
+        pr = p.pr[q];
+    }
+    constexpr int GROUP = 8;
+    const int group = item / (GROUP * pr.tiles_n), first = group * GROUP, size = pr.tiles_m - first < GROUP ? pr.tiles_m - first : GROUP;
+    item -= group * GROUP * pr.tiles_n;
+    *tile_m = first + item % size;
+    *tile_n = item / size;
+    return pr;
+}
+
+// act(u) and act'(u) from one exponential
+__device__ __forceinline__ void act_both(float u, int act, float* a, float* da) {
+    if (act == SUHPE_ACT_SILU) {
+        const float s = fast_sigmoid(u);
+        *a = u * s;
+        *da = s * (1.f + u * (1.f - s));
+    } else if (act == SUHPE_ACT_GELU) {
+        float e;
+        const float cdf = 0.5f * (1.f + fast_erf(u * 0.70710678118654752f, &e));
+        *a = u * cdf;
+        *da = cdf + u * 0.3989422804014327f * e;
+    } else {
+        *a = act_apply(u, act);
+        *da = act_grad(u, act);
+    }
+}
 
 template <typename T> struct Mfma;
 template <> struct Mfma<bf16> {
@@ -85,8 +117,11 @@ template <int N> __device__ __forceinline__ void dma(const unsigned (&off)[N], c
                      "buffer_load_dwordx4 %3, %5, 0 offen lds\n\ts_add_u32 m0, m0, 1024\n\ts_nop 2\n\t"
                      "buffer_load_dwordx4 %4, %5, 0 offen lds\n\ts_mov_b32 m0, %0"
                      : "=&s"(keep) : "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(r), "s"(lds) : "memory", "scc");
+    else if constexpr (N == 1)
+        asm volatile("s_nop 4\n\ts_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 2\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds\n\ts_mov_b32 m0, %0"
+                     : "=&s"(keep) : "v"(off[0]), "s"(r), "s"(lds) : "memory");
     else {
-        static_assert(N == 2, "two or four pieces");
+        static_assert(N == 2, "one, two or four pieces");
         asm volatile("s_nop 4\n\ts_mov_b32 %0, m0\n\ts_mov_b32 m0, %4\n\ts_nop 2\n\t"
                      "buffer_load_dwordx4 %1, %3, 0 offen lds\n\ts_add_u32 m0, m0, 1024\n\ts_nop 2\n\t"
                      "buffer_load_dwordx4 %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
@@ -94,15 +129,16 @@ template <int N> __device__ __forceinline__ void dma(const unsigned (&off)[N], c
     }
 }
 
-// LDS-side geometry of one operand: R rows of the tile, k contiguous or k-major
-template <typename T, int R, bool KM> struct Side {
-    static constexpr int ES = sizeof(T), BKE = 128 / ES, CH = 16 / ES, RB = R * ES;
+// LDS-side geometry of one operand: R rows of the tile, BKB bytes of k a step, k contiguous or k-major
+template <typename T, int R, int BKB, bool KM> struct Side {
+    static constexpr int ES = sizeof(T), BKE = BKB / ES, CH = 16 / ES, RB = R * ES, CPR = BKB / 16;
+    static __device__ __forceinline__ int swizzle(int r) { return BKB == 128 ? (r >> 1) & 7 : (r >> 2) & 3; }
     // tile row (or k) and global 16-byte chunk that lane `lane` of piece q fills
     static __device__ __forceinline__ void place(int q, int lane, int* row, int* chunk) {
         if constexpr (!KM) {
-            const int r = q * 8 + (lane >> 3);
+            const int r = q * (1024 / BKB) + lane / CPR;
             *row = r;
-            *chunk = (lane & 7) ^ ((r >> 1) & 7);
+            *chunk = (lane % CPR) ^ swizzle(r);
         } else {
             const int at = q * 1024 + lane * 16, k = at / RB, c = (at % RB) >> 4;
             *row = k;
@@ -112,14 +148,14 @@ template <typename T, int R, bool KM> struct Side {
     // byte offset of this lane's share of the fragment of rows 16 rb .. 16 rb + 15, k-group 0
     static __device__ __forceinline__ int lane_base(int lane) {
         const int g = lane >> 4, t = lane & 15;
-        if constexpr (!KM) return t * 128;
+        if constexpr (!KM) return t * BKB;
         else if constexpr (ES == 2) return (g * 8 + (t >> 2)) * RB + (t & 1) * 8;
         else return (g * 4) * RB + (t & 3) * 4;
     }
     static __device__ __forceinline__ i32x4 read(const char* tile, int base, int lane, int rb, int kk) {
         const int g = lane >> 4, t = lane & 15;
         if constexpr (!KM) {
-            return *reinterpret_cast<const i32x4*>(tile + base + rb * 2048 + (((kk * 4 + g) ^ ((t >> 1) & 7)) << 4));
+            return *reinterpret_cast<const i32x4*>(tile + base + rb * 16 * BKB + (((kk * 4 + g) ^ swizzle(t)) << 4));
         } else if constexpr (ES == 2) {
             const int c = (rb * 2 + ((t & 3) >> 1)) ^ (((t >> 2) | ((g & 1) << 2)) << 1);
             const char* p = tile + base + kk * 32 * RB + (c << 4);
@@ -143,6 +179,11 @@ template <typename T, int R, bool KM> struct Side {
 __device__ __forceinline__ int xcd_order(int bid, int total) {
     const int xcd = bid & 7, i = bid >> 3, per = total >> 3, extra = total & 7;
     return xcd * per + (xcd < extra ? xcd : extra) + i;
+}
+
+// at most `pending` of this wavefront's memory operations under way, none of its LDS reads; then the workgroup's barrier
+template <int pending> __device__ __forceinline__ void wait_steps() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(pending) : "memory");
 }
 
 // 8 consecutive columns from / to memory (any element address); columns from `limit` on are zeros / left alone
@@ -170,61 +211,48 @@ template <typename T> __device__ __forceinline__ void store8(T* p, int n, int li
     }
 }
 
-template <typename T, typename O, int TM, int TN, int WM, int WN, bool AKM, bool BKM, int EPI>
-__global__ __launch_bounds__(64 * WM * WN) void gemm_lowp(const GemmArgs p) {
+template <typename T, typename O, int TM, int TN, int WM, int WN, int BKB, int ST, bool AKM, bool BKM, int EPI>
+__global__ __launch_bounds__(64 * WM * WN, 2) void gemm_lowp(const GemmArgs p) {
     constexpr int BM = 16 * TM * WM, BN = 16 * TN * WN, NW = WM * WN, NT = 64 * NW;
-    using SA = Side<T, BM, AKM>;
-    using SB = Side<T, BN, BKM>;
-    constexpr int BKE = SA::BKE, CH = SA::CH, KG = 2;                   // k-groups of a step: 2 x 32 (fp32: 2 x 16)
-    constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW, STAGE = (BM + BN) * 128;
+    using SA = Side<T, BM, BKB, AKM>;
+    using SB = Side<T, BN, BKB, BKM>;
+    constexpr int BKE = SA::BKE, CH = SA::CH, KG = BKB / 64;            // k-groups of a step: 32 sixteen-bit or 16 fp32 elements each
+    constexpr int PA = BM * BKB / 1024 / NW, PB = BN * BKB / 1024 / NW, STAGE = (BM + BN) * BKB;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
     const int wm = wave / WN, wn = wave % WN;
     const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
     const int basea = SA::lane_base(lane), baseb = SB::lane_base(lane);
-    const int steps = p.nk * p.nseg, tiles = p.tiles_m * p.tiles_n;
-
-    // this workgroup's share: one whole tile, or a range of the shared tiles' steps (pieces of at most two tiles and whole ones between them)
-    int64_t at, end;
-    int stream = -1;
-    if ((int)blockIdx.x < p.whole) {
-        at = (int64_t)xcd_order(blockIdx.x, p.whole) * steps;
-        end = at + steps;
+    // this workgroup's share: a whole tile, or one of the equal parts of a shared tile's steps (all tiles' first parts come first: workgroups side by side on an
+    // XCD then read the same rows of k, and its L2 fetches them once)
+    const int steps = p.nk * p.nseg;
+    int item, split = 0;
+    const bool complete = (int)blockIdx.x < p.whole;
+    if (complete) {
+        item = xcd_order(blockIdx.x, p.whole);
     } else {
-        const int64_t total = ((int64_t)tiles * p.problems - p.whole) * steps;
-        stream = xcd_order(blockIdx.x - p.whole, p.streams);
-        at = (int64_t)p.whole * steps + stream_start(total, p.streams, stream);
-        end = (int64_t)p.whole * steps + stream_start(total, p.streams, stream + 1);
+        const int rest = p.tiles - p.whole;
+        item = xcd_order(blockIdx.x - p.whole, rest * p.splits);
+        split = item / rest;
+        item += p.whole - split * rest;
     }
-    for (int piece = 0; at < end; piece = 1) {
-        int item = (int)(at / steps);
-        const int s0 = (int)(at - (int64_t)item * steps), s1 = (int)(end - at < steps - s0 ? s0 + (end - at) : steps);
-        at += s1 - s0;
-        const bool complete = s0 == 0 && s1 == steps;
-        const int prob = item / tiles;
-        item -= prob * tiles;
-        // tiles in groups of 8 rows of tiles x all columns: neighbours in the order share operands in L2
-        constexpr int GROUP = 8;
-        const int group = item / (GROUP * p.tiles_n), gm0 = group * GROUP, gsize = p.tiles_m - gm0 < GROUP ? p.tiles_m - gm0 : GROUP;
-        item -= group * GROUP * p.tiles_n;
-        const int tile_m = gm0 + item % gsize;
-        const int64_t m0 = (int64_t)tile_m * BM;
-        const int n0 = (item / gsize) * (EPI == EPI_GATE ? BN / 2 : BN);
-
-        // this lane's pieces: byte offset within the step's source rows, and the first k of its chunk (k-major: its row of k) for the tail of the reduction
+    const int s0 = complete ? 0 : (int)((int64_t)steps * split / p.splits), s1 = complete ? steps : (int)((int64_t)steps * (split + 1) / p.splits);
+    int tile_m, tile_n;
+    const Product pr = tile_of(p, item, &tile_m, &tile_n);
+    const int64_t m0 = (int64_t)tile_m * BM;
+    const int n0 = tile_n * (EPI == EPI_GATE ? BN / 2 : BN);
+    {
+        // this lane's pieces: byte offset within the step's source rows
         unsigned offa[PA], offb[PB];
-        int ka[PA], kb[PB];
 #pragma unroll
         for (int i = 0; i < PA; ++i) {
             int row, chunk;
             SA::place(wave * PA + i, lane, &row, &chunk);
             if constexpr (!AKM) {
-                const int64_t r = m0 + row < p.a.rows ? row : p.a.rows - 1 - m0;                // rows beyond the last repeat it: never stored
-                offa[i] = (unsigned)(r * p.a.ld + chunk * 16);
-                ka[i] = chunk * CH;
+                const int64_t r = m0 + row < pr.M ? row : pr.M - 1 - m0;                // rows beyond the last repeat it: never stored
+                offa[i] = (unsigned)(r * pr.lda + chunk * 16);
             } else {
-                offa[i] = m0 + chunk * CH < p.a.rows ? (unsigned)(row * p.a.ld + chunk * 16) : kOob;
-                ka[i] = row;
+                offa[i] = m0 + chunk * CH < pr.M ? (unsigned)(row * pr.lda + chunk * 16) : kOob;
             }
         }
 #pragma unroll
@@ -233,36 +261,51 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_lowp(const GemmArgs p) {
             SB::place(wave * PB + i, lane, &row, &chunk);
             if constexpr (!BKM) {
                 if constexpr (EPI == EPI_GATE) row = (row >> 5) * 16 + (row & 15);              // 16 gate rows, 16 up rows, ...
-                const int64_t r = n0 + row < p.b.rows ? row : p.b.rows - 1 - n0;
-                offb[i] = (unsigned)(r * p.b.ld + chunk * 16);
-                kb[i] = chunk * CH;
+                const int64_t r = n0 + row < pr.N ? row : pr.N - 1 - n0;
+                offb[i] = (unsigned)(r * pr.ldb + chunk * 16);
             } else {
-                offb[i] = n0 + chunk * CH < p.b.rows ? (unsigned)(row * p.b.ld + chunk * 16) : kOob;
-                kb[i] = row;
+                offb[i] = n0 + chunk * CH < pr.N ? (unsigned)(row * pr.ldb + chunk * 16) : kOob;
             }
         }
-        auto issue = [&](int s, int stage) __attribute__((always_inline)) {
-            const int seg = s >= p.nk ? 1 : 0, kt = s - seg * p.nk, which = seg + prob;
-            const int64_t k0 = (int64_t)kt * BKE;
-            const int left = (int)(p.K - k0 < BKE ? p.K - k0 : BKE);                            // elements of k in this step
-            const char* pa = p.a.p[which] + (AKM ? k0 * p.a.ld + m0 * SA::ES : m0 * p.a.ld + k0 * SA::ES);
-            unsigned oa[PA], ob[PB];
-#pragma unroll
-            for (int i = 0; i < PA; ++i) oa[i] = ka[i] < left ? offa[i] : kOob;
-#pragma unroll
-            for (int i = 0; i < PB; ++i) ob[i] = kb[i] < left ? offb[i] : kOob;
+        auto send = [&](const unsigned (&oa)[PA], const unsigned (&ob)[PB], int which, int64_t k0, int stage) __attribute__((always_inline)) {
+            const char* pa = (which ? pr.a[1] : pr.a[0]) + (AKM ? k0 * pr.lda + m0 * SA::ES : m0 * pr.lda + k0 * SA::ES);
             const unsigned la = __builtin_amdgcn_readfirstlane(lds0 + stage * STAGE + wave * PA * 1024);
-            const unsigned lb = __builtin_amdgcn_readfirstlane(lds0 + stage * STAGE + BM * 128 + wave * PB * 1024);
+            const unsigned lb = __builtin_amdgcn_readfirstlane(lds0 + stage * STAGE + BM * BKB + wave * PB * 1024);
             dma<PA>(oa, pa, la);
-            if constexpr (EPI == EPI_GATE) {                           // pieces 4 q, 4 q + 1: gate rows; 4 q + 2, 4 q + 3: up rows
-                static_assert(PB == 4 && !BKM, "a wavefront fills whole blocks of 16 gate and 16 up rows");
-                const int64_t off = n0 * p.b.ld + k0 * SB::ES;
-                const unsigned g[2] = {ob[0], ob[1]}, u[2] = {ob[2], ob[3]};
-                dma<2>(g, p.b.p[0] + off, lb);
-                dma<2>(u, p.b.p[1] + off, lb + 2048);
+            if constexpr (EPI == EPI_GATE) {                           // a wavefront's pieces: 16 gate rows, then 16 up rows
+                static_assert(PB * 1024 == 32 * BKB && !BKM, "a wavefront fills whole blocks of 16 gate and 16 up rows");
+                const int64_t off = n0 * pr.ldb + k0 * SB::ES;
+                unsigned g[PB / 2], u[PB / 2];
+#pragma unroll
+                for (int i = 0; i < PB / 2; ++i) { g[i] = ob[i]; u[i] = ob[PB / 2 + i]; }
+                dma<PB / 2>(g, pr.b[0] + off, lb);
+                dma<PB / 2>(u, pr.b[1] + off, lb + PB * 512);
             } else {
-                const char* pb = p.b.p[which] + (BKM ? k0 * p.b.ld + (int64_t)n0 * SB::ES : n0 * p.b.ld + k0 * SB::ES);
+                const char* pb = (which ? pr.b[1] : pr.b[0]) + (BKM ? k0 * pr.ldb + (int64_t)n0 * SB::ES : n0 * pr.ldb + k0 * SB::ES);
                 dma<PB>(ob, pb, lb);
+            }
+        };
+        auto issue = [&](int s, int stage) __attribute__((always_inline)) {
+            const int seg = s >= p.nk ? 1 : 0, kt = s - seg * p.nk;
+            const int64_t k0 = (int64_t)kt * BKE;
+            if (p.K - k0 >= BKE) {
+                send(offa, offb, seg, k0, stage);
+            } else {                                                    // the last step of a reduction that no whole steps make: what lies beyond reads as zero
+                const int left = (int)(p.K - k0);
+                unsigned oa[PA], ob[PB];
+#pragma unroll
+                for (int i = 0; i < PA; ++i) {
+                    int row, chunk;
+                    SA::place(wave * PA + i, lane, &row, &chunk);
+                    oa[i] = (AKM ? row : chunk * CH) < left ? offa[i] : kOob;
+                }
+#pragma unroll
+                for (int i = 0; i < PB; ++i) {
+                    int row, chunk;
+                    SB::place(wave * PB + i, lane, &row, &chunk);
+                    ob[i] = (BKM ? row : chunk * CH) < left ? offb[i] : kOob;
+                }
+                send(oa, ob, seg, k0, stage);
             }
         };
 
@@ -271,37 +314,62 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_lowp(const GemmArgs p) {
         for (int i = 0; i < TM; ++i)
 #pragma unroll
             for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (piece) __syncthreads();                                    // the previous piece's results have left LDS
         issue(s0, 0);
+        if (s0 + 1 < s1) issue(s0 + 1, 1);
+        // Fragments of a k-group: the weights' side and the last two rows have two register sets in turn, the other rows one: row i's next fragment is read behind the
+        // last matrix instruction that takes its present one (256 accumulator and fragment registers hold no second set of all of them).
+        i32x4 fa[TM - 2], fz[2][2], fb[2][TN];
+        // matrix instructions of the group in `set`, the next group's reads (from `stage`, k-group kk) between them; first: nothing to multiply yet
+        auto advance = [&](auto set_, bool first, bool more, int stage, int kk) __attribute__((always_inline)) {
+            constexpr int set = decltype(set_)::value;
+            const char *ta = smem + stage * STAGE, *tb = ta + BM * BKB;
+            if (more) {
+#pragma unroll
+                for (int j = 0; j < TN; ++j) fb[set ^ 1][j] = SB::read(tb, baseb, lane, wn * TN + j, kk);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) fz[set ^ 1][i] = SA::read(ta, basea, lane, wm * TM + TM - 2 + i, kk);
+            }
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                if (!first)
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) acc[i][j] = Mfma<T>::run(fb[set][j], i < TM - 2 ? fa[i] : fz[set][i - (TM - 2)], acc[i][j]);
+                if (more && i < TM - 2) fa[i] = SA::read(ta, basea, lane, wm * TM + i, kk);
+            }
+            if (!first) {
+                constexpr int RA = AKM ? (sizeof(T) == 2 ? 2 : 4) : 1, RB = BKM ? (sizeof(T) == 2 ? 2 : 4) : 1, PER = sizeof(T) == 2 ? 1 : 4;
+                __builtin_amdgcn_sched_group_barrier(0x100, RB * TN + 2 * RA, 0);               // LDS reads
+#pragma unroll
+                for (int i = 0; i < TM - 2; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, TN * PER, 0);                   // matrix instructions
+                    __builtin_amdgcn_sched_group_barrier(0x100, RA, 0);
+                }
+                __builtin_amdgcn_sched_group_barrier(0x008, 2 * TN * PER, 0);
+            }
+        };
+        // One barrier per step, between its two k-groups: it publishes the next step's buffer (every wavefront has waited for its own DMA) and frees this step's
+        // (both groups' fragments are in registers), which the DMA of the step after next then fills.  Fragments are read one group ahead throughout.
+        static_assert(KG == 2 && ST == 2, "two buffers of two k-groups");
+        if (s0 + 1 < s1) wait_steps<PA + PB>();
+        else wait_steps<0>();
+        advance(std::integral_constant<int, 1>{}, true, true, 0, 0);
         for (int s = s0; s < s1; ++s) {
             const int stage = (s - s0) & 1;
-            // this wavefront's DMA of step s has landed and its reads of the other buffer are done; after the barrier that holds for all of them
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if (s + 1 < s1) issue(s + 1, stage ^ 1);
-            const char *ta = smem + stage * STAGE, *tb = ta + BM * 128;
-#pragma unroll
-            for (int kk = 0; kk < KG; ++kk) {
-                i32x4 fa[TM], fb[TN];
-#pragma unroll
-                for (int j = 0; j < TN; ++j) fb[j] = SB::read(tb, baseb, lane, wn * TN + j, kk);
-#pragma unroll
-                for (int i = 0; i < TM; ++i) fa[i] = SA::read(ta, basea, lane, wm * TM + i, kk);
-#pragma unroll
-                for (int i = 0; i < TM; ++i)
-#pragma unroll
-                    for (int j = 0; j < TN; ++j) acc[i][j] = Mfma<T>::run(fb[j], fa[i], acc[i][j]);
-            }
+            advance(std::integral_constant<int, 0>{}, false, true, stage, 1);
+            wait_steps<0>();
+            if (s + 2 < s1) issue(s + 2, stage);
+            advance(std::integral_constant<int, 1>{}, false, true, stage ^ 1, 0);                 // (behind the last step: reads of a finished buffer, not used)
         }
 
-        // ---- epilogue.  A lane holds 4 columns of a row (8 bytes of a 16-bit row): the sums go through LDS, 64 rows of each row of wavefronts at a time, and come
+        // ---- epilogue.  A lane holds 4 columns of a row (8 bytes of a 16-bit row): the sums go through LDS, some rows of each row of wavefronts at a time, and come
         // back as 8 columns of one row per thread, neighbouring threads side by side: whole 128-byte lines to memory.  16-byte chunk c of a staged row lies at
         // c ^ (row & 15): the 16 rows of a write pass and the 2 rows of a read pass cover the banks once.
-        constexpr int CHUNKS = TM / 4, ROWS = 64 * WM, PITCH = BN * 4;
-        static_assert(TM % 4 == 0 && ROWS * PITCH <= 2 * STAGE, "a chunk fits the two stages");
+        constexpr int PITCH = BN * 4, CI = 64 * WM * PITCH <= ST * STAGE ? 4 : 2, CHUNKS = TM / CI, ROWS = 16 * CI * WM;
+        static_assert(TM % CI == 0 && ROWS * PITCH <= ST * STAGE, "a chunk fits the stages");
         const int t = lane & 15, g4 = lane >> 4;
         constexpr int WIDE = EPI == EPI_GATE ? BN / 2 : BN, LANES = WIDE / 8, RPP = NT / LANES, PASSES = ROWS / RPP;
         const int cg = threadIdx.x % LANES, r0 = threadIdx.x / LANES, n = n0 + cg * 8;
-        const int limit = EPI == EPI_GATE_BWD ? p.ldo : p.N;
+        const int part_tile = item - p.whole, limit = EPI == EPI_GATE_BWD ? pr.ldo : pr.N;
         float b1[8], b2[8], c1[8], c2[8];
         if constexpr (EPI == EPI_GATE_BWD) {
 #pragma unroll
@@ -316,11 +384,11 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_lowp(const GemmArgs p) {
             constexpr int chunk = decltype(which_chunk)::value;
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < CI; ++i)
 #pragma unroll
                 for (int j = 0; j < TN; ++j) {
                     const int c = (wn * TN + j) * 4 + g4;
-                    *reinterpret_cast<f32x4*>(smem + (wm * 64 + i * 16 + t) * PITCH + ((c ^ t) << 4)) = acc[chunk * 4 + i][j];
+                    *reinterpret_cast<f32x4*>(smem + ((wm * CI + i) * 16 + t) * PITCH + ((c ^ t) << 4)) = acc[chunk * CI + i][j];
                 }
             __syncthreads();
             auto staged = [&](int r, int col, float (&v)[8]) __attribute__((always_inline)) {
@@ -330,13 +398,14 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_lowp(const GemmArgs p) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) { v[e] = lo[e]; v[4 + e] = hi[e]; }
             };
-            auto row_of = [&](int r) { return m0 + (r >> 6) * (16 * TM) + chunk * 64 + (r & 63); };
+            auto tile_row = [&](int r) { return r / (16 * CI) * (16 * TM) + chunk * (16 * CI) + r % (16 * CI); };
+            auto row_of = [&](int r) { return m0 + tile_row(r); };
             if constexpr (EPI == EPI_GATE) {
 #pragma unroll
                 for (int q = 0; q < PASSES; ++q) {
                     const int r = r0 + q * RPP;
                     const int64_t m = row_of(r);
-                    if (m >= p.M || n >= limit) continue;
+                    if (m >= pr.M || n >= limit) continue;
                     float gv[8], uv[8], hv[8];
                     const int col = (cg >> 1) * 32 + (cg & 1) * 8;     // 16 gate columns, 16 up columns, ...
                     staged(r, col, gv);
@@ -347,30 +416,30 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_lowp(const GemmArgs p) {
                         uv[e] += b2[e];
                         hv[e] = act_apply(gv[e], p.act) * uv[e];
                     }
-                    const int64_t o = m * p.ldo + n;
+                    const int64_t o = m * pr.ldo + n;
                     if (p.gout) {
                         store8(static_cast<T*>(p.gout) + o, n, limit, gv);
                         store8(static_cast<T*>(p.uout) + o, n, limit, uv);
                     }
-                    store8(static_cast<T*>(p.out[0]) + o, n, limit, hv);
+                    store8(static_cast<T*>(pr.out) + o, n, limit, hv);
                 }
             } else if constexpr (EPI == EPI_GATE_BWD) {
-                constexpr int BATCH = 16 / (int)sizeof(T) / 2;          // rows whose g and u are in flight together
+                constexpr int BATCH = 8 / (int)sizeof(T) < PASSES ? 8 / (int)sizeof(T) : PASSES;      // rows whose g and u are in flight together
                 static_assert(PASSES % BATCH == 0, "");
 #pragma unroll 1
                 for (int q0 = 0; q0 < PASSES; q0 += BATCH) {
                     T gr[BATCH][8], ur[BATCH][8];
 #pragma unroll
                     for (int q = 0; q < BATCH; ++q) {
-                        const int64_t m = row_of(r0 + (q0 + q) * RPP), o = m * p.N + n;
+                        const int64_t m = row_of(r0 + (q0 + q) * RPP), o = m * pr.N + n;
                         const T *gi = static_cast<const T*>(p.gin) + o, *ui = static_cast<const T*>(p.uin) + o;
-                        if (m < p.M && n + 8 <= p.N) {
+                        if (m < pr.M && n + 8 <= pr.N) {
                             __builtin_memcpy(gr[q], gi, sizeof gr[q]);
                             __builtin_memcpy(ur[q], ui, sizeof ur[q]);
                         } else {
 #pragma unroll
                             for (int e = 0; e < 8; ++e) {
-                                const bool ok = m < p.M && n + e < p.N;
+                                const bool ok = m < pr.M && n + e < pr.N;
                                 gr[q][e] = ok ? gi[e] : (T)0.f;
                                 ur[q][e] = ok ? ui[e] : (T)0.f;
                             }
@@ -380,20 +449,21 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_lowp(const GemmArgs p) {
                     for (int q = 0; q < BATCH; ++q) {
                         const int r = r0 + (q0 + q) * RPP;
                         const int64_t m = row_of(r);
-                        if (m >= p.M || n >= limit) continue;
+                        if (m >= pr.M || n >= limit) continue;
                         float dh[8], dg[8], du[8];
                         staged(r, cg * 8, dh);
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
-                            const float gv = (float)gr[q][e], uv = (float)ur[q][e];
-                            const bool ok = n + e < p.N;               // (columns of padding are written as zeros)
-                            dg[e] = ok ? dh[e] * uv * act_grad(gv, p.act) : 0.f;
-                            du[e] = ok ? dh[e] * act_apply(gv, p.act) : 0.f;
+                            float a, da;
+                            act_both((float)gr[q][e], p.act, &a, &da);
+                            const bool ok = n + e < pr.N;               // (columns of padding are written as zeros)
+                            dg[e] = ok ? dh[e] * (float)ur[q][e] * da : 0.f;
+                            du[e] = ok ? dh[e] * a : 0.f;
                             c1[e] += dg[e];
                             c2[e] += du[e];
                         }
-                        const int64_t o = m * p.ldo + n;
-                        store8(static_cast<T*>(p.gout) + o, n, limit, dg);
+                        const int64_t o = m * pr.ldo + n;
+                        store8(static_cast<T*>(pr.out) + o, n, limit, dg);
                         store8(static_cast<T*>(p.uout) + o, n, limit, du);
                     }
                 }
@@ -403,14 +473,14 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_lowp(const GemmArgs p) {
                     const int r = r0 + q * RPP;
                     float v[8];
                     staged(r, cg * 8, v);
-                    if (!complete) {                                    // a shared tile's piece: the first tile of the stream in slot 2 w, the last in 2 w + 1
-                        float* o = p.part + ((int64_t)(2 * stream + piece) * BM + (r >> 6) * (16 * TM) + chunk * 64 + (r & 63)) * BN + cg * 8;
+                    if (!complete) {
+                        float* o = p.part + (((int64_t)part_tile * p.splits + split) * BM + tile_row(r)) * BN + cg * 8;
                         __builtin_memcpy(o, v, sizeof v);
                         continue;
                     }
                     const int64_t m = row_of(r);
-                    if (m >= p.M || n >= limit) continue;
-                    O* o = static_cast<O*>(p.out[prob]) + m * p.ldo + n;
+                    if (m >= pr.M || n >= limit) continue;
+                    O* o = static_cast<O*>(pr.out) + m * pr.ldo + n;
                     float old[8];
                     if (p.accumulate) load8(o, n, limit, old);
 #pragma unroll
@@ -420,8 +490,12 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_lowp(const GemmArgs p) {
             }
         };
         finish(std::integral_constant<int, 0>{});
-        if constexpr (CHUNKS == 2) finish(std::integral_constant<int, 1>{});
-        static_assert(CHUNKS <= 2, "");
+        if constexpr (CHUNKS > 1) finish(std::integral_constant<int, 1>{});
+        if constexpr (CHUNKS > 2) {
+            finish(std::integral_constant<int, 2>{});
+            finish(std::integral_constant<int, 3>{});
+        }
+        static_assert(CHUNKS == 1 || CHUNKS == 2 || CHUNKS == 4, "");
         if constexpr (EPI == EPI_GATE_BWD)
             if (p.cols) {                                               // the tile's column sums of dg and du: RPP partial sums per column, in order
                 float* red = reinterpret_cast<float*>(smem);
@@ -437,53 +511,45 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_lowp(const GemmArgs p) {
                     float sum = 0.f;
 #pragma unroll
                     for (int r = 0; r < RPP; ++r) sum += red[(which * RPP + r) * BN + c];
-                    if (n0 + c < p.N) (which ? p.cols2 : p.cols)[(int64_t)tile_m * p.N + n0 + c] = sum;
+                    if (n0 + c < pr.N) (which ? p.cols2 : p.cols)[(int64_t)tile_m * pr.N + n0 + c] = sum;
                 }
             }
     }
 }
 
-// The shared tiles: out[m][n] = sum of the pieces, in the order of k [+ bias[n]] [+ out].  Grid: (shared tiles, slices of a tile's rows)
+// The shared tiles: out[m][n] = sum of the parts, in the order of k [+ bias[n]] [+ out].  Grid: (shared tiles, slices of a tile's rows)
 template <typename T, typename O, int BM, int BN>
 __global__ __launch_bounds__(256) void gemm_lowp_join(const GemmArgs p) {
-    const int steps = p.nk * p.nseg, tiles = p.tiles_m * p.tiles_n;
-    const int64_t total = ((int64_t)tiles * p.problems - p.whole) * steps, lo = (int64_t)blockIdx.x * steps, hi = lo + steps;
-    int64_t w0 = lo * p.streams / total;                                // the stream that holds step lo
-    while (w0 > 0 && stream_start(total, p.streams, w0) > lo) --w0;
-    while (stream_start(total, p.streams, w0 + 1) <= lo) ++w0;
-    if (stream_start(total, p.streams, w0) <= lo && stream_start(total, p.streams, w0 + 1) >= hi) return;      // one stream had it all
-    int item = (int)blockIdx.x + p.whole;
-    const int prob = item / tiles;
-    item -= prob * tiles;
-    constexpr int GROUP = 8, LANES = BN / 8, RPP = 256 / LANES;
-    const int group = item / (GROUP * p.tiles_n), gm0 = group * GROUP, gsize = p.tiles_m - gm0 < GROUP ? p.tiles_m - gm0 : GROUP;
-    item -= group * GROUP * p.tiles_n;
-    const int64_t m0 = (int64_t)(gm0 + item % gsize) * BM;
-    const int n0 = (item / gsize) * BN, cg = threadIdx.x % LANES, n = n0 + cg * 8;
-    if (n >= p.N) return;
+    int tile_m, tile_n;
+    const Product pr = tile_of(p, (int)blockIdx.x + p.whole, &tile_m, &tile_n);
+    constexpr int LANES = BN / 8, RPP = 256 / LANES;
+    const int64_t m0 = (int64_t)tile_m * BM;
+    const int cg = threadIdx.x % LANES, n = tile_n * BN + cg * 8;
+    if (n >= pr.N) return;
     const int rows = BM / gridDim.y;
     for (int r = blockIdx.y * rows + threadIdx.x / LANES; r < (int)(blockIdx.y + 1) * rows; r += RPP) {
         const int64_t m = m0 + r;
-        if (m >= p.M) return;
+        if (m >= pr.M) return;
         float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, v[8];
-        for (int64_t w = w0; w < p.streams && stream_start(total, p.streams, w) < hi; ++w) {
-            const bool first = stream_start(total, p.streams, w) / steps == (int64_t)blockIdx.x;
-            __builtin_memcpy(v, p.part + ((2 * w + (first ? 0 : 1)) * BM + r) * BN + cg * 8, sizeof v);
+        const float* part = p.part + ((int64_t)blockIdx.x * p.splits * BM + r) * BN + cg * 8;
+#pragma unroll 4
+        for (int z = 0; z < p.splits; ++z) {
+            __builtin_memcpy(v, part + (int64_t)z * BM * BN, sizeof v);
 #pragma unroll
             for (int e = 0; e < 8; ++e) s[e] += v[e];
         }
         if (p.bias) {
-            load8(static_cast<const T*>(p.bias) + n, n, p.N, v);
+            load8(static_cast<const T*>(p.bias) + n, n, pr.N, v);
 #pragma unroll
             for (int e = 0; e < 8; ++e) s[e] += v[e];
         }
-        O* o = static_cast<O*>(p.out[prob]) + m * p.ldo + n;
+        O* o = static_cast<O*>(pr.out) + m * pr.ldo + n;
         if (p.accumulate) {
-            load8(o, n, p.N, v);
+            load8(o, n, pr.N, v);
 #pragma unroll
             for (int e = 0; e < 8; ++e) s[e] += v[e];
         }
-        store8(o, n, p.N, s);
+        store8(o, n, pr.N, s);
     }
 }
 
@@ -504,65 +570,79 @@ __global__ __launch_bounds__(256) void pad_rows(const T* __restrict__ src, int64
 
 // ------------------------------------------------------------------------------------------ host side
 struct Plan {
-    int big, whole, streams;
-    int64_t tiles_m, tiles_n;
-    int64_t part_bytes() const { return streams ? (int64_t)2 * streams * (big ? 256 * 256 : 128 * 128) * 4 : 0; }
+    int big = 0, tiles = 0, whole = 0, splits = 1;
+    int grid() const { return whole + (tiles - whole) * splits; }
+    int64_t part_bytes() const { return (int64_t)(tiles - whole) * splits * (big ? 256 * 256 : 128 * 128) * 4; }
 };
 
-// Tile: 256 x 256 (one workgroup of 8 wavefronts per CU) or 128 x 128 (4 wavefronts, two workgroups per CU).  A step of a large tile takes about 1.9 us on the
-// full chip, a step of two small ones 1.1 us for half the work; filling the pipeline and storing costs about 6 and 3 us.  Whichever the sizes make cheaper by
+// Tile: 256 x 256 (one workgroup of 8 wavefronts per CU) or 128 x 128 (4 wavefronts, two workgroups per CU).  A step of a large tile takes about 1.5 us on the
+// full chip, a step of two small ones 1.0 us for half the work; filling the pipeline and storing costs about 6 and 3 us.  Whichever the sizes make cheaper by
 // that count, padding of the last tiles and the last round of workgroups included, is taken.
-// Shared tiles (products whose epilogue is linear): the tiles beyond the last full round are cut along k, their steps laid end to end and dealt out evenly, at
-// least 8 to a workgroup; the pieces are summed by a second launch in the order of k.  2 x 5632 x 2048 weight gradients over 16384 rows: 352 tiles take 2 rounds of
-// 256 (31 % idle), shared 1.375.
-inline Plan plan_gemm(int64_t M, int64_t N, int64_t steps, int problems, bool share) {
-    Plan best{};
-    if (M == 0) return best;
+// Shared tiles (products whose epilogue is linear): the tiles beyond the last full round are cut along k in equal parts, whose sums meet in a second launch in
+// the order of k, where the parts' way through memory costs less than the idle CUs.
+inline Plan plan_gemm(int count, const int64_t (*mn)[2], int64_t steps, bool share) {
+    Plan best;
     double best_us = 0.;
     for (int big = 0; big < 2; ++big) {
         const int64_t b = big ? 256 : 128, slots = big ? 256 : 512;
-        Plan q{big, 0, 0, ceil_div(M, b), ceil_div(N, b)};
-        const int64_t tiles = q.tiles_m * q.tiles_n * problems, rounds = tiles / slots, rest = tiles - rounds * slots;
-        const double step = big ? 1.9 : 1.1, ends = big ? 6. : 3.;
-        double us = (double)rounds * ((double)steps * step + ends);
-        // alone, the rest runs as long as a full round (the two small tiles of a CU at least share it); shared, its part plus the pieces' way through memory
-        const double alone = (double)steps * step * (big || rest > slots / 2 ? 1. : 0.6) + ends;
-        int64_t w = rest * steps / 8;
-        if (w > slots) w = slots;
-        const double shared = w > 0 ? (double)(rest * steps) / (double)w * step + 2 * ends + (double)w * 2 * (big ? 0.262 : 0.0655) * 2 / 4. : 1e30;
-        if (rest == 0) q.whole = (int)tiles;
-        else if (share && w > rest && shared < alone) { q.whole = (int)(rounds * slots); q.streams = (int)w; us += shared; }
-        else { q.whole = (int)tiles; us += alone; }
-        if (!big || us < best_us) { best = q; best_us = us; }
+        int64_t tiles = 0;
+        for (int i = 0; i < count; ++i) tiles += ceil_div(mn[i][0], b) * ceil_div(mn[i][1], b);
+        if (tiles == 0) return best;
+        const int64_t rest = tiles % slots;
+        const double step = big ? 1.5 : 1.0, ends = big ? 6. : 3., full = (double)steps * step + ends;
+        Plan q;
+        q.big = big;
+        q.tiles = q.whole = (int)tiles;
+        // (a last round with one small workgroup per CU runs faster than one with two)
+        double tail = rest == 0 ? 0. : (big || rest > slots / 2 ? full : 0.6 * full);
+        if (share)
+            for (int64_t z = 2; z <= 64 && rest > 0 && steps / z >= 8; ++z) {
+                const double us = (double)ceil_div(rest * z, slots) * ((double)ceil_div(steps, z) * step + ends) + 6. + (double)(rest * z) * (big ? 0.262 : 0.0655) * 2 / 4.;
+                if (us < tail) {
+                    tail = us;
+                    q.whole = (int)(tiles - rest);
+                    q.splits = (int)z;
+                }
+            }
+        const double us = (double)(tiles / slots) * full + tail;
+        if (!big || us < best_us) {
+            best = q;
+            best_us = us;
+        }
     }
     return best;
 }
+inline Plan plan_gemm(int64_t M, int64_t N, int64_t steps, bool share) {
+    const int64_t mn[1][2] = {{M, N}};
+    return plan_gemm(1, mn, steps, share);
+}
 
 template <typename T, typename O, bool AKM, bool BKM, int EPI>
-int gemm_launch(GemmArgs a, const Plan& q, hipStream_t st) {
-    const int bm = q.big ? 256 : 128;
-    a.tiles_m = (int)q.tiles_m;
-    a.tiles_n = (int)q.tiles_n;
+int gemm_launch(GemmArgs a, int products, const Plan& q, hipStream_t st) {
+    const int bm = q.big ? 256 : 128, bn = EPI == EPI_GATE ? bm / 2 : bm;
+    for (int i = 0; i < products; ++i) {
+        a.pr[i].tiles_m = (int)ceil_div(a.pr[i].M, bm);
+        a.pr[i].tiles_n = (int)ceil_div(EPI == EPI_GATE_BWD ? a.pr[i].ldo : a.pr[i].N, bn);
+    }
+    a.tiles = q.tiles;
     a.whole = q.whole;
-    a.streams = q.streams;
+    a.splits = q.splits;
     a.nk = (int)ceil_div(a.K, 128 / (int)sizeof(T));
-    SUHPE_REQUIRE(q.tiles_m * q.tiles_n * a.problems < 0x7fffffff, "gated_ffn: too many tiles");
+    const dim3 grid((unsigned)q.grid());
     const int lds = 2 * (bm + bm) * 128;                               // two stages of 128 bytes per row of either side
-    const dim3 grid((unsigned)(q.whole + q.streams));
     if (q.big) {
-        auto k = gemm_lowp<T, O, 8, 4, 2, 4, AKM, BKM, EPI>;
+        auto k = gemm_lowp<T, O, 8, 4, 2, 4, 128, 2, AKM, BKM, EPI>;
         (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         hipLaunchKernelGGL(k, grid, dim3(512), lds, st, a);
     } else {
-        auto k = gemm_lowp<T, O, 4, 4, 2, 2, AKM, BKM, EPI>;
+        auto k = gemm_lowp<T, O, 4, 4, 2, 2, 128, 2, AKM, BKM, EPI>;
         (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         hipLaunchKernelGGL(k, grid, dim3(256), lds, st, a);
     }
     if constexpr (EPI == EPI_STORE)
-        if (q.streams) {
-            const unsigned rest = (unsigned)(q.tiles_m * q.tiles_n * a.problems - q.whole);
-            if (q.big) hipLaunchKernelGGL((gemm_lowp_join<T, O, 256, 256>), dim3(rest, 16), dim3(256), 0, st, a);
-            else hipLaunchKernelGGL((gemm_lowp_join<T, O, 128, 128>), dim3(rest, 8), dim3(256), 0, st, a);
+        if (q.whole < q.tiles) {
+            if (q.big) hipLaunchKernelGGL((gemm_lowp_join<T, O, 256, 256>), dim3(q.tiles - q.whole, 16), dim3(256), 0, st, a);
+            else hipLaunchKernelGGL((gemm_lowp_join<T, O, 128, 128>), dim3(q.tiles - q.whole, 8), dim3(256), 0, st, a);
         }
     return check_launch("gated_ffn: product");
 }
