@@ -180,7 +180,7 @@ struct FwdSpace {
     void *xp, *gp, *up, *hp, *dp;
     float* part;
     Plan gate, down;
-    FwdSpace(const Dims& d, Space& s) : gate(plan_gemm(d.m, 2 * (int64_t)d.n, d.steps(d.k), false)), down(plan_gemm(d.m, d.o, d.steps(d.n), true)) {
+    FwdSpace(const Dims& d, Space& s) : gate(plan_gemm(d.m, 2 * (int64_t)d.n, d.steps(d.k), d.es, false)), down(plan_gemm(d.m, d.o, d.steps(d.n), d.es, true)) {
         xp = d.copy(s, d.m, d.k); gp = d.copy(s, d.n, d.k); up = d.copy(s, d.n, d.k); hp = d.copy(s, d.m, d.n); dp = d.copy(s, d.o, d.n);
         part = static_cast<float*>(s.take(down.part_bytes()));
     }
@@ -190,9 +190,9 @@ struct BwdSpace {
     float *part, *cols[3];
     Plan gate, dx, dw;
     int64_t gate_rows(const Dims& d) const { return ceil_div(d.m, gate.big ? 256 : 128); }
-    BwdSpace(const Dims& d, Space& s) : gate(plan_gemm(d.m, d.pad(d.n), d.steps(d.o), false)), dx(plan_gemm(d.m, d.k, 2 * d.steps(d.n), true)) {
+    BwdSpace(const Dims& d, Space& s) : gate(plan_gemm(d.m, d.pad(d.n), d.steps(d.o), d.es, false)), dx(plan_gemm(d.m, d.k, 2 * d.steps(d.n), d.es, true)) {
         const int64_t mn[3][2] = {{d.n, d.k}, {d.n, d.k}, {d.o, d.n}};
-        dw = plan_gemm(3, mn, d.steps(d.m), true);
+        dw = plan_gemm(3, mn, d.steps(d.m), d.es, true);
         dg = s.take(d.m * d.pad(d.n) * d.es);
         du = s.take(d.m * d.pad(d.n) * d.es);
         xp = d.copy(s, d.m, d.k); gp = d.copy(s, d.n, d.k); up = d.copy(s, d.n, d.k); hp = d.copy(s, d.m, d.n); dp = d.copy(s, d.o, d.n); yp = d.copy(s, d.m, d.o);

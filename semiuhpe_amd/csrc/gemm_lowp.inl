@@ -576,11 +576,11 @@ struct Plan {
 };
 
 // Tile: 256 x 256 (one workgroup of 8 wavefronts per CU) or 128 x 128 (4 wavefronts, two workgroups per CU).  A step of a large tile takes about 1.5 us on the
-// full chip, a step of two small ones 1.0 us for half the work; filling the pipeline and storing costs about 6 and 3 us.  Whichever the sizes make cheaper by
+// full chip, a step of two small ones 1.0 us for half the work (fp32: 7.8 and 4.2 us); filling the pipeline and storing costs about 6 and 3 us.  Whichever the sizes make cheaper by
 // that count, padding of the last tiles and the last round of workgroups included, is taken.
 // Shared tiles (products whose epilogue is linear): the tiles beyond the last full round are cut along k in equal parts, whose sums meet in a second launch in
 // the order of k, where the parts' way through memory costs less than the idle CUs.
-inline Plan plan_gemm(int count, const int64_t (*mn)[2], int64_t steps, bool share) {
+inline Plan plan_gemm(int count, const int64_t (*mn)[2], int64_t steps, int es, bool share) {
     Plan best;
     double best_us = 0.;
     for (int big = 0; big < 2; ++big) {
@@ -589,7 +589,7 @@ inline Plan plan_gemm(int count, const int64_t (*mn)[2], int64_t steps, bool sha
         for (int i = 0; i < count; ++i) tiles += ceil_div(mn[i][0], b) * ceil_div(mn[i][1], b);
         if (tiles == 0) return best;
         const int64_t rest = tiles % slots;
-        const double step = big ? 1.5 : 1.0, ends = big ? 6. : 3., full = (double)steps * step + ends;
+        const double step = es == 2 ? (big ? 1.5 : 1.0) : (big ? 7.8 : 4.2), ends = big ? 6. : 3., full = (double)steps * step + ends;
         Plan q;
         q.big = big;
         q.tiles = q.whole = (int)tiles;
@@ -612,9 +612,9 @@ inline Plan plan_gemm(int count, const int64_t (*mn)[2], int64_t steps, bool sha
     }
     return best;
 }
-inline Plan plan_gemm(int64_t M, int64_t N, int64_t steps, bool share) {
+inline Plan plan_gemm(int64_t M, int64_t N, int64_t steps, int es, bool share) {
     const int64_t mn[1][2] = {{M, N}};
-    return plan_gemm(1, mn, steps, share);
+    return plan_gemm(1, mn, steps, es, share);
 }
 
 template <typename T, typename O, bool AKM, bool BKM, int EPI>
