@@ -13,85 +13,138 @@ namespace suhpe {
 namespace {
 
 // ------------------------------------------------------------------------------------------ few rows (serving)
-// At most 16 MT rows: the weights are the traffic, each is read once, straight from memory into the matrix instructions' registers.  A workgroup takes 16 rows of the
-// weights (GATE: of both) and its W wavefronts split k; their sums meet in LDS in a fixed order.  Rows may start at any element: 16-byte loads from any
-// address, and the end of a row whose length no vector divides is read element by element.
-template <typename T> __device__ __forceinline__ i32x4 load_k(const T* row, int64_t k, int64_t K) {
-    constexpr int CH = 16 / sizeof(T);
-    i32x4 v = {0, 0, 0, 0};
-    if (k + CH <= K) {
-        __builtin_memcpy(&v, row + k, 16);
-    } else if (k < K) {
-        T e[CH];
-#pragma unroll
-        for (int i = 0; i < CH; ++i) e[i] = k + i < K ? row[k + i] : (T)0.f;
-        __builtin_memcpy(&v, e, 16);
+// At most 32 rows: the weights are the traffic, each is read once, straight from memory into the matrix instructions' registers.  A workgroup takes 16 / P rows of
+// the weights (GATE: of both); its W wavefronts split k and their sums meet in LDS in a fixed order.
+// P > 1 (at most 16 / P rows of x): the 16 x 16 matrix instruction takes P stretches of k at once -- weight row r and x row m of stretch p in its rows and columns
+// 16 / P * p + r, + m -- and the blocks on its diagonal are summed: P times as many workgroups, and P * 64 bytes of a weight row side by side in one load.
+// Rows may start at any element (16-byte loads from any address); the last chunk of a row starts at K - CH, with what the chunk before it holds set to zero.
+//
+// A 16-byte load from an address that is not a multiple of 4 takes several times as long (13 x 1001 x 2727 fp16, the whole block: 22 us against 10 us for
+// 13 x 1002 x 2726).  ODD: a chunk that starts on an odd element is read as the 16 bytes one element further (at a row's end: one element before) and the element
+// that is missing there, and shifted into place.
+struct Chunk { i32x4 d; unsigned short e; };
+template <typename T, bool ODD> __device__ __forceinline__ Chunk load_k(const T* row, int k, int last) {
+    Chunk c;
+    const int at = k < last ? k : last;
+    if constexpr (!ODD) {
+        __builtin_memcpy(&c.d, row + at, 16);
+        c.e = 0;
+    } else {
+        const bool odd = reinterpret_cast<uintptr_t>(row + at) & 2;
+        __builtin_memcpy(&c.d, row + at + (odd ? (at < last ? 1 : -1) : 0), 16);
+        __builtin_memcpy(&c.e, row + at + (odd && at == last ? 7 : 0), 2);
     }
-    return v;
+    return c;
+}
+template <typename T, bool ODD> __device__ __forceinline__ i32x4 chunk_of(const Chunk& c, const T* row, int k, int last) {
+    if constexpr (!ODD) {
+        return c.d;
+    } else {
+        const int at = k < last ? k : last;
+        const bool odd = reinterpret_cast<uintptr_t>(row + at) & 2, behind = at < last;
+        const unsigned w[5] = {behind ? (unsigned)c.e << 16 : (unsigned)c.d[0], (unsigned)(behind ? c.d[0] : c.d[1]), (unsigned)(behind ? c.d[1] : c.d[2]),
+                               (unsigned)(behind ? c.d[2] : c.d[3]), behind ? (unsigned)c.d[3] : (unsigned)c.e};
+        i32x4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = odd ? (int)__builtin_amdgcn_alignbit(w[i + 1], w[i], 16) : c.d[i];
+        return v;
+    }
+}
+// zeroes the first `gone` elements of a chunk
+template <typename T> __device__ __forceinline__ i32x4 drop_first(i32x4 v, int gone) {
+    constexpr int CH = 16 / (int)sizeof(T);
+    typename Vec<T, CH>::type e = __builtin_bit_cast(typename Vec<T, CH>::type, v);
+#pragma unroll
+    for (int i = 0; i < CH; ++i) e[i] = i < gone ? (T)0.f : e[i];
+    return __builtin_bit_cast(i32x4, e);
 }
 
-template <typename T, int MT, int W, bool GATE>
+template <typename T, int P, int MT, int W, bool GATE, bool ODD>
 __global__ __launch_bounds__(64 * W) void ffn_few_rows(const T* __restrict__ x, int M, int64_t K, const T* __restrict__ w, const T* __restrict__ w2, int N, const T* __restrict__ bias,
                                                        const T* __restrict__ bias2, int act, T* __restrict__ gout, T* __restrict__ uout, T* __restrict__ out) {
-    constexpr int KE = 64 / (int)sizeof(T), CH = 16 / (int)sizeof(T), S = GATE ? 2 : 1;      // k of one matrix step
-    __shared__ f32x4 sums[W][S][MT][64];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, t = lane & 15, g = lane >> 4;
-    const int n0 = blockIdx.x * 16, nr = n0 + t < N ? n0 + t : N - 1;
+    static_assert(P == 1 || MT == 1, "");
+    constexpr int CH = 16 / (int)sizeof(T), KE = 4 * CH * P, S = GATE ? 2 : 1, R = 16 / P;      // KE: k of one matrix step
+    __shared__ float sums[W * P][S][MT][16 * R];
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, t = lane & 15, g = lane >> 4;
+    const int n0 = blockIdx.x * R, part = t / R, rt = t % R, nr = n0 + rt < N ? n0 + rt : N - 1;
     const T *r1 = w + nr * K, *r2 = GATE ? w2 + nr * K : nullptr;
     const T* xr[MT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) xr[i] = x + (int64_t)(16 * i + t < M ? 16 * i + t : M - 1) * K;
-    const int64_t steps = (K + KE - 1) / KE, lo = steps * wave / W, hi = steps * (wave + 1) / W;
+    for (int i = 0; i < MT; ++i) xr[i] = x + (int64_t)(16 * i + rt < M ? 16 * i + rt : M - 1) * K;
+    const int steps = (int)((K + KE - 1) / KE), lo = steps * wave / W, hi = steps * (wave + 1) / W, last = (int)K - CH;
     f32x4 acc[S][MT];
 #pragma unroll
     for (int s = 0; s < S; ++s)
 #pragma unroll
         for (int i = 0; i < MT; ++i) acc[s][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    constexpr int U = MT > 2 ? 2 : 4;
-    for (int64_t q = lo; q < hi; q += U) {
-        i32x4 a[U][S], b[U][MT];
+    constexpr int U = 4;
+    for (int q = lo; q < hi; q += U) {
+        Chunk ca[U][S], cb[U][MT];
 #pragma unroll
         for (int v = 0; v < U; ++v) {
-            const int64_t k = q + v < hi ? (q + v) * KE + g * CH : K;      // (steps past the slice read nothing: zeros)
-            a[v][0] = load_k(r1, k, K);
-            if constexpr (GATE) a[v][1] = load_k(r2, k, K);
+            if (q + v >= hi) break;
+            const int k = (q + v) * KE + (part * 4 + g) * CH;
+            ca[v][0] = load_k<T, ODD>(r1, k, last);
+            if constexpr (GATE) ca[v][1] = load_k<T, ODD>(r2, k, last);
 #pragma unroll
-            for (int i = 0; i < MT; ++i) b[v][i] = load_k(xr[i], k, K);
+            for (int i = 0; i < MT; ++i) cb[v][i] = load_k<T, ODD>(xr[i], k, last);
         }
 #pragma unroll
-        for (int v = 0; v < U; ++v)
+        for (int v = 0; v < U; ++v) {
+            if (q + v >= hi) break;
+            const int k = (q + v) * KE + (part * 4 + g) * CH;
+            i32x4 a[S], b[MT];
+            a[0] = chunk_of<T, ODD>(ca[v][0], r1, k, last);
+            if constexpr (GATE) a[1] = chunk_of<T, ODD>(ca[v][1], r2, k, last);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) b[i] = chunk_of<T, ODD>(cb[v][i], xr[i], k, last);
+            if ((q + v + 1) * KE > K) {                                // the row ends in this step
+                const int over = k - last;
+                const int gone = over < 0 ? 0 : over > CH ? CH : over;
+#pragma unroll
+                for (int s = 0; s < S; ++s) a[s] = drop_first<T>(a[s], gone);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) b[i] = drop_first<T>(b[i], gone);
+            }
 #pragma unroll
             for (int s = 0; s < S; ++s)
 #pragma unroll
-                for (int i = 0; i < MT; ++i) acc[s][i] = Mfma<T>::run(a[v][s], b[v][i], acc[s][i]);
+                for (int i = 0; i < MT; ++i) acc[s][i] = Mfma<T>::run(a[s], b[i], acc[s][i]);
+        }
     }
+    // lane (t, g) holds weight rows 4 g .. 4 g + 3, x row t of each product: kept where both lie in the same stretch
 #pragma unroll
     for (int s = 0; s < S; ++s)
 #pragma unroll
-        for (int i = 0; i < MT; ++i) sums[wave][s][i][lane] = acc[s][i];
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if ((4 * g + r) / R == part) sums[wave * P + part][s][i][rt * R + (4 * g + r) % R] = acc[s][i][r];
     __syncthreads();
-    if (wave >= MT) return;
-    f32x4 total[S];
+    // 16 R sums of W P terms each (MT = 2: twice), in order; Q lanes share one
+    constexpr int OUT = MT * R * R, Q = OUT >= 64 * W ? 1 : OUT <= 64 ? 64 / OUT : 1;
+    const int o = (int)threadIdx.x / Q, slice = (int)threadIdx.x % Q;
+    if (o >= OUT) return;
+    const int i = o / (R * R), at = o % (R * R);
+    float total[S];
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-        total[s] = sums[0][s][wave][lane];
+        total[s] = 0.f;
 #pragma unroll
-        for (int v = 1; v < W; ++v) total[s] += sums[v][s][wave][lane];
+        for (int v = 0; v < W * P / Q; ++v) total[s] += sums[slice * (W * P / Q) + v][s][i][at];
+#pragma unroll
+        for (int d = 1; d < Q; d <<= 1) total[s] += __shfl_xor(total[s], d, 64);
     }
-    const int m = 16 * wave + t, n = n0 + 4 * g;
-    if (m >= M) return;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        if (n + r >= N) break;
-        const int64_t at = (int64_t)m * N + n + r;
-        const float v = total[0][r] + (bias ? (float)bias[n + r] : 0.f);
-        if constexpr (GATE) {
-            const float u = total[1][r] + (bias2 ? (float)bias2[n + r] : 0.f);
-            if (gout) { gout[at] = (T)v; uout[at] = (T)u; }
-            out[at] = (T)(act_apply(v, act) * u);
-        } else {
-            out[at] = (T)v;
-        }
+    const int m = 16 * i + at / R, n = n0 + at % R;
+    if (slice || m >= M || n >= N) return;
+    const int64_t to = (int64_t)m * N + n;
+    const float v = total[0] + (bias ? (float)bias[n] : 0.f);
+    if constexpr (GATE) {
+        const float u = total[1] + (bias2 ? (float)bias2[n] : 0.f);
+        if (gout) { gout[to] = (T)v; uout[to] = (T)u; }
+        out[to] = (T)(act_apply(v, act) * u);
+    } else {
+        out[to] = (T)v;
     }
 }
 
@@ -99,10 +152,22 @@ constexpr int kFewRows = 32;
 
 template <typename T, bool GATE>
 void few_rows(const T* x, int M, int64_t K, const T* w, const T* w2, int N, const T* bias, const T* bias2, int act, T* g, T* u, T* out, hipStream_t st) {
-    const dim3 grid((unsigned)ceil_div(N, 16));
-    constexpr int W = GATE ? 8 : 16;                                   // (both weights in flight need the registers of 8 wavefronts)
-    if (M <= 16) hipLaunchKernelGGL((ffn_few_rows<T, 1, W, GATE>), grid, dim3(64 * W), 0, st, x, M, K, w, w2, N, bias, bias2, act, g, u, out);
-    else hipLaunchKernelGGL((ffn_few_rows<T, 2, W, GATE>), grid, dim3(64 * W), 0, st, x, M, K, w, w2, N, bias, bias2, act, g, u, out);
+#define FEW_(P, MT, W, ODD) \
+    hipLaunchKernelGGL((ffn_few_rows<T, P, MT, W, GATE, ODD>), dim3((unsigned)ceil_div(N, 16 / P)), dim3(64 * W), 0, st, x, M, K, w, w2, N, bias, bias2, act, g, u, out)
+#define FEW(P, MT, W)                                       \
+    do {                                                    \
+        if constexpr (sizeof(T) == 2) {                     \
+            if (odd) { FEW_(P, MT, W, true); break; }       \
+        }                                                   \
+        FEW_(P, MT, W, false);                              \
+    } while (0)
+    const bool odd = K % 2 || !aligned(x, 4) || !aligned(w, 4) || (w2 && !aligned(w2, 4));
+    if (M <= 4) FEW(4, 1, 8);
+    else if (M <= 8) FEW(2, 1, 8);
+    else if (M <= 16) FEW(1, 1, 16);
+    else FEW(1, 2, 16);
+#undef FEW_
+#undef FEW
 }
 
 // ------------------------------------------------------------------------------------------ column sums (bias gradients)
@@ -172,6 +237,7 @@ struct Dims {
     int ch() const { return 16 / es; }
     int pad(int c) const { return (int)ceil_div(c, ch()) * ch(); }
     bool odd(int c) const { return c % ch() != 0; }
+    bool few() const { return m <= kFewRows && k >= ch() && n >= ch(); }      // (a row holds one chunk at least)
     int64_t steps(int64_t c) const { return ceil_div(c, 128 / es); }
     void* copy(Space& s, int64_t rows, int c) const { return odd(c) ? s.take(rows * pad(c) * es) : nullptr; }
 };
@@ -218,7 +284,7 @@ int ffn_fwd(int act, const Dims& d, const void* x, const void* wg, const void* w
             void* y, void* workspace, hipStream_t st) {
     auto c = [](const void* p) { return static_cast<const T*>(p); };
     auto w = [](void* p) { return static_cast<T*>(p); };
-    if (d.m <= kFewRows) {
+    if (d.few()) {
         few_rows<T, true>(c(x), (int)d.m, d.k, c(wg), c(wu), d.n, c(bg), c(bu), act, w(g), w(u), w(h), st);
         few_rows<T, false>(c(h), (int)d.m, d.n, c(wd), nullptr, d.o, c(bd), nullptr, 0, nullptr, nullptr, w(y), st);
         return check_launch("suhpe_gated_ffn_fwd");
@@ -316,9 +382,11 @@ using namespace suhpe;
 extern "C" {
 
 int64_t suhpe_gated_ffn_fwd_workspace_bytes(int dtype, int64_t m, int k, int n, int o) {
-    if (ffn_sizes("suhpe_gated_ffn_fwd_workspace_bytes", dtype, 0, m, k, n, o) || m <= kFewRows) return 0;
+    if (ffn_sizes("suhpe_gated_ffn_fwd_workspace_bytes", dtype, 0, m, k, n, o) || m == 0) return 0;
+    const Dims d{m, k, n, o, dtype_size(dtype)};
+    if (d.few()) return 0;
     Space space{nullptr};
-    const FwdSpace s(Dims{m, k, n, o, dtype_size(dtype)}, space);
+    const FwdSpace s(d, space);
     return space.used;
 }
 
@@ -329,7 +397,7 @@ int suhpe_gated_ffn_fwd(int dtype, int act, int64_t m, int k, int n, int o, cons
     if (m == 0) return SUHPE_OK;
     SUHPE_REQUIRE(x && wg && wu && wd && h && y, "suhpe_gated_ffn_fwd: null pointer");
     const Dims d{m, k, n, o, dtype_size(dtype)};
-    if (m > kFewRows)
+    if (!d.few())
         SUHPE_REQUIRE((d.odd(k) || (aligned(x, 16) && aligned(wg, 16) && aligned(wu, 16))) && (d.odd(n) || (aligned(h, 16) && aligned(wd, 16))),
                       "suhpe_gated_ffn_fwd: x, wg, wu, wd and h start on 16-byte boundaries");
     if (int rc = space_short("suhpe_gated_ffn_fwd", workspace, workspace_bytes, suhpe_gated_ffn_fwd_workspace_bytes(dtype, m, k, n, o))) return rc;

@@ -45,6 +45,14 @@ SIZES = [
     (1, 64, 128, 64),
     (3, 7, 5, 9),
     (16, 96, 256, 96),
+    (2, 9, 8, 3),
+    (4, 130, 71, 1),
+    (5, 257, 1025, 17),
+    (8, 1000, 40, 33),
+    (13, 1001, 2727, 1001),
+    (32, 200, 333, 70),
+    (7, 3, 900, 5),
+    (20, 900, 2, 900),
     (17, 33, 65, 31),
     (64, 64, 64, 64),
     (65, 72, 136, 40),
