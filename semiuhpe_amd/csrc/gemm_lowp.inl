@@ -13,6 +13,7 @@
 // Fragment order of k is the same for every layout (lane group g of 16 takes k = 8 g .. 8 g + 7 of 32, fp32: 4 g + e of 16), so results do not depend on it.
 // The weights' side is the FIRST matrix operand: a lane then holds 4 consecutive output columns of one row, stored as one vector.
 
+#include <atomic>
 #include <type_traits>
 
 namespace suhpe {
@@ -617,6 +618,18 @@ inline Plan plan_gemm(int64_t M, int64_t N, int64_t steps, int es, bool share) {
     return plan_gemm(1, mn, steps, es, share);
 }
 
+// more than 64 KB of LDS for a kernel: asked for once per device
+template <auto kernel> int allow_lds(int bytes) {
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) return check_launch("gated_ffn: device");
+    const uint64_t bit = 1ull << (dev & 63);
+    if (done.load(std::memory_order_relaxed) & bit) return SUHPE_OK;
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return check_launch("gated_ffn: LDS size");
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return SUHPE_OK;
+}
+
 template <typename T, typename O, bool AKM, bool BKM, int EPI>
 int gemm_launch(GemmArgs a, int products, const Plan& q, hipStream_t st) {
     const int bm = q.big ? 256 : 128, bn = EPI == EPI_GATE ? bm / 2 : bm;
@@ -631,12 +644,11 @@ int gemm_launch(GemmArgs a, int products, const Plan& q, hipStream_t st) {
     const dim3 grid((unsigned)q.grid());
     const int lds = 2 * (bm + bm) * 128;                               // two stages of 128 bytes per row of either side
     if (q.big) {
-        auto k = gemm_lowp<T, O, 8, 4, 2, 4, 128, 2, AKM, BKM, EPI>;
-        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        constexpr auto k = gemm_lowp<T, O, 8, 4, 2, 4, 128, 2, AKM, BKM, EPI>;
+        if (int rc = allow_lds<k>(lds)) return rc;
         hipLaunchKernelGGL(k, grid, dim3(512), lds, st, a);
     } else {
-        auto k = gemm_lowp<T, O, 4, 4, 2, 2, 128, 2, AKM, BKM, EPI>;
-        (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        constexpr auto k = gemm_lowp<T, O, 4, 4, 2, 2, 128, 2, AKM, BKM, EPI>;
         hipLaunchKernelGGL(k, grid, dim3(256), lds, st, a);
     }
     if constexpr (EPI == EPI_STORE)

@@ -1631,9 +1631,13 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _LOWP = (torch.bfloat16, torch.float16)
 
 
-def _chk_tok(t, name, dtype=None, device=None, shape=None):
-    """contiguous fp32 / bf16 / fp16 tensor on the HIP device (None passes)"""
+def _chk_tok(t, name, dtype=None, dev=None, shape=None):
+    """contiguous fp32 / bf16 / fp16 tensor on the HIP device (number `dev`), of that type and shape where given (None passes)"""
     if t is None:
+        return
+    # one test for the calls that are right; what is wrong is looked for only if it fails (these checks are a good part of a small call's time)
+    if torch.is_tensor(t) and t.is_cuda and t.dtype in _DTYPES and (dtype is None or t.dtype is dtype) and t.is_contiguous() \
+            and (dev is None or t.get_device() == dev) and (shape is None or t.shape == shape):
         return
     if not torch.is_tensor(t):
         raise ValueError(f"{name}: expected a tensor, got {type(t).__name__}")
@@ -1642,14 +1646,18 @@ def _chk_tok(t, name, dtype=None, device=None, shape=None):
         raise RuntimeError(f"semiuhpe_amd: {name} must live on the HIP device (got {t.device}); there is no CPU path")
     if t.dtype not in _DTYPES:
         raise ValueError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
-    if dtype is not None and t.dtype != dtype:
+    if dtype is not None and t.dtype is not dtype:
         raise ValueError(f"{name}: expected {dtype}, got {t.dtype}")
     if not t.is_contiguous():
         raise ValueError(f"{name}: expected a contiguous tensor, got strides {t.stride()} for shape {tuple(t.shape)}")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name}: on {t.device}, the other tensors on {device}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    if dev is not None and t.get_device() != dev:
+        raise ValueError(f"{name}: on {t.device}, the other tensors on cuda:{dev}")
+    raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+
+
+def _chk_counter(counter, dev):
+    if not (torch.is_tensor(counter) and counter.dtype is torch.int64 and counter.shape == (2,) and counter.is_contiguous() and counter.get_device() == dev):
+        raise ValueError(f"counter: an int64 pair (seed, offset) on cuda:{dev}")
 
 
 def _overlap(a, b):
@@ -1658,12 +1666,21 @@ def _overlap(a, b):
     return na > 0 and nb > 0 and a0 < b0 + nb and b0 < a0 + na and (a0, na) != (b0, nb)
 
 
-def _call_on(device, name, *args):
-    """_lib.call with `device` current: the launch goes to that device's current stream"""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return call(name, *args)
-    with torch.cuda.device(device):
-        return call(name, *args)
+_ENTRY = {}
+
+
+def _call_on(dev, name, *args):
+    """the entry point on device number `dev`'s current stream (that device made current for the call if it is not)"""
+    fn = _ENTRY.get(name)
+    if fn is None:
+        fn = _ENTRY[name] = getattr(_lib.load(), name)
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return call(name, *args)
+    rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc != 0:
+        msg = f"{name} failed ({rc}): {_lib.last_error()}"
+        raise ValueError(msg) if rc == -1 else RuntimeError(msg)
 
 
 def _scratch(nbytes, device):
@@ -1677,14 +1694,15 @@ def _on_16_bytes(t):
 
 def _layernorm16_fwd(x, c, eps, gamma, beta):
     _chk_tok(x, "x")
-    _chk_tok(gamma, "gamma", torch.float32, x.device, (c,)); _chk_tok(beta, "beta", torch.float32, x.device, (c,))
+    dev = x.get_device()
+    _chk_tok(gamma, "gamma", torch.float32, dev, (c,)); _chk_tok(beta, "beta", torch.float32, dev, (c,))
     if c < 1 or x.dim() == 0 or x.shape[-1] != c:
         raise ValueError(f"x: expected rows of {c}, got shape {tuple(x.shape)}")
     rows = x.numel() // c
     y = torch.empty_like(x)
     mean = torch.empty(rows, dtype=torch.float32, device=x.device)
     rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
-    _call_on(x.device, "suhpe_layernorm16_fwd", ptr(x), _DTYPES[x.dtype], rows, c, float(eps), ptr(gamma), ptr(beta), ptr(y), ptr(mean), ptr(rstd))
+    _call_on(dev, "suhpe_layernorm16_fwd", ptr(x), _DTYPES[x.dtype], rows, c, float(eps), ptr(gamma), ptr(beta), ptr(y), ptr(mean), ptr(rstd))
     return y, mean, rstd
 
 
@@ -1692,14 +1710,14 @@ def _layernorm16_bwd(x, dy, c, mean, rstd, gamma, dgamma, dbeta, accumulate, ski
     _chk_tok(x, "x")
     if c < 1 or x.dim() == 0 or x.shape[-1] != c:
         raise ValueError(f"x: expected rows of {c}, got shape {tuple(x.shape)}")
-    rows = x.numel() // c
-    _chk_tok(dy, "dy", x.dtype, x.device, x.shape); _chk_tok(skip, "skip", x.dtype, x.device, x.shape)
+    rows, dev = x.numel() // c, x.get_device()
+    _chk_tok(dy, "dy", x.dtype, dev, x.shape); _chk_tok(skip, "skip", x.dtype, dev, x.shape)
     for t, name, n in ((mean, "mean", rows), (rstd, "rstd", rows), (gamma, "gamma", c), (dgamma, "dgamma", c), (dbeta, "dbeta", c)):
-        _chk_tok(t, name, torch.float32, x.device, (n,))
+        _chk_tok(t, name, torch.float32, dev, (n,))
     dx = torch.empty_like(x)
     nbytes = _lib.load().suhpe_layernorm16_bwd_workspace_bytes(c) if dgamma is not None or dbeta is not None else 0
     ws = _scratch(nbytes, x.device)
-    _call_on(x.device, "suhpe_layernorm16_bwd", ptr(x), ptr(dy), _DTYPES[x.dtype], rows, c, ptr(mean), ptr(rstd), ptr(gamma), ptr(skip), ptr(dx), ptr(dgamma),
+    _call_on(dev, "suhpe_layernorm16_bwd", ptr(x), ptr(dy), _DTYPES[x.dtype], rows, c, ptr(mean), ptr(rstd), ptr(gamma), ptr(skip), ptr(dx), ptr(dgamma),
              ptr(dbeta), int(accumulate), ptr(ws), nbytes)
     return dx
 
@@ -1739,19 +1757,20 @@ def rope_axes(x, pos, plan, heads, parts=1, rotated=None, inverse=False, out=Non
     if x.dim() == 0 or x.shape[-1] != width:
         raise ValueError(f"x: expected rows of {heads} heads * {parts} parts * {plan.dh} = {width}, got shape {tuple(x.shape)}")
     rows = x.numel() // width
+    dev = x.get_device()
     if not torch.is_tensor(pos) or pos.dtype not in _POS_TYPES:
         raise ValueError("pos: an int32, int64 or float32 tensor")
-    if tuple(pos.shape) != (rows, len(plan.axes)) or not pos.is_contiguous():
+    if pos.shape != (rows, len(plan.axes)) or not pos.is_contiguous():
         raise ValueError(f"pos: expected a contiguous tensor of shape {(rows, len(plan.axes))}, got {tuple(pos.shape)}")
-    if pos.device != x.device or plan.freq.device != x.device:
+    if pos.get_device() != dev or plan.freq.get_device() != dev:
         raise ValueError(f"x on {x.device}, pos on {pos.device}, plan on {plan.freq.device}")
     if out is None:
         out = torch.empty_like(x)
     else:
-        _chk_tok(out, "out", x.dtype, x.device, x.shape)
+        _chk_tok(out, "out", x.dtype, dev, x.shape)
         if _overlap(x, out):
             raise ValueError("out: x itself or a tensor that shares no memory with it")
-    _call_on(x.device, "suhpe_rope_axes", ptr(x), _DTYPES[x.dtype], rows, heads, parts, rotated, plan.dh, ptr(pos), _POS_TYPES[pos.dtype], len(plan.axes),
+    _call_on(dev, "suhpe_rope_axes", ptr(x), _DTYPES[x.dtype], rows, heads, parts, rotated, plan.dh, ptr(pos), _POS_TYPES[pos.dtype], len(plan.axes),
              ptr(plan.freq), ptr(plan.axis), plan.pairs, int(plan.layout == "halves"), int(inverse), ptr(out))
     return out
 
@@ -1762,20 +1781,20 @@ def dropout_apply(x, keep, counter, position, skip=None, out=None):
     `counter` (device int64 pair: seed, offset) at `position`, without storing it.  The gradient is dropout_apply(dy, keep, counter, position).
     Uses (x.numel() + 3) // 4 positions.  out: may be x or skip."""
     _chk_tok(x, "x")
-    _chk_tok(skip, "skip", x.dtype, x.device, x.shape)
+    dev = x.get_device()
+    _chk_tok(skip, "skip", x.dtype, dev, x.shape)
     if not 0.0 <= keep <= 1.0:
         raise ValueError(f"keep {keep}: a probability")
-    if not torch.is_tensor(counter) or counter.dtype != torch.int64 or tuple(counter.shape) != (2,) or not counter.is_contiguous() or counter.device != x.device:
-        raise ValueError(f"counter: an int64 pair (seed, offset) on {x.device}")
+    _chk_counter(counter, dev)
     if position < 0:
         raise ValueError(f"position {position}: not negative")
     if out is None:
         out = torch.empty_like(x)
     else:
-        _chk_tok(out, "out", x.dtype, x.device, x.shape)
+        _chk_tok(out, "out", x.dtype, dev, x.shape)
         if _overlap(x, out) or (skip is not None and _overlap(skip, out)):
             raise ValueError("out: x or skip itself, or a tensor that shares no memory with them")
-    _call_on(x.device, "suhpe_dropout_apply", ptr(x), _DTYPES[x.dtype], x.numel(), float(keep), ptr(counter), int(position), ptr(skip), ptr(out))
+    _call_on(dev, "suhpe_dropout_apply", ptr(x), _DTYPES[x.dtype], x.numel(), float(keep), ptr(counter), int(position), ptr(skip), ptr(out))
     return out
 
 
@@ -1797,44 +1816,46 @@ def dropout_bwd(dy, draw):
 
 def dropout_advance(counter, by):
     """move `counter` on by `by` positions on the device: at the end of a captured graph that draws, so that every replay draws fresh numbers"""
-    if not torch.is_tensor(counter) or not counter.is_cuda or counter.dtype != torch.int64 or tuple(counter.shape) != (2,) or not counter.is_contiguous():
+    if not torch.is_tensor(counter) or not counter.is_cuda:
         raise ValueError("counter: an int64 pair (seed, offset) on the HIP device")
+    _chk_counter(counter, counter.get_device())
     if by < 0:
         raise ValueError(f"by {by}: not negative")
-    _call_on(counter.device, "suhpe_dropout_advance", ptr(counter), int(by))
+    _call_on(counter.get_device(), "suhpe_dropout_advance", ptr(counter), int(by))
 
 
 def _ffn_sizes(x, wg, wu, wd, act):
     _chk_tok(x, "x")
     if act not in ACT:
         raise ValueError(f"act {act!r}: one of {sorted(k for k in ACT if k)}")
+    dev = x.get_device()
     for t, name in ((wg, "wg"), (wu, "wu"), (wd, "wd")):
-        _chk_tok(t, name, x.dtype, x.device)
+        _chk_tok(t, name, x.dtype, dev)
         if t is None or t.dim() != 2:
             raise ValueError(f"{name}: expected a matrix")
     n, k = wg.shape
     o = wd.shape[0]
-    if tuple(wu.shape) != (n, k) or wd.shape[1] != n or min(n, k, o) < 1:
+    if wu.shape != wg.shape or wd.shape[1] != n or n < 1 or k < 1 or o < 1:
         raise ValueError(f"wg {tuple(wg.shape)}, wu {tuple(wu.shape)}, wd {tuple(wd.shape)}: expected (n, k), (n, k), (o, n)")
     if x.dim() == 0 or x.shape[-1] != k:
         raise ValueError(f"x: expected rows of {k}, got shape {tuple(x.shape)}")
-    return x.numel() // k, k, n, o
+    return dev, x.numel() // k, k, n, o
 
 
 @_memop
 def gated_ffn_fwd(x, wg, wu, wd, bg=None, bu=None, bd=None, act="silu", save=True):
     """The gated feed-forward block y = (act(x wg^T + bg) * (x wu^T + bu)) wd^T + bd: x (..., k), wg and wu (n, k), wd (o, n) -> y (..., o) and, with save=True, what
     gated_ffn_bwd needs (g, u, h: both projections and the product, each rounded to x's type once), else None."""
-    m, k, n, o = _ffn_sizes(x, wg, wu, wd, act)
+    dev, m, k, n, o = _ffn_sizes(x, wg, wu, wd, act)
     x, wg, wu, wd = (_on_16_bytes(t) for t in (x, wg, wu, wd))
     for t, name, c in ((bg, "bg", n), (bu, "bu", n), (bd, "bd", o)):
-        _chk_tok(t, name, x.dtype, x.device, (c,))
+        _chk_tok(t, name, x.dtype, dev, (c,))
     y = torch.empty(x.shape[:-1] + (o,), dtype=x.dtype, device=x.device)
     h = torch.empty((m, n), dtype=x.dtype, device=x.device)
     g, u = (torch.empty_like(h), torch.empty_like(h)) if save else (None, None)
     nbytes = _lib.load().suhpe_gated_ffn_fwd_workspace_bytes(_DTYPES[x.dtype], m, k, n, o)
     ws = _scratch(nbytes, x.device)
-    _call_on(x.device, "suhpe_gated_ffn_fwd", _DTYPES[x.dtype], ACT[act], m, k, n, o, ptr(x), ptr(wg), ptr(wu), ptr(wd), ptr(bg), ptr(bu), ptr(bd), ptr(g), ptr(u), ptr(h),
+    _call_on(dev, "suhpe_gated_ffn_fwd", _DTYPES[x.dtype], ACT[act], m, k, n, o, ptr(x), ptr(wg), ptr(wu), ptr(wd), ptr(bg), ptr(bu), ptr(bd), ptr(g), ptr(u), ptr(h),
              ptr(y), ptr(ws), nbytes)
     return y, ((g, u, h) if save else None)
 
@@ -1843,12 +1864,12 @@ def gated_ffn_fwd(x, wg, wu, wd, bg=None, bu=None, bd=None, act="silu", save=Tru
 def gated_ffn_bwd(dy, x, wg, wu, wd, saved, act="silu", dwg=None, dwu=None, dwd=None, dbg=None, dbu=None, dbd=None, accumulate=False, need_dx=True):
     """-> dx (None with need_dx=False); writes the gradients it is given buffers for (added to what they hold with accumulate=True): dwg, dwu, dwd together, each of
     dbg, dbu, dbd by itself, all of x's type or all fp32.  `saved`: what gated_ffn_fwd(save=True) returned for this x."""
-    m, k, n, o = _ffn_sizes(x, wg, wu, wd, act)
-    _chk_tok(dy, "dy", x.dtype, x.device, x.shape[:-1] + (o,))
+    dev, m, k, n, o = _ffn_sizes(x, wg, wu, wd, act)
+    _chk_tok(dy, "dy", x.dtype, dev, x.shape[:-1] + (o,))
     if saved is None:
         raise ValueError("saved: the forward ran with save=False")
     for t, name in zip(saved, ("g", "u", "h")):
-        _chk_tok(t, name, x.dtype, x.device, (m, n))
+        _chk_tok(t, name, x.dtype, dev, (m, n))
     if len({t is None for t in (dwg, dwu, dwd)}) != 1:
         raise ValueError("dwg, dwu, dwd: all three or none")
     grads = [(dwg, "dwg", (n, k)), (dwu, "dwu", (n, k)), (dwd, "dwd", (o, n)), (dbg, "dbg", (n,)), (dbu, "dbu", (n,)), (dbd, "dbd", (o,))]
@@ -1857,13 +1878,13 @@ def gated_ffn_bwd(dy, x, wg, wu, wd, saved, act="silu", dwg=None, dwu=None, dwd=
     if len(types) != 1 or gtype not in (x.dtype, torch.float32):
         raise ValueError(f"gradients: all {x.dtype} or all float32")
     for t, name, shape in grads:
-        _chk_tok(t, name, gtype, x.device, shape)
+        _chk_tok(t, name, gtype, dev, shape)
     dx = torch.empty_like(x) if need_dx else None
     dy, x, wg, wu, wd = (_on_16_bytes(t) for t in (dy, x, wg, wu, wd))
     nbytes = _lib.load().suhpe_gated_ffn_bwd_workspace_bytes(_DTYPES[x.dtype], m, k, n, o)
     ws = _scratch(nbytes, x.device)
     g, u, h = (_on_16_bytes(t) for t in saved)
-    _call_on(x.device, "suhpe_gated_ffn_bwd", _DTYPES[x.dtype], ACT[act], m, k, n, o, ptr(dy), ptr(x), ptr(wg), ptr(wu), ptr(wd), ptr(g), ptr(u), ptr(h), ptr(dx),
+    _call_on(dev, "suhpe_gated_ffn_bwd", _DTYPES[x.dtype], ACT[act], m, k, n, o, ptr(dy), ptr(x), ptr(wg), ptr(wu), ptr(wd), ptr(g), ptr(u), ptr(h), ptr(dx),
              ptr(dwg), ptr(dwu), ptr(dwd), ptr(dbg), ptr(dbu), ptr(dbd), _DTYPES[gtype], int(accumulate), ptr(ws), nbytes)
     return dx
 
