@@ -86,7 +86,10 @@ def grad_of(p):
     flattened the model; allocated lazily otherwise)."""
     if p.grad is None:
         p.grad = torch.empty_strided(p.shape, p.stride(), dtype=p.dtype, device=p.device)
-        K.fill_(p.grad, 0.0)
+        if p.dtype == torch.float32:
+            K.fill_(p.grad, 0.0)
+        else:                                               # (16-bit weights of a GatedFeedForward; the fill kernel writes fp32)
+            p.grad.zero_()
     if _grad_watch is not None:
         _grad_watch(p.grad)
     return p.grad
@@ -549,6 +552,11 @@ class Dropout(Layer):
             if tape is not None:
                 tape.append(None)
             return x
+        if _mask_hook is None and not _mask_queue:          # drawn and applied in one pass, drawn again by the backward: no mask is stored
+            y, draw = K.dropout_fwd(x, 1.0 - self.p)
+            if tape is not None:
+                tape.append(draw)
+            return y
         mask = draw_mask("dropout", x.shape, 1.0 - self.p, x.device)
         if tape is not None:
             tape.append(mask)
@@ -556,7 +564,71 @@ class Dropout(Layer):
 
     def bwd(self, dy, tape):
         mask = tape.pop()
+        if isinstance(mask, tuple):                         # (generator, position, keep): the draw itself
+            return K.dropout_bwd(dy, mask)
         return dy if mask is None else K.mul(dy, mask)
+
+
+class ResidualDropout(Layer):
+    """y = skip + dropout(branch), the end of a transformer block's half, in one pass and without a stored mask"""
+
+    def __init__(self, p=0.0):
+        super().__init__()
+        self.p = p
+
+    def active(self):
+        return self.training and self.p > 0.0
+
+    def fwd2(self, branch, skip, tape):
+        if not self.active():
+            if tape is not None:
+                tape.append(None)
+            return K.add(skip, branch)
+        if _mask_hook is not None:                          # host-made masks
+            mask = draw_mask("dropout", branch.shape, 1.0 - self.p, branch.device)
+            if tape is not None:
+                tape.append(mask)
+            return K.add(skip, K.mul(branch, mask))
+        y, draw = K.dropout_fwd(branch, 1.0 - self.p, skip=skip)
+        if tape is not None:
+            tape.append(draw)
+        return y
+
+    def bwd2(self, dy, tape):
+        """-> (d_branch, d_skip)"""
+        draw = tape.pop()
+        if draw is None:
+            return dy, dy
+        return (K.dropout_bwd(dy, draw) if isinstance(draw, tuple) else K.mul(dy, draw)), dy
+
+
+class GatedFeedForward(Layer):
+    """y = (act(x Wg^T + bg) * (x Wu^T + bu)) Wd^T + bd (kernels.gated_ffn_fwd / _bwd): children `gate`, `up`, `down` hold the parameters.  Rows and parameters share
+    a type: fp32, bf16 or fp16."""
+
+    def __init__(self, dim, hidden, out_dim=None, act="silu", bias=True):
+        super().__init__()
+        self.act = act
+        self.gate = Linear(dim, hidden, bias)
+        self.up = Linear(dim, hidden, bias)
+        self.down = Linear(hidden, out_dim or dim, bias)
+
+    def _weights(self):
+        return [m.weight for m in (self.gate, self.up, self.down)]
+
+    def _biases(self):
+        return [m.bias for m in (self.gate, self.up, self.down)]
+
+    def fwd(self, x, tape):
+        y, saved = K.gated_ffn_fwd(x, *self._weights(), *self._biases(), act=self.act, save=tape is not None)
+        if tape is not None:
+            tape.append((x, saved))
+        return y
+
+    def bwd(self, dy, tape):
+        x, saved = tape.pop()
+        grads = [None if p is None else grad_of(p) for p in self._weights() + self._biases()]
+        return K.gated_ffn_bwd(dy, x, *self._weights(), saved, self.act, *grads, accumulate=True)
 
 
 class StochasticDepth(Layer):

@@ -36,6 +36,8 @@ _OPTIONS = [
     ("data_dir_WildHead", str, None), ("train_labeled", str, None), ("train_unlabeled", str, None), ("test_set", str, None),
     # network
     ("network", str, None),
+    # TinyViT's blocks with the gated feed-forward block, rotary positions on q and k, dropout of both halves (not in the reference; defaults: its network)
+    ("vit_mlp", str, "gelu"), ("vit_rope", "flag", False), ("vit_drop", float, 0.0),
     # training
     ("lr", float, None), ("batch_size", int, None), ("num_workers", int, None), ("stage1_iteration", int, None),
     ("max_iteration", int, None), ("log_frequency", int, None), ("val_frequency", int, None), ("save_frequency", int, None),
@@ -109,6 +111,8 @@ class Config(object):
                 ap.add_argument("--" + name, action="store_true")
             elif name == "network":
                 ap.add_argument("--network", type=str, choices=_NETWORKS)
+            elif name == "vit_mlp":
+                ap.add_argument("--vit_mlp", type=str, choices=["gelu", "gated"])
             elif name == "type_unsuper":
                 ap.add_argument("--type_unsuper", type=str, choices=["ce", "nll"])
             elif name == "distribution":

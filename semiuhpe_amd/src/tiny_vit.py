@@ -13,8 +13,8 @@ import torch
 import torch.nn as nn
 
 from .. import kernels as K
-from ..layers import (BatchNorm2d, Conv2d, Dropout, Identity, Layer, LayerNorm, Linear, Network, Sequential, conv_bn_fwd, draw_mask,
-                      grad_of)
+from ..layers import (BatchNorm2d, Conv2d, Dropout, GatedFeedForward, Identity, Layer, LayerNorm, Linear, Network, ResidualDropout, Sequential, conv_bn_fwd,
+                      draw_mask, grad_of)
 from .efficientnet_v2 import bn_sums_from_dw_ok, dw_dgrad_expand_bwd, init_regression_head_, regression_head
 
 
@@ -142,10 +142,13 @@ ATTN_RECOMPUTE = os.environ.get("SUHPE_ATTN_RECOMPUTE", "1") != "0"
 
 
 class Attention(Layer):
-    """src/tiny_vit.py:216-286 (attn_ratio = 1): LayerNorm -> qkv -> windowed softmax(q k^T s + bias) v -> proj"""
+    """src/tiny_vit.py:216-286 (attn_ratio = 1): LayerNorm -> qkv -> windowed softmax(q k^T s + bias) v -> proj.
+    rope: q and k are turned by the tokens' rows and columns first (kernels.rope_axes, half a head's channels each), next to the learnt bias table"""
 
-    def __init__(self, dim, key_dim, num_heads, window):
+    def __init__(self, dim, key_dim, num_heads, window, rope=False):
         super().__init__()
+        self.rope = rope
+        self._plan, self._grid = None, None
         self.dim, self.key_dim, self.num_heads, self.window = dim, key_dim, num_heads, window
         self.scale = key_dim ** -0.5
         self.norm = LayerNorm(dim)
@@ -173,11 +176,22 @@ class Attention(Layer):
             self._idx32 = self.attention_bias_idxs.to(device=device, dtype=torch.int32).contiguous()
         return self._idx32
 
+    def _turn(self, qkv, B, H, W, inverse):
+        """q and k of the packed rows turned in place (qkv is this block's own: the backward works on the turned ones, and its gradient is turned back)"""
+        if self._plan is None or self._plan.freq.device != qkv.device:
+            self._plan = K.RopeAxes(self.key_dim, (self.key_dim // 2, self.key_dim // 2), device=qkv.device)
+        if self._grid is None or self._grid[0] != (B, H, W) or self._grid[1].device != qkv.device:
+            pos = torch.cartesian_prod(torch.arange(H), torch.arange(W)).to(torch.int32).repeat(B, 1)
+            self._grid = ((B, H, W), pos.to(qkv.device))
+        return K.rope_axes(qkv, self._grid[1], self._plan, self.num_heads, parts=3, rotated=2, inverse=inverse, out=qkv)
+
     def fwd(self, x, tape, residual=None):
         """residual = (skip, keep scale per sample or None): x + drop_path(attn(x)) closed by the proj GEMM's epilogue (src/tiny_vit.py:366)"""
         B, H, W, C = x.shape
         xn = self.norm.fwd(x, tape)
         qkv = self.qkv.fwd(xn.view(-1, C), tape)
+        if self.rope:
+            self._turn(qkv, B, H, W, False)
         if ATTN_RECOMPUTE:
             out, stats = K.window_attn_fwd_rs(qkv, self.attention_biases, self._index(x.device), B, H, W, self.window, self.num_heads,
                                               self.scale, save_stats=tape is not None)
@@ -204,6 +218,8 @@ class Attention(Layer):
         else:
             dqkv = K.window_attn_bwd(qkv, probs, d_out, self._index(dy.device), B, H, W, self.window, self.num_heads,
                                      self.attention_biases.shape[1], self.scale, grad_of(self.attention_biases), inverse=inverse)
+        if self.rope:
+            self._turn(dqkv, B, H, W, True)
         d_xn = self.qkv.bwd(dqkv, tape)
         return self.norm.bwd(d_xn.view(B, H, W, C), tape, skip=skip)
 
@@ -254,18 +270,57 @@ class Mlp(Layer):
         return self.norm.bwd(self.fc1.bwd(dh, tape).view(shp), tape, skip=skip)
 
 
-class TinyViTBlock(Layer):
-    """src/tiny_vit.py:289-379"""
+class GatedMlp(Layer):
+    """Mlp's place with the gated block: LayerNorm -> down(silu(gate(x)) * up(x)); three matrices of two thirds of Mlp's width hold Mlp's parameters"""
 
-    def __init__(self, dim, input_resolution, num_heads, window_size=7, mlp_ratio=4.0, drop_path=0.0):
+    def __init__(self, in_features, hidden_features):
         super().__init__()
+        self.norm = LayerNorm(in_features)
+        self.ffn = GatedFeedForward(in_features, hidden_features // 3 * 2)
+
+    def fwd(self, x, tape, residual=None):
+        return self.ffn.fwd(self.norm.fwd(x, tape), tape)
+
+    def bwd(self, dy, tape, skip=None):
+        return self.norm.bwd(self.ffn.bwd(dy, tape), tape, skip=skip)
+
+
+class TinyViTBlock(Layer):
+    """src/tiny_vit.py:289-379.  Options that the reference has not: mlp="gated" (GatedMlp), rope (Attention), drop (dropout of both halves' results before their
+    residual connections, with drop_path on what is left)"""
+
+    def __init__(self, dim, input_resolution, num_heads, window_size=7, mlp_ratio=4.0, drop_path=0.0, mlp="gelu", rope=False, drop=0.0):
+        super().__init__()
+        if mlp not in ("gelu", "gated"):
+            raise ValueError(f"mlp {mlp!r}: 'gelu' or 'gated'")
+        if not 0.0 <= drop < 1.0:
+            raise ValueError(f"drop {drop}: a probability below 1")
         self.dim, self.input_resolution, self.window_size = dim, input_resolution, window_size
         self.drop_path = DropPath(drop_path)
-        self.attn = Attention(dim, dim // num_heads, num_heads, window_size)
-        self.mlp = Mlp(dim, int(dim * mlp_ratio))
+        self.drop = ResidualDropout(drop)
+        self.attn = Attention(dim, dim // num_heads, num_heads, window_size, rope=rope)
+        self.mlp = (GatedMlp if mlp == "gated" else Mlp)(dim, int(dim * mlp_ratio))
         self.local_conv = Conv2d_BN(dim, dim, 3, 1, 1, groups=dim)
 
+    def _join(self, branch, skip, tape):
+        """skip + drop_path(drop(branch)); without drop_path's scale in one pass"""
+        rs = self.drop_path.draw(branch.shape[0], branch.device)
+        if tape is not None:
+            tape.append(rs)
+        if rs is None:
+            return self.drop.fwd2(branch, skip, tape)
+        return self.drop.fwd2(K.add_rowscale(None, branch, rs), skip, tape)     # (the scale is one per sample: the order does not matter)
+
+    def _split(self, dy, tape):
+        d_branch, d_skip = self.drop.bwd2(dy, tape)
+        rs = tape.pop()
+        return (d_branch if rs is None else K.add_rowscale(None, d_branch, rs)), d_skip
+
     def fwd(self, x, tape):
+        if self.drop.p > 0.0 or isinstance(self.mlp, GatedMlp):
+            x1 = self._join(self.attn.fwd(x, tape), x, tape)
+            x2 = self.local_conv.fwd(x1, tape)
+            return self._join(self.mlp.fwd(x2, tape), x2, tape)
         if not RESIDUAL_EPILOGUE:
             a = self.attn.fwd(x, tape)
             x1 = self.drop_path.fwd2(a, x, tape)
@@ -286,6 +341,11 @@ class TinyViTBlock(Layer):
         return y
 
     def bwd(self, dy, tape):
+        if self.drop.p > 0.0 or isinstance(self.mlp, GatedMlp):
+            d_m, d_x2 = self._split(dy, tape)
+            d_x1 = self.local_conv.bwd(self.mlp.bwd(d_m, tape, skip=d_x2), tape)
+            d_a, d_x = self._split(d_x1, tape)
+            return self.attn.bwd(d_a, tape, skip=d_x)
         d_m, d_x2 = self.drop_path.bwd2(dy, tape)
         d_x2 = self.mlp.bwd(d_m, tape, skip=d_x2)            # (+ the skip gradient: in the LayerNorm backward's kernel)
         d_x1 = self.local_conv.bwd(d_x2, tape)
@@ -311,10 +371,11 @@ class _Stage(Layer):
 
 
 class TinyViT21M(Network):
-    """tiny_vit_21m_224: embed_dims 96/192/384/576, depths 2/2/6/2, heads 3/6/12/18, windows 7/7/14/7, drop_path 0.2"""
+    """tiny_vit_21m_224: embed_dims 96/192/384/576, depths 2/2/6/2, heads 3/6/12/18, windows 7/7/14/7, drop_path 0.2.
+    mlp="gated", rope=True, drop > 0: TinyViTBlock's options (the defaults are the reference's network)"""
     DIMS, DEPTHS, HEADS, WS = (96, 192, 384, 576), (2, 2, 6, 2), (3, 6, 12, 18), (7, 7, 14, 7)
 
-    def __init__(self, num_classes=9, drop_path_rate=0.2):
+    def __init__(self, num_classes=9, drop_path_rate=0.2, mlp="gelu", rope=False, drop=0.0):
         super().__init__()
         d = self.DIMS
         self.patch_embed = PatchEmbed(3, d[0])
@@ -324,7 +385,8 @@ class TinyViT21M(Network):
             if i == 0:
                 blocks = [MBConv(d[0], d[0], 4.0, dpr[k + j]) for j in range(self.DEPTHS[0])]
             else:
-                blocks = [TinyViTBlock(d[i], (res, res), self.HEADS[i], self.WS[i], 4.0, dpr[k + j]) for j in range(self.DEPTHS[i])]
+                blocks = [TinyViTBlock(d[i], (res, res), self.HEADS[i], self.WS[i], 4.0, dpr[k + j], mlp=mlp, rope=rope, drop=drop)
+                          for j in range(self.DEPTHS[i])]
             k += self.DEPTHS[i]
             stages.append(_Stage(blocks, PatchMerging(d[i], d[min(i + 1, 3)]) if i < 3 else None))
             if i < 3:
@@ -363,4 +425,5 @@ def get_TinyViT(config, pretrain=True, model_name="21m"):
     """src/networks.py:407-441 (pretrained blobs are not available offline; same init recipe)."""
     if model_name != "21m":
         raise NotImplementedError("the reference hard-codes the 21m variant (src/networks.py:29)")
-    return TinyViT21M(num_classes=config.num_classes)
+    return TinyViT21M(num_classes=config.num_classes, mlp=getattr(config, "vit_mlp", None) or "gelu", rope=bool(getattr(config, "vit_rope", False)),
+                      drop=getattr(config, "vit_drop", None) or 0.0)
