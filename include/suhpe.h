@@ -598,16 +598,18 @@ int64_t suhpe_layernorm16_bwd_workspace_bytes(int c);
 int suhpe_layernorm16_bwd(const void* x, const void* dy, int dtype, int64_t rows, int c, const float* mean, const float* rstd, const float* gamma, const void* skip,
                           void* dx, float* dgamma, float* dbeta, int accumulate, void* workspace, int64_t workspace_bytes, suhpe_stream_t stream);
 /* Gated feed-forward block: g = x wg^T + bg, u = x wu^T + bu, h = act(g) u, y = h wd^T + bd.  x (m, k), wg / wu (n, k), wd (o, n), y (m, o); biases may be
- * NULL.  h (m, n) is always written; g and u (m, n) where not NULL (the backward needs all three).  Products are summed in fp32; g, u and h are rounded
- * to dtype once.  act: any SUHPE_ACT_*.
+ * NULL.  h (m, n) is always written; g and u go to `kept` where that is not NULL (suhpe_gated_ffn_kept_bytes; the backward needs both buffers).  Products are
+ * summed in fp32; h is rounded to dtype once, g and u are cut to 24 bits (fp32: not at all).  act: any SUHPE_ACT_*.  More than 32 rows: x, wg, wu, wd, h (and dy) start on
+ * 16-byte boundaries unless the rows are no multiple of 16 bytes long.
  * Backward: dx (NULL: not wanted), dwg / dwu / dwd and dbg / dbu / dbd (NULL: not wanted; the three weights' together) of type grad_dtype (dtype or
  * SUHPE_F32), added to what they hold where accumulate != 0.  Every sum has a fixed order: results do not vary from call to call. */
+int64_t suhpe_gated_ffn_kept_bytes(int dtype, int64_t m, int n);
 int64_t suhpe_gated_ffn_fwd_workspace_bytes(int dtype, int64_t m, int k, int n, int o);
 int suhpe_gated_ffn_fwd(int dtype, int act, int64_t m, int k, int n, int o, const void* x, const void* wg, const void* wu, const void* wd, const void* bg, const void* bu,
-                        const void* bd, void* g, void* u, void* h, void* y, void* workspace, int64_t workspace_bytes, suhpe_stream_t stream);
+                        const void* bd, void* kept, void* h, void* y, void* workspace, int64_t workspace_bytes, suhpe_stream_t stream);
 int64_t suhpe_gated_ffn_bwd_workspace_bytes(int dtype, int64_t m, int k, int n, int o);
-int suhpe_gated_ffn_bwd(int dtype, int act, int64_t m, int k, int n, int o, const void* dy, const void* x, const void* wg, const void* wu, const void* wd, const void* g,
-                        const void* u, const void* h, void* dx, void* dwg, void* dwu, void* dwd, void* dbg, void* dbu, void* dbd, int grad_dtype, int accumulate,
+int suhpe_gated_ffn_bwd(int dtype, int act, int64_t m, int k, int n, int o, const void* dy, const void* x, const void* wg, const void* wu, const void* wd, const void* kept,
+                        const void* h, void* dx, void* dwg, void* dwu, void* dwd, void* dbg, void* dbu, void* dbd, int grad_dtype, int accumulate,
                         void* workspace, int64_t workspace_bytes, suhpe_stream_t stream);
 
 /* ---- data-parallel exchange (new capability: the reference trains on one GPU, train.py:24-25).

@@ -4,8 +4,8 @@
 //
 // Forward, two products: [g | u] with the activation and the product in the epilogue (a tile takes the SAME columns of Wg and Wu, so both factors of an
 // output element meet in one lane's registers), then y.  Backward, four: dh whose epilogue turns it into dg and du at once (dh itself is never stored),
-// dx as one product over two ranges of n, dWg and dWu in one launch, dWd.  g, u and h are rounded to the tensors' type once on their way to memory (they are
-// operands of 16-bit matrix instructions next); every sum runs in fp32.
+// dx as one product over two ranges of n, and the three weight gradients in one launch.  h, dg and du are rounded to the tensors' type once on their way to memory
+// (they are operands of 16-bit matrix instructions next), g and u keep 24 bits; every sum runs in fp32.
 #include "lowp.h"
 #include "gemm_lowp.inl"
 
@@ -61,7 +61,7 @@ template <typename T> __device__ __forceinline__ i32x4 drop_first(i32x4 v, int g
 
 template <typename T, int P, int MT, int W, bool GATE, bool ODD>
 __global__ __launch_bounds__(64 * W) void ffn_few_rows(const T* __restrict__ x, int M, int64_t K, const T* __restrict__ w, const T* __restrict__ w2, int N, const T* __restrict__ bias,
-                                                       const T* __restrict__ bias2, int act, T* __restrict__ gout, T* __restrict__ uout, T* __restrict__ out) {
+                                                       const T* __restrict__ bias2, int act, void* kept, T* __restrict__ out) {
     static_assert(P == 1 || MT == 1, "");
     constexpr int CH = 16 / (int)sizeof(T), KE = 4 * CH * P, S = GATE ? 2 : 1, R = 16 / P;      // KE: k of one matrix step
     __shared__ float sums[W * P][S][MT][16 * R];
@@ -141,7 +141,11 @@ __global__ __launch_bounds__(64 * W) void ffn_few_rows(const T* __restrict__ x, 
     const float v = total[0] + (bias ? (float)bias[n] : 0.f);
     if constexpr (GATE) {
         const float u = total[1] + (bias2 ? (float)bias2[n] : 0.f);
-        if (gout) { gout[to] = (T)v; uout[to] = (T)u; }
+        if (kept) {                                                    // (one value at a time: the last of eight columns)
+            const float gv[8] = {v}, uv[8] = {u};
+            keep8<T>(kept, (int64_t)M * N, 0, to, 7, 8, gv);
+            keep8<T>(kept, (int64_t)M * N, 1, to, 7, 8, uv);
+        }
         out[to] = (T)(act_apply(v, act) * u);
     } else {
         out[to] = (T)v;
@@ -151,9 +155,9 @@ __global__ __launch_bounds__(64 * W) void ffn_few_rows(const T* __restrict__ x, 
 constexpr int kFewRows = 32;
 
 template <typename T, bool GATE>
-void few_rows(const T* x, int M, int64_t K, const T* w, const T* w2, int N, const T* bias, const T* bias2, int act, T* g, T* u, T* out, hipStream_t st) {
+void few_rows(const T* x, int M, int64_t K, const T* w, const T* w2, int N, const T* bias, const T* bias2, int act, void* kept, T* out, hipStream_t st) {
 #define FEW_(P, MT, W, ODD) \
-    hipLaunchKernelGGL((ffn_few_rows<T, P, MT, W, GATE, ODD>), dim3((unsigned)ceil_div(N, 16 / P)), dim3(64 * W), 0, st, x, M, K, w, w2, N, bias, bias2, act, g, u, out)
+    hipLaunchKernelGGL((ffn_few_rows<T, P, MT, W, GATE, ODD>), dim3((unsigned)ceil_div(N, 16 / P)), dim3(64 * W), 0, st, x, M, K, w, w2, N, bias, bias2, act, kept, out)
 #define FEW(P, MT, W)                                       \
     do {                                                    \
         if constexpr (sizeof(T) == 2) {                     \
@@ -280,13 +284,13 @@ template <typename O> __global__ __launch_bounds__(256) void ffn_zero(O* p, int6
 }
 
 template <typename T>
-int ffn_fwd(int act, const Dims& d, const void* x, const void* wg, const void* wu, const void* wd, const void* bg, const void* bu, const void* bd, void* g, void* u, void* h,
+int ffn_fwd(int act, const Dims& d, const void* x, const void* wg, const void* wu, const void* wd, const void* bg, const void* bu, const void* bd, void* kept, void* h,
             void* y, void* workspace, hipStream_t st) {
     auto c = [](const void* p) { return static_cast<const T*>(p); };
     auto w = [](void* p) { return static_cast<T*>(p); };
     if (d.few()) {
-        few_rows<T, true>(c(x), (int)d.m, d.k, c(wg), c(wu), d.n, c(bg), c(bu), act, w(g), w(u), w(h), st);
-        few_rows<T, false>(c(h), (int)d.m, d.n, c(wd), nullptr, d.o, c(bd), nullptr, 0, nullptr, nullptr, w(y), st);
+        few_rows<T, true>(c(x), (int)d.m, d.k, c(wg), c(wu), d.n, c(bg), c(bu), act, kept, w(h), st);
+        few_rows<T, false>(c(h), (int)d.m, d.n, c(wd), nullptr, d.o, c(bd), nullptr, 0, nullptr, w(y), st);
         return check_launch("suhpe_gated_ffn_fwd");
     }
     Space space{static_cast<char*>(workspace)};
@@ -295,7 +299,7 @@ int ffn_fwd(int act, const Dims& d, const void* x, const void* wg, const void* w
     GemmArgs a{};
     a.pr[0] = {{rows_of<T>(x, s.xp, d.m, d.k, d, st), nullptr}, {rows_of<T>(wg, s.gp, d.n, d.k, d, st), rows_of<T>(wu, s.up, d.n, d.k, d, st)}, kp, kp, d.m, d.n, d.n, h, 0, 0};
     a.K = d.pad(d.k); a.nseg = 1;
-    a.bias = bg; a.bias2 = bu; a.gout = g; a.uout = u; a.act = act;
+    a.bias = bg; a.bias2 = bu; a.kept = kept; a.act = act;
     if (int rc = gemm_launch<T, T, false, false, EPI_GATE>(a, 1, s.gate, st)) return rc;
     a = GemmArgs{};
     a.pr[0] = {{rows_of<T>(h, s.hp, d.m, d.n, d, st), nullptr}, {rows_of<T>(wd, s.dp, d.o, d.n, d, st), nullptr}, np, np, d.m, d.o, d.o, y, 0, 0};
@@ -305,7 +309,7 @@ int ffn_fwd(int act, const Dims& d, const void* x, const void* wg, const void* w
 }
 
 template <typename T, typename O>
-int ffn_bwd(int act, const Dims& d, const void* dy, const void* x, const void* wg, const void* wu, const void* wd, const void* g, const void* u, const void* h, void* dx, void* dwg,
+int ffn_bwd(int act, const Dims& d, const void* dy, const void* x, const void* wg, const void* wu, const void* wd, const void* kept, const void* h, void* dx, void* dwg,
             void* dwu, void* dwd, void* dbg, void* dbu, void* dbd, int accumulate, void* workspace, hipStream_t st) {
     Space space{static_cast<char*>(workspace)};
     const BwdSpace s(d, space);
@@ -315,7 +319,7 @@ int ffn_bwd(int act, const Dims& d, const void* dy, const void* x, const void* w
         GemmArgs a{};
         a.pr[0] = {{dyr, nullptr}, {rows_of<T>(wd, s.dp, d.o, d.n, d, st), nullptr}, op, np, d.m, d.n, d.pad(d.n), s.dg, 0, 0};
         a.K = d.o; a.nseg = 1;
-        a.gin = g; a.uin = u; a.uout = s.du; a.act = act;
+        a.kept = const_cast<void*>(kept); a.uout = s.du; a.act = act;
         if (dbg || dbu) { a.cols = s.cols[0]; a.cols2 = s.cols[1]; }
         if (int rc = gemm_launch<T, T, false, true, EPI_GATE_BWD>(a, 1, s.gate, st)) return rc;
         if (dx) {
@@ -381,6 +385,11 @@ using namespace suhpe;
 
 extern "C" {
 
+int64_t suhpe_gated_ffn_kept_bytes(int dtype, int64_t m, int n) {
+    SUHPE_REQUIRE(dtype_ok(dtype) && m >= 0 && n > 0, "suhpe_gated_ffn_kept_bytes: bad dtype or sizes");
+    return kept_bytes(dtype_size(dtype), m, n);
+}
+
 int64_t suhpe_gated_ffn_fwd_workspace_bytes(int dtype, int64_t m, int k, int n, int o) {
     if (ffn_sizes("suhpe_gated_ffn_fwd_workspace_bytes", dtype, 0, m, k, n, o) || m == 0) return 0;
     const Dims d{m, k, n, o, dtype_size(dtype)};
@@ -391,9 +400,8 @@ int64_t suhpe_gated_ffn_fwd_workspace_bytes(int dtype, int64_t m, int k, int n, 
 }
 
 int suhpe_gated_ffn_fwd(int dtype, int act, int64_t m, int k, int n, int o, const void* x, const void* wg, const void* wu, const void* wd, const void* bg, const void* bu,
-                        const void* bd, void* g, void* u, void* h, void* y, void* workspace, int64_t workspace_bytes, suhpe_stream_t stream) {
+                        const void* bd, void* kept, void* h, void* y, void* workspace, int64_t workspace_bytes, suhpe_stream_t stream) {
     if (int rc = ffn_sizes("suhpe_gated_ffn_fwd", dtype, act, m, k, n, o)) return rc;
-    SUHPE_REQUIRE((g == nullptr) == (u == nullptr), "suhpe_gated_ffn_fwd: g and u are kept together or not at all");
     if (m == 0) return SUHPE_OK;
     SUHPE_REQUIRE(x && wg && wu && wd && h && y, "suhpe_gated_ffn_fwd: null pointer");
     const Dims d{m, k, n, o, dtype_size(dtype)};
@@ -402,9 +410,9 @@ int suhpe_gated_ffn_fwd(int dtype, int act, int64_t m, int k, int n, int o, cons
                       "suhpe_gated_ffn_fwd: x, wg, wu, wd and h start on 16-byte boundaries");
     if (int rc = space_short("suhpe_gated_ffn_fwd", workspace, workspace_bytes, suhpe_gated_ffn_fwd_workspace_bytes(dtype, m, k, n, o))) return rc;
     hipStream_t st = as_stream(stream);
-    if (dtype == SUHPE_F32) return ffn_fwd<float>(act, d, x, wg, wu, wd, bg, bu, bd, g, u, h, y, workspace, st);
-    if (dtype == SUHPE_BF16) return ffn_fwd<bf16>(act, d, x, wg, wu, wd, bg, bu, bd, g, u, h, y, workspace, st);
-    return ffn_fwd<f16>(act, d, x, wg, wu, wd, bg, bu, bd, g, u, h, y, workspace, st);
+    if (dtype == SUHPE_F32) return ffn_fwd<float>(act, d, x, wg, wu, wd, bg, bu, bd, kept, h, y, workspace, st);
+    if (dtype == SUHPE_BF16) return ffn_fwd<bf16>(act, d, x, wg, wu, wd, bg, bu, bd, kept, h, y, workspace, st);
+    return ffn_fwd<f16>(act, d, x, wg, wu, wd, bg, bu, bd, kept, h, y, workspace, st);
 }
 
 int64_t suhpe_gated_ffn_bwd_workspace_bytes(int dtype, int64_t m, int k, int n, int o) {
@@ -414,13 +422,13 @@ int64_t suhpe_gated_ffn_bwd_workspace_bytes(int dtype, int64_t m, int k, int n, 
     return space.used;
 }
 
-int suhpe_gated_ffn_bwd(int dtype, int act, int64_t m, int k, int n, int o, const void* dy, const void* x, const void* wg, const void* wu, const void* wd, const void* g,
-                        const void* u, const void* h, void* dx, void* dwg, void* dwu, void* dwd, void* dbg, void* dbu, void* dbd, int grad_dtype, int accumulate,
+int suhpe_gated_ffn_bwd(int dtype, int act, int64_t m, int k, int n, int o, const void* dy, const void* x, const void* wg, const void* wu, const void* wd, const void* kept,
+                        const void* h, void* dx, void* dwg, void* dwu, void* dwd, void* dbg, void* dbu, void* dbd, int grad_dtype, int accumulate,
                         void* workspace, int64_t workspace_bytes, suhpe_stream_t stream) {
     if (int rc = ffn_sizes("suhpe_gated_ffn_bwd", dtype, act, m, k, n, o)) return rc;
     SUHPE_REQUIRE(grad_dtype == dtype || grad_dtype == SUHPE_F32, "suhpe_gated_ffn_bwd: gradients have the weights' type or fp32");
     SUHPE_REQUIRE((dwg != nullptr) == (dwu != nullptr) && (dwg != nullptr) == (dwd != nullptr), "suhpe_gated_ffn_bwd: the three weights' gradients are wanted together or not at all");
-    SUHPE_REQUIRE(m == 0 || (dy && x && wg && wu && wd && g && u && h), "suhpe_gated_ffn_bwd: null pointer");
+    SUHPE_REQUIRE(m == 0 || (dy && x && wg && wu && wd && kept && h), "suhpe_gated_ffn_bwd: null pointer");
     if (m == 0 && (accumulate || !(dwg || dbg || dbu || dbd))) return SUHPE_OK;      // nothing to write
     const Dims d{m, k, n, o, dtype_size(dtype)};
     if (m > 0)
@@ -428,7 +436,7 @@ int suhpe_gated_ffn_bwd(int dtype, int act, int64_t m, int k, int n, int o, cons
                       "suhpe_gated_ffn_bwd: dy, x, wg, wu, wd and h start on 16-byte boundaries");
     if (int rc = space_short("suhpe_gated_ffn_bwd", workspace, workspace_bytes, suhpe_gated_ffn_bwd_workspace_bytes(dtype, m, k, n, o))) return rc;
     hipStream_t st = as_stream(stream);
-#define FFN_BWD(T, O) ffn_bwd<T, O>(act, d, dy, x, wg, wu, wd, g, u, h, dx, dwg, dwu, dwd, dbg, dbu, dbd, accumulate, workspace, st)
+#define FFN_BWD(T, O) ffn_bwd<T, O>(act, d, dy, x, wg, wu, wd, kept, h, dx, dwg, dwu, dwd, dbg, dbu, dbd, accumulate, workspace, st)
     if (dtype == SUHPE_F32) return FFN_BWD(float, float);
     if (dtype == SUHPE_BF16) return grad_dtype == SUHPE_F32 ? FFN_BWD(bf16, float) : FFN_BWD(bf16, bf16);
     return grad_dtype == SUHPE_F32 ? FFN_BWD(f16, float) : FFN_BWD(f16, f16);

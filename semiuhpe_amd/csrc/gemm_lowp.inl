@@ -40,8 +40,9 @@ struct GemmArgs {
     int64_t K;                                                         // reduction of ONE segment
     int nk, nseg;                                                      // steps of a segment; segments
     int tiles, whole, splits;                                          // all tiles; the first `whole` reduced by one workgroup each, the others by `splits` in equal parts
-    const void *bias, *bias2, *gin, *uin;
-    void *gout, *uout;                                                 // EPI_GATE: g, u or null; EPI_GATE_BWD: uout = du
+    const void *bias, *bias2;
+    void* kept;                                                        // EPI_GATE: where g and u go, or null; EPI_GATE_BWD: where they come from
+    void* uout;                                                        // EPI_GATE_BWD: du
     int act, accumulate;
     float* part;                                                       // [tile behind `whole`][split][BM][BN]
     float *cols, *cols2;                                               // EPI_GATE_BWD: column sums of dg and du, [row tile][N], or null
@@ -65,20 +66,42 @@ __device__ __forceinline__ Product tile_of(const GemmArgs& p, int item, int* til
     return pr;
 }
 
-// act(u) and act'(u) from one exponential
-__device__ __forceinline__ void act_both(float u, int act, float* a, float* da) {
+// act and act' of 8 values, both from one exponential each.  One branch on the activation for all 8: chosen inside, per value, it cost the epilogues more vector time
+// than the activation
+__device__ __forceinline__ void act8(const float (&u)[8], int act, float (&a)[8]) {
     if (act == SUHPE_ACT_SILU) {
-        const float s = fast_sigmoid(u);
-        *a = u * s;
-        *da = s * (1.f + u * (1.f - s));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) a[e] = act_apply(u[e], SUHPE_ACT_SILU);
     } else if (act == SUHPE_ACT_GELU) {
-        float e;
-        const float cdf = 0.5f * (1.f + fast_erf(u * 0.70710678118654752f, &e));
-        *a = u * cdf;
-        *da = cdf + u * 0.3989422804014327f * e;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) a[e] = act_apply(u[e], SUHPE_ACT_GELU);
     } else {
-        *a = act_apply(u, act);
-        *da = act_grad(u, act);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) a[e] = act_apply(u[e], act);
+    }
+}
+__device__ __forceinline__ void act8_both(const float (&u)[8], int act, float (&a)[8], float (&da)[8]) {
+    if (act == SUHPE_ACT_SILU) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float s = fast_sigmoid(u[e]);
+            a[e] = u[e] * s;
+            da[e] = s * (1.f + u[e] * (1.f - s));
+        }
+    } else if (act == SUHPE_ACT_GELU) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            float x;
+            const float cdf = 0.5f * (1.f + fast_erf(u[e] * 0.70710678118654752f, &x));
+            a[e] = u[e] * cdf;
+            da[e] = cdf + u[e] * 0.3989422804014327f * x;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            a[e] = act_apply(u[e], act);
+            da[e] = act_grad(u[e], act);
+        }
     }
 }
 
@@ -211,6 +234,68 @@ template <typename T> __device__ __forceinline__ void store8(T* p, int n, int li
             if (n + e < limit) p[e] = (T)v[e];
     }
 }
+
+// g and u between forward and backward.  fp32: as they are.  16-bit types: the upper 24 bits of their fp32 values (off by less than 2^-15), as [g: 16][u: 16][g: 8]
+// [u: 8] bits.  Rounded to the tensors' type they would cost the gradients more than their own rounding does (31 360 x 384 x 1 024 bf16: dx, dWg and dWu off by
+// 3.1e-3 of their norm, with 24 bits 2.3e-3, of which 1.7e-3 is the last rounding); 24 bits instead of 32 save a quarter of their way through memory.
+inline int64_t kept_bytes(int es, int64_t m, int n) { return m * n * (es == 4 ? 8 : 6); }
+template <typename T> __device__ __forceinline__ void keep8(void* kept, int64_t count, int which, int64_t at, int n, int limit, const float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        store8(static_cast<float*>(kept) + which * count + at, n, limit, v);
+    } else {
+        unsigned short* ph = static_cast<unsigned short*>(kept) + which * count + at;
+        unsigned char* pl = static_cast<unsigned char*>(kept) + (4 + which) * count + at;
+        if (n + 8 <= limit) {
+            unsigned b[8], hi[4], lo[2];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) b[e] = __float_as_uint(v[e]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) hi[e] = __builtin_amdgcn_perm(b[2 * e + 1], b[2 * e], 0x07060302);
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                lo[e] = __builtin_amdgcn_perm(b[4 * e + 1], b[4 * e], 0x0c0c0501) | __builtin_amdgcn_perm(b[4 * e + 3], b[4 * e + 2], 0x05010c0c);
+            __builtin_memcpy(ph, hi, sizeof hi);
+            __builtin_memcpy(pl, lo, sizeof lo);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (n + e < limit) {
+                    ph[e] = (unsigned short)(__float_as_uint(v[e]) >> 16);
+                    pl[e] = (unsigned char)(__float_as_uint(v[e]) >> 8);
+                }
+        }
+    }
+}
+template <typename T> struct Kept8 {                                   // 8 values under way
+    float f[sizeof(T) == 4 ? 8 : 1];
+    unsigned hi[sizeof(T) == 4 ? 1 : 4], lo[sizeof(T) == 4 ? 1 : 2];
+    __device__ __forceinline__ void load(const void* kept, int64_t count, int which, int64_t at, int n, int limit) {
+        if constexpr (sizeof(T) == 4) {
+            load8(static_cast<const float*>(kept) + which * count + at, n, limit, f);
+        } else {
+            const unsigned short* ph = static_cast<const unsigned short*>(kept) + which * count + at;
+            const unsigned char* pl = static_cast<const unsigned char*>(kept) + (4 + which) * count + at;
+            if (n + 8 <= limit) {
+                __builtin_memcpy(hi, ph, sizeof hi);
+                __builtin_memcpy(lo, pl, sizeof lo);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) hi[e] = 0;
+                lo[0] = lo[1] = 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (n + e < limit) {
+                        hi[e / 2] |= (unsigned)ph[e] << (16 * (e & 1));
+                        lo[e / 4] |= (unsigned)pl[e] << (8 * (e & 3));
+                    }
+            }
+        }
+    }
+    __device__ __forceinline__ float get(int e) const {
+        if constexpr (sizeof(T) == 4) return f[e];
+        else return __uint_as_float((e & 1 ? hi[e / 2] & 0xffff0000u : hi[e / 2] << 16) | (lo[e / 4] >> (8 * (e & 3)) & 0xffu) << 8);
+    }
+};
 
 template <typename T, typename O, int TM, int TN, int WM, int WN, int BKB, int ST, bool AKM, bool BKM, int EPI>
 __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_lowp(const GemmArgs p) {
@@ -370,6 +455,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_lowp(const GemmArgs p) {
         const int t = lane & 15, g4 = lane >> 4;
         constexpr int WIDE = EPI == EPI_GATE ? BN / 2 : BN, LANES = WIDE / 8, RPP = NT / LANES, PASSES = ROWS / RPP;
         const int cg = threadIdx.x % LANES, r0 = threadIdx.x / LANES, n = n0 + cg * 8;
+        const int rows_here = (int)(pr.M - m0 < BM ? pr.M - m0 : BM);
         const int part_tile = item - p.whole, limit = EPI == EPI_GATE_BWD ? pr.ldo : pr.N;
         float b1[8], b2[8], c1[8], c2[8];
         if constexpr (EPI == EPI_GATE_BWD) {
@@ -400,13 +486,13 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_lowp(const GemmArgs p) {
                 for (int e = 0; e < 4; ++e) { v[e] = lo[e]; v[4 + e] = hi[e]; }
             };
             auto tile_row = [&](int r) { return r / (16 * CI) * (16 * TM) + chunk * (16 * CI) + r % (16 * CI); };
-            auto row_of = [&](int r) { return m0 + tile_row(r); };
+            // element offset of a row's columns: 32 bits from the tile's first row on
+            auto at_row = [&](int r, int ld) { return m0 * ld + n + (unsigned)(tile_row(r) * ld); };
             if constexpr (EPI == EPI_GATE) {
 #pragma unroll
                 for (int q = 0; q < PASSES; ++q) {
                     const int r = r0 + q * RPP;
-                    const int64_t m = row_of(r);
-                    if (m >= pr.M || n >= limit) continue;
+                    if (tile_row(r) >= rows_here || n >= limit) continue;
                     float gv[8], uv[8], hv[8];
                     const int col = (cg >> 1) * 32 + (cg & 1) * 8;     // 16 gate columns, 16 up columns, ...
                     staged(r, col, gv);
@@ -415,12 +501,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_lowp(const GemmArgs p) {
                     for (int e = 0; e < 8; ++e) {
                         gv[e] += b1[e];
                         uv[e] += b2[e];
-                        hv[e] = act_apply(gv[e], p.act) * uv[e];
                     }
-                    const int64_t o = m * pr.ldo + n;
-                    if (p.gout) {
-                        store8(static_cast<T*>(p.gout) + o, n, limit, gv);
-                        store8(static_cast<T*>(p.uout) + o, n, limit, uv);
+                    act8(gv, p.act, hv);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) hv[e] *= uv[e];
+                    const int64_t o = at_row(r, pr.ldo);
+                    if (p.kept) {
+                        keep8<T>(p.kept, pr.M * pr.N, 0, o, n, limit, gv);
+                        keep8<T>(p.kept, pr.M * pr.N, 1, o, n, limit, uv);
                     }
                     store8(static_cast<T*>(pr.out) + o, n, limit, hv);
                 }
@@ -429,41 +517,38 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_lowp(const GemmArgs p) {
                 static_assert(PASSES % BATCH == 0, "");
 #pragma unroll 1
                 for (int q0 = 0; q0 < PASSES; q0 += BATCH) {
-                    T gr[BATCH][8], ur[BATCH][8];
+                    Kept8<T> gr[BATCH], ur[BATCH];
 #pragma unroll
                     for (int q = 0; q < BATCH; ++q) {
-                        const int64_t m = row_of(r0 + (q0 + q) * RPP), o = m * pr.N + n;
-                        const T *gi = static_cast<const T*>(p.gin) + o, *ui = static_cast<const T*>(p.uin) + o;
-                        if (m < pr.M && n + 8 <= pr.N) {
-                            __builtin_memcpy(gr[q], gi, sizeof gr[q]);
-                            __builtin_memcpy(ur[q], ui, sizeof ur[q]);
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                const bool ok = m < pr.M && n + e < pr.N;
-                                gr[q][e] = ok ? gi[e] : (T)0.f;
-                                ur[q][e] = ok ? ui[e] : (T)0.f;
-                            }
-                        }
+                        const int r = r0 + (q0 + q) * RPP, lim = tile_row(r) < rows_here ? pr.N : 0;
+                        const int64_t o = at_row(r, pr.N);
+                        gr[q].load(p.kept, pr.M * pr.N, 0, o, n, lim);
+                        ur[q].load(p.kept, pr.M * pr.N, 1, o, n, lim);
                     }
 #pragma unroll
                     for (int q = 0; q < BATCH; ++q) {
                         const int r = r0 + (q0 + q) * RPP;
-                        const int64_t m = row_of(r);
-                        if (m >= pr.M || n >= limit) continue;
-                        float dh[8], dg[8], du[8];
+                        if (tile_row(r) >= rows_here || n >= limit) continue;
+                        float dh[8], gv[8], a[8], da[8], dg[8], du[8];
                         staged(r, cg * 8, dh);
 #pragma unroll
+                        for (int e = 0; e < 8; ++e) gv[e] = gr[q].get(e);
+                        act8_both(gv, p.act, a, da);
+#pragma unroll
                         for (int e = 0; e < 8; ++e) {
-                            float a, da;
-                            act_both((float)gr[q][e], p.act, &a, &da);
-                            const bool ok = n + e < pr.N;               // (columns of padding are written as zeros)
-                            dg[e] = ok ? dh[e] * (float)ur[q][e] * da : 0.f;
-                            du[e] = ok ? dh[e] * a : 0.f;
+                            dg[e] = dh[e] * ur[q].get(e) * da[e];
+                            du[e] = dh[e] * a[e];
+                        }
+                        if (n + 8 > pr.N)                               // columns of padding are written as zeros
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                if (n + e >= pr.N) dg[e] = du[e] = 0.f;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
                             c1[e] += dg[e];
                             c2[e] += du[e];
                         }
-                        const int64_t o = m * pr.ldo + n;
+                        const int64_t o = at_row(r, pr.ldo);
                         store8(static_cast<T*>(pr.out) + o, n, limit, dg);
                         store8(static_cast<T*>(p.uout) + o, n, limit, du);
                     }
@@ -479,9 +564,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_lowp(const GemmArgs p) {
                         __builtin_memcpy(o, v, sizeof v);
                         continue;
                     }
-                    const int64_t m = row_of(r);
-                    if (m >= pr.M || n >= limit) continue;
-                    O* o = static_cast<O*>(pr.out) + m * pr.ldo + n;
+                    if (tile_row(r) >= rows_here || n >= limit) continue;
+                    O* o = static_cast<O*>(pr.out) + at_row(r, pr.ldo);
                     float old[8];
                     if (p.accumulate) load8(o, n, limit, old);
 #pragma unroll

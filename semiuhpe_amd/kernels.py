@@ -1845,19 +1845,20 @@ def _ffn_sizes(x, wg, wu, wd, act):
 @_memop
 def gated_ffn_fwd(x, wg, wu, wd, bg=None, bu=None, bd=None, act="silu", save=True):
     """The gated feed-forward block y = (act(x wg^T + bg) * (x wu^T + bu)) wd^T + bd: x (..., k), wg and wu (n, k), wd (o, n) -> y (..., o) and, with save=True, what
-    gated_ffn_bwd needs (g, u, h: both projections and the product, each rounded to x's type once), else None."""
+    gated_ffn_bwd needs (both projections, in 24 bits where x has 16, and h, their product, in x's type), else None."""
     dev, m, k, n, o = _ffn_sizes(x, wg, wu, wd, act)
     x, wg, wu, wd = (_on_16_bytes(t) for t in (x, wg, wu, wd))
     for t, name, c in ((bg, "bg", n), (bu, "bu", n), (bd, "bd", o)):
         _chk_tok(t, name, x.dtype, dev, (c,))
     y = torch.empty(x.shape[:-1] + (o,), dtype=x.dtype, device=x.device)
     h = torch.empty((m, n), dtype=x.dtype, device=x.device)
-    g, u = (torch.empty_like(h), torch.empty_like(h)) if save else (None, None)
-    nbytes = _lib.load().suhpe_gated_ffn_fwd_workspace_bytes(_DTYPES[x.dtype], m, k, n, o)
+    lib = _lib.load()
+    kept = torch.empty(lib.suhpe_gated_ffn_kept_bytes(_DTYPES[x.dtype], m, n), dtype=torch.uint8, device=x.device) if save else None
+    nbytes = lib.suhpe_gated_ffn_fwd_workspace_bytes(_DTYPES[x.dtype], m, k, n, o)
     ws = _scratch(nbytes, x.device)
-    _call_on(dev, "suhpe_gated_ffn_fwd", _DTYPES[x.dtype], ACT[act], m, k, n, o, ptr(x), ptr(wg), ptr(wu), ptr(wd), ptr(bg), ptr(bu), ptr(bd), ptr(g), ptr(u), ptr(h),
-             ptr(y), ptr(ws), nbytes)
-    return y, ((g, u, h) if save else None)
+    _call_on(dev, "suhpe_gated_ffn_fwd", _DTYPES[x.dtype], ACT[act], m, k, n, o, ptr(x), ptr(wg), ptr(wu), ptr(wd), ptr(bg), ptr(bu), ptr(bd), ptr(kept), ptr(h), ptr(y),
+             ptr(ws), nbytes)
+    return y, ((kept, h) if save else None)
 
 
 @_memop
@@ -1868,8 +1869,10 @@ def gated_ffn_bwd(dy, x, wg, wu, wd, saved, act="silu", dwg=None, dwu=None, dwd=
     _chk_tok(dy, "dy", x.dtype, dev, x.shape[:-1] + (o,))
     if saved is None:
         raise ValueError("saved: the forward ran with save=False")
-    for t, name in zip(saved, ("g", "u", "h")):
-        _chk_tok(t, name, x.dtype, dev, (m, n))
+    kept, h = saved
+    _chk_tok(h, "saved h", x.dtype, dev, (m, n))
+    if kept.dtype is not torch.uint8 or kept.numel() != _lib.load().suhpe_gated_ffn_kept_bytes(_DTYPES[x.dtype], m, n) or kept.get_device() != dev:
+        raise ValueError("saved: not what gated_ffn_fwd returned for rows of this number and type")
     if len({t is None for t in (dwg, dwu, dwd)}) != 1:
         raise ValueError("dwg, dwu, dwd: all three or none")
     grads = [(dwg, "dwg", (n, k)), (dwu, "dwu", (n, k)), (dwd, "dwd", (o, n)), (dbg, "dbg", (n,)), (dbu, "dbu", (n,)), (dbd, "dbd", (o,))]
@@ -1883,8 +1886,8 @@ def gated_ffn_bwd(dy, x, wg, wu, wd, saved, act="silu", dwg=None, dwu=None, dwd=
     dy, x, wg, wu, wd = (_on_16_bytes(t) for t in (dy, x, wg, wu, wd))
     nbytes = _lib.load().suhpe_gated_ffn_bwd_workspace_bytes(_DTYPES[x.dtype], m, k, n, o)
     ws = _scratch(nbytes, x.device)
-    g, u, h = (_on_16_bytes(t) for t in saved)
-    _call_on(dev, "suhpe_gated_ffn_bwd", _DTYPES[x.dtype], ACT[act], m, k, n, o, ptr(dy), ptr(x), ptr(wg), ptr(wu), ptr(wd), ptr(g), ptr(u), ptr(h), ptr(dx),
+    h = _on_16_bytes(h)
+    _call_on(dev, "suhpe_gated_ffn_bwd", _DTYPES[x.dtype], ACT[act], m, k, n, o, ptr(dy), ptr(x), ptr(wg), ptr(wu), ptr(wd), ptr(kept), ptr(h), ptr(dx),
              ptr(dwg), ptr(dwu), ptr(dwd), ptr(dbg), ptr(dbu), ptr(dbd), _DTYPES[gtype], int(accumulate), ptr(ws), nbytes)
     return dx
 

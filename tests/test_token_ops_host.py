@@ -47,22 +47,23 @@ def test_layernorm16_refusals(lib):
 
 
 def test_gated_ffn_refusals(lib):
-    def fwd(dtype=BF16, act=3, m=8, k=16, n=24, o=16, x=P, g=P, u=P, h=P):
+    def fwd(dtype=BF16, act=3, m=8, k=16, n=24, o=16, x=P, h=P):
         ws = max(1, lib.suhpe_gated_ffn_fwd_workspace_bytes(max(0, min(2, dtype)), 8, 16, 24, 16))
-        return lib.suhpe_gated_ffn_fwd(dtype, act, m, k, n, o, x, P, P, P, None, None, None, g, u, h, P, P, ws, None)
-    for bad in (dict(dtype=5), dict(act=9), dict(act=-1), dict(m=-1), dict(k=0), dict(n=-4), dict(o=0), dict(k=1 << 21), dict(x=None), dict(g=None), dict(h=None)):
+        return lib.suhpe_gated_ffn_fwd(dtype, act, m, k, n, o, x, P, P, P, None, None, None, P, h, P, P, ws, None)
+    for bad in (dict(dtype=5), dict(act=9), dict(act=-1), dict(m=-1), dict(k=0), dict(n=-4), dict(o=0), dict(k=1 << 21), dict(x=None), dict(h=None)):
         assert fwd(**bad) == -1, bad
         assert b"suhpe_gated_ffn_fwd" in lib.suhpe_last_error()
     assert fwd(m=0) == 0
+    assert lib.suhpe_gated_ffn_kept_bytes(F32, 10, 7) == 560 and lib.suhpe_gated_ffn_kept_bytes(BF16, 10, 7) == 420 and lib.suhpe_gated_ffn_kept_bytes(4, 10, 7) == -1
     need = lib.suhpe_gated_ffn_bwd_workspace_bytes(BF16, 8, 16, 24, 16)
     assert need > 0
 
     def bwd(grad=BF16, dy=P, dwg=P, dwu=P, dwd=P, nbytes=need, ws=P):
-        return lib.suhpe_gated_ffn_bwd(BF16, 3, 8, 16, 24, 16, dy, P, P, P, P, P, P, P, P, dwg, dwu, dwd, None, None, None, grad, 0, ws, nbytes, None)
+        return lib.suhpe_gated_ffn_bwd(BF16, 3, 8, 16, 24, 16, dy, P, P, P, P, P, P, P, dwg, dwu, dwd, None, None, None, grad, 0, ws, nbytes, None)
     for bad in (dict(grad=F16), dict(grad=4), dict(dy=None), dict(dwg=None), dict(dwd=None)):
         assert bwd(**bad) == -1, bad
         assert b"suhpe_gated_ffn_bwd" in lib.suhpe_last_error()
-    assert lib.suhpe_gated_ffn_bwd(BF16, 3, 0, 16, 24, 16, None, None, None, None, None, None, None, None, None, None, None, None, None, None, None, BF16, 0, None, 0, None) == 0
+    assert lib.suhpe_gated_ffn_bwd(BF16, 3, 0, 16, 24, 16, None, None, None, None, None, None, None, None, None, None, None, None, None, None, BF16, 0, None, 0, None) == 0
     assert lib.suhpe_gated_ffn_bwd_workspace_bytes(BF16, 0, 16, 24, 16) == 0
     assert bwd(nbytes=need - 1) == -3
     assert bwd(ws=None) == -3

@@ -153,8 +153,9 @@ def gated_ffn(x, wg, wu, wd, bg, bu, bd, dy, name, grad_type=None, device="cpu")
     if dy is not None:
         Y = f(dy).reshape(-1, o)
         q = half(grad_type) * 1.001 if grad_type is not None else r
-        # the backward works on g and u as they were rounded
-        eg, eu = e_g + r * (g.abs() + e_g) + tiny, e_u + r * (u.abs() + e_u) + tiny
+        # the backward works on g and u as they were kept: the upper 24 bits, 15 of them behind the leading one
+        kept = 2.0 ** -15
+        eg, eu = e_g + kept * (g.abs() + e_g), e_u + kept * (u.abs() + e_u)
         dh = Y @ D
         e_dh = (o + 2) * U * (Y.abs() @ D.abs())
         e_da = d2 * eg + e_act(g)
