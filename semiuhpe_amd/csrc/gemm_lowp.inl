@@ -513,7 +513,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_lowp(const GemmArgs p) {
                     store8(static_cast<T*>(pr.out) + o, n, limit, hv);
                 }
             } else if constexpr (EPI == EPI_GATE_BWD) {
-                constexpr int BATCH = 8 / (int)sizeof(T) < PASSES ? 8 / (int)sizeof(T) : PASSES;      // rows whose g and u are in flight together
+                constexpr int BATCH = sizeof(T) == 2 || TM == 4 ? 4 : 2;    // rows whose g and u are in flight together
                 static_assert(PASSES % BATCH == 0, "");
 #pragma unroll 1
                 for (int q0 = 0; q0 < PASSES; q0 += BATCH) {

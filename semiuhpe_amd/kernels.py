@@ -1847,7 +1847,8 @@ def gated_ffn_fwd(x, wg, wu, wd, bg=None, bu=None, bd=None, act="silu", save=Tru
     """The gated feed-forward block y = (act(x wg^T + bg) * (x wu^T + bu)) wd^T + bd: x (..., k), wg and wu (n, k), wd (o, n) -> y (..., o) and, with save=True, what
     gated_ffn_bwd needs (both projections, in 24 bits where x has 16, and h, their product, in x's type), else None."""
     dev, m, k, n, o = _ffn_sizes(x, wg, wu, wd, act)
-    x, wg, wu, wd = (_on_16_bytes(t) for t in (x, wg, wu, wd))
+    if (x.data_ptr() | wg.data_ptr() | wu.data_ptr() | wd.data_ptr()) & 15:
+        x, wg, wu, wd = (_on_16_bytes(t) for t in (x, wg, wu, wd))
     for t, name, c in ((bg, "bg", n), (bu, "bu", n), (bd, "bd", o)):
         _chk_tok(t, name, x.dtype, dev, (c,))
     y = torch.empty(x.shape[:-1] + (o,), dtype=x.dtype, device=x.device)
@@ -1883,10 +1884,10 @@ def gated_ffn_bwd(dy, x, wg, wu, wd, saved, act="silu", dwg=None, dwu=None, dwd=
     for t, name, shape in grads:
         _chk_tok(t, name, gtype, dev, shape)
     dx = torch.empty_like(x) if need_dx else None
-    dy, x, wg, wu, wd = (_on_16_bytes(t) for t in (dy, x, wg, wu, wd))
+    if (dy.data_ptr() | x.data_ptr() | wg.data_ptr() | wu.data_ptr() | wd.data_ptr() | h.data_ptr()) & 15:
+        dy, x, wg, wu, wd, h = (_on_16_bytes(t) for t in (dy, x, wg, wu, wd, h))
     nbytes = _lib.load().suhpe_gated_ffn_bwd_workspace_bytes(_DTYPES[x.dtype], m, k, n, o)
     ws = _scratch(nbytes, x.device)
-    h = _on_16_bytes(h)
     _call_on(dev, "suhpe_gated_ffn_bwd", _DTYPES[x.dtype], ACT[act], m, k, n, o, ptr(dy), ptr(x), ptr(wg), ptr(wu), ptr(wd), ptr(kept), ptr(h), ptr(dx),
              ptr(dwg), ptr(dwu), ptr(dwd), ptr(dbg), ptr(dbu), ptr(dbd), _DTYPES[gtype], int(accumulate), ptr(ws), nbytes)
     return dx
