@@ -16,7 +16,8 @@ LIB = os.path.join(CSRC, "libsuhpe.so")
 SOURCES = ["common.hip", "head.hip", "nn_elem.hip", "layout_aug.hip", "conv_igemm.hip", "conv_wino.hip", "conv_wino_small.hip", "dwconv.hip", "attention.hip", "se_fused.hip", "augment.hip", "comm.hip", "raster.hip",
            "token_ops.hip", "gated_ffn.hip"]
 # -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 (some of their forms have given wrong results on MI355X; hipcc -O3 forms them from ordinary float
-# code by itself).  The rounding of every operation is the same without them.  hipcc's host pass warns that it does not know the feature: harmless.
+# code by itself).  Where a packed add kept a product from being fused into it the scalar one may fuse it, so sums can round differently than with them (add_square in
+# common.h).  hipcc's host pass warns that it does not know the feature: harmless.
 FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 

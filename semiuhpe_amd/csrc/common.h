@@ -65,6 +65,17 @@ __device__ __forceinline__ float wave_max(float v) {
     return v;
 }
 
+// v^2 and q + v^2 with both roundings (no fused multiply-add, whatever the target's packed instructions make the compiler prefer): the kernels that emit BatchNorm's
+// statistics records all round alike, and as they did before the packed fp32 instructions were left out
+__device__ __forceinline__ float square(float v) {
+#pragma clang fp contract(off)
+    return v * v;
+}
+__device__ __forceinline__ float add_square(float q, float v) {
+#pragma clang fp contract(off)
+    return q + v * v;
+}
+
 // Predicated loads go through buffer descriptors: a lane that must read zero (padding tap, row beyond M, column beyond N)
 // gets an out-of-range offset and the hardware bounds check returns 0.  With a plain load + select the select sits right
 // behind the load, and the compiler then waits for the data there (before the MFMAs of the current slab) instead of at

@@ -284,7 +284,7 @@ __global__ __launch_bounds__(512) void gemm_nt_dma(const NtParams p, int total_v
 #pragma unroll
                             for (int i = 0; i < TM; ++i)
 #pragma unroll
-                                for (int e = 0; e < 16; ++e) { const float v = acc[i][j][e] - k; a += v; q += v * v; }
+                                for (int e = 0; e < 16; ++e) { const float v = acc[i][j][e] - k; a += v; q = add_square(q, v); }
                         } else {
 #pragma unroll
                             for (int i = 0; i < TM; ++i)
@@ -293,7 +293,7 @@ __global__ __launch_bounds__(512) void gemm_nt_dma(const NtParams p, int total_v
                                     const int lr = i * 32 + (e & 3) + 8 * (e >> 2) + 4 * h;
                                     const float v = (lr >= lo && lr < hi) ? acc[i][j][e] - k : 0.f;
                                     a += v;
-                                    q += v * v;
+                                    q = add_square(q, v);
                                 }
                         }
                         a += __shfl_xor(a, 32, 64);

@@ -333,7 +333,7 @@ void igemm_nt3x3_kernel(const NtParams p, const HaloGeom hg) {
 #pragma unroll
                     for (int i = 0; i < TM; ++i)
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) { const float v = acc[i][j][e] - k; a += v; q += v * v; }
+                        for (int e = 0; e < 16; ++e) { const float v = acc[i][j][e] - k; a += v; q = add_square(q, v); }
                 } else {
 #pragma unroll
                     for (int i = 0; i < TM; ++i)
@@ -342,7 +342,7 @@ void igemm_nt3x3_kernel(const NtParams p, const HaloGeom hg) {
                             const int lr = i * 32 + (e & 3) + 8 * (e >> 2) + 4 * h;
                             const float v = (lr >= wlo && lr < whi) ? acc[i][j][e] - k : 0.f;
                             a += v;
-                            q += v * v;
+                            q = add_square(q, v);
                         }
                 }
                 a += __shfl_xor(a, 32, 64);

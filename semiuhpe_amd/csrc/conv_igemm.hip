@@ -479,7 +479,7 @@ void igemm_nt_kernel(const NtParams p) {
 #pragma unroll
                     for (int i = 0; i < TM; ++i)
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) { const float v = acc[i][j][e] - k; a += v; q += v * v; }
+                        for (int e = 0; e < 16; ++e) { const float v = acc[i][j][e] - k; a += v; q = add_square(q, v); }
                 } else {
 #pragma unroll
                     for (int i = 0; i < TM; ++i)
@@ -488,7 +488,7 @@ void igemm_nt_kernel(const NtParams p) {
                             const int lr = i * 32 + (e & 3) + 8 * (e >> 2) + 4 * h;
                             const float v = (lr >= wlo && lr < whi) ? acc[i][j][e] - k : 0.f;
                             a += v;
-                            q += v * v;
+                            q = add_square(q, v);
                         }
                 }
                 a += __shfl_xor(a, 32, 64);
@@ -713,7 +713,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, (BM * BN >= 128 * 128) 
 #pragma unroll
                         for (int i = 0; i < TM; ++i)
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) { const float v = acc[i][j][e] - k; a += v; q += v * v; }
+                            for (int e = 0; e < 16; ++e) { const float v = acc[i][j][e] - k; a += v; q = add_square(q, v); }
                     } else {
 #pragma unroll
                         for (int i = 0; i < TM; ++i)
@@ -722,7 +722,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, (BM * BN >= 128 * 128) 
                                 const int lr = i * 32 + (e & 3) + 8 * (e >> 2) + 4 * h;
                                 const float v = (lr >= wlo && lr < whi) ? acc[i][j][e] - k : 0.f;
                                 a += v;
-                                q += v * v;
+                                q = add_square(q, v);
                             }
                     }
                     a += __shfl_xor(a, 32, 64);

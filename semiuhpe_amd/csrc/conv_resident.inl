@@ -163,7 +163,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void gemm_nt_resident(const NtPara
 #pragma unroll
                     for (int i = 0; i < TMU; ++i)
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) { const float v = acc[i][e] - k; a += v; q += v * v; }
+                        for (int e = 0; e < 16; ++e) { const float v = acc[i][e] - k; a += v; q = add_square(q, v); }
                 } else {
 #pragma unroll
                     for (int i = 0; i < TMU; ++i)
@@ -172,7 +172,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void gemm_nt_resident(const NtPara
                             const int lr = i * 32 + (e & 3) + 8 * (e >> 2) + 4 * h;
                             const float v = (lr >= lo && lr < hi) ? acc[i][e] - k : 0.f;
                             a += v;
-                            q += v * v;
+                            q = add_square(q, v);
                         }
                 }
                 a += __shfl_xor(a, 32, 64);

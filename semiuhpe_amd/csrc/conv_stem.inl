@@ -61,7 +61,7 @@ __global__ __launch_bounds__(256) void rgb_conv3x3_kernel(const float* __restric
 #pragma unroll
         for (int c = 0; c < COUT; ++c) {
             const float v = in ? acc[c] - kk[c] : 0.f;
-            float a = v, q = v * v;
+            float a = v, q = square(v);
 #pragma unroll
             for (int o = 32; o > 0; o >>= 1) { a += __shfl_xor(a, o, 64); q += __shfl_xor(q, o, 64); }
             if (lane == 0) { red[(wave * COUT + c) * 2] = a; red[(wave * COUT + c) * 2 + 1] = q; }

@@ -426,7 +426,7 @@ __global__ __launch_bounds__(512, 2) void wino_nt_kernel(const NtParams p, const
                     const float k = __int_as_float(__builtin_amdgcn_ds_swizzle(__float_as_int(out[0][e]), 0x0010));
                     float a = 0.f, qq = 0.f;
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) { const float v = out[q][e] - k; a += v; qq += v * v; }
+                    for (int q = 0; q < 4; ++q) { const float v = out[q][e] - k; a += v; qq = add_square(qq, v); }
                     float a1 = first ? a : 0.f, q1 = first ? qq : 0.f, a2 = second ? a : 0.f, q2 = second ? qq : 0.f;
                     a1 += quad_dpp<0x128>(a1); q1 += quad_dpp<0x128>(q1);       // row_ror:8, 4, 2, 1: every lane of the row ends with the row's sum
                     a1 += quad_dpp<0x124>(a1); q1 += quad_dpp<0x124>(q1);

@@ -9,7 +9,8 @@ namespace {
 // Pair p of a head belongs to axis[p] and turns by pos[row][axis[p]] * freq[p] radians.  The angle is formed in 64 bits as REVOLUTIONS (freq holds
 // radians / 2 pi): the whole turns are dropped exactly before the 32-bit sine and cosine, so a position of 10^6 is as exact as one of 10.
 // A block takes R rows: it evaluates sine and cosine of each (row, pair) ONCE into LDS and then streams all heads of those rows past the table
-// (q and k, every head: the evaluation is amortised over heads * rotated vectors).
+// (q and k, every head: the evaluation is amortised over heads * rotated vectors).  Bound by memory: 31 360 rows of 12 heads x (q k v) x 32 fp32 out of place
+// (289 MB) 55 us, 57 600 rows of 16 x 128 bf16 (473 MB) 92 us = 5.2 TB/s, what a large copy reaches.
 template <typename P> __device__ __forceinline__ double pos_of(const P* pos, int64_t i) { return (double)pos[i]; }
 
 struct RopeArgs {
@@ -132,7 +133,8 @@ int rope_types(const void* x, void* y, const void* pos, int pos_type, const Rope
 // ------------------------------------------------------------------------------------------ dropout without a stored mask
 // y_i = [skip_i +] (r_i < keep ? x_i / keep : 0) with r_i the 24-bit number that suhpe_dropout_mask draws for element i at the same stream position:
 // word i % 4 of Philox call counter[1] + position + i / 4.  The gradient is the same call on dy: nothing is kept between the two.
-// A dropped element is 0 whatever x holds there (also infinities and NaN).
+// A dropped element is 0 whatever x holds there (also infinities and NaN).  20 wide multiplies per 4 elements (one 32 x 32 -> 64 bit product gives both halves) hide
+// behind the memory: 24 M bf16 elements, skip + dropout (145 MB) and the gradient (96 MB) 50 us = 4.8 TB/s.
 template <typename T, bool VECTOR>
 __global__ __launch_bounds__(256) void dropout_apply_kernel(const T* x, const T* skip, T* y, int64_t count, uint32_t bound, float scale,
                                                             const uint64_t* __restrict__ counter, uint64_t position) {
@@ -190,7 +192,9 @@ int dropout_launch(const void* x, const void* skip, void* y, int64_t count, uint
 // y = (x - mean) rstd gamma + beta with the statistics, gamma, beta and the parameters' gradients in fp32: only x, y, dy, dx have 16 bits.
 // LPR lanes share a row (8 .. 64, or the 256 of a block), each holding NV vectors of 8 elements in registers between the statistics and the result: one pass
 // over memory.  Blocks are persistent: gamma and beta (8 bytes an element, twice what x and y take together) are loaded once per lane, not once per row, and
-// the next row's loads are issued before this row's sums.  Any width >= 8 runs on full vectors: a row's last vector starts at c - 8 and leaves out of the sums
+// the next row's loads are issued before this row's sums.  125 440 x 192 bf16: forward 17.5 us (5.5 TB/s), backward with the parameters' gradients 35 us
+// (4.1 TB/s; 26 us without them: 48 more accumulators a lane leave two wavefronts per SIMD instead of three, and 512 partial rows are summed by a second launch).
+//  Any width >= 8 runs on full vectors: a row's last vector starts at c - 8 and leaves out of the sums
 // what the vector before it holds (both write the same bits there), and 16-byte accesses may start at any element.
 template <typename T, int LPR, int NV> struct LnRow {
     typename Vec<T, 8>::type v[NV];

@@ -1636,7 +1636,7 @@ def _chk_tok(t, name, dtype=None, dev=None, shape=None):
     if t is None:
         return
     # one test for the calls that are right; what is wrong is looked for only if it fails (these checks are a good part of a small call's time)
-    if torch.is_tensor(t) and t.is_cuda and t.dtype in _DTYPES and (dtype is None or t.dtype is dtype) and t.is_contiguous() \
+    if isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in _DTYPES and (dtype is None or t.dtype is dtype) and t.is_contiguous() \
             and (dev is None or t.get_device() == dev) and (shape is None or t.shape == shape):
         return
     if not torch.is_tensor(t):
@@ -1656,7 +1656,7 @@ def _chk_tok(t, name, dtype=None, dev=None, shape=None):
 
 
 def _chk_counter(counter, dev):
-    if not (torch.is_tensor(counter) and counter.dtype is torch.int64 and counter.shape == (2,) and counter.is_contiguous() and counter.get_device() == dev):
+    if not (isinstance(counter, torch.Tensor) and counter.dtype is torch.int64 and counter.shape == (2,) and counter.is_contiguous() and counter.get_device() == dev):
         raise ValueError(f"counter: an int64 pair (seed, offset) on cuda:{dev}")
 
 
