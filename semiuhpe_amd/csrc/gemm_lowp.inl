@@ -407,6 +407,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_lowp(const GemmArgs p) {
             for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
         issue(s0, 0);
         if (s0 + 1 < s1) issue(s0 + 1, 1);
+        if constexpr (ST == 4) {
+            if (s0 + 2 < s1) issue(s0 + 2, 2);
+            if (s0 + 3 < s1) issue(s0 + 3, 3);
+        }
         // Fragments of a k-group: the weights' side and the last two rows have two register sets in turn, the other rows one: row i's next fragment is read behind the
         // last matrix instruction that takes its present one (256 accumulator and fragment registers hold no second set of all of them).
         i32x4 fa[TM - 2], fz[2][2], fb[2][TN];
@@ -439,17 +443,19 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_lowp(const GemmArgs p) {
             }
         };
         // One barrier per step, between its two k-groups: it publishes the next step's buffer (every wavefront has waited for its own DMA) and frees this step's
-        // (both groups' fragments are in registers), which the DMA of the step after next then fills.  Fragments are read one group ahead throughout.
-        static_assert(KG == 2 && ST == 2, "two buffers of two k-groups");
-        if (s0 + 1 < s1) wait_steps<PA + PB>();
+        // (both groups' fragments are in registers), which the DMA of the step ST later then fills.  Fragments are read one group ahead throughout.
+        static_assert(KG == 2 && (ST == 2 || ST == 4), "two k-groups a step, two or four buffers");
+        if (s0 + ST - 1 < s1) wait_steps<(ST - 1) * (PA + PB)>();
         else wait_steps<0>();
         advance(std::integral_constant<int, 1>{}, true, true, 0, 0);
         for (int s = s0; s < s1; ++s) {
-            const int stage = (s - s0) & 1;
+            const int stage = (s - s0) & (ST - 1);
             advance(std::integral_constant<int, 0>{}, false, true, stage, 1);
-            wait_steps<0>();
-            if (s + 2 < s1) issue(s + 2, stage);
-            advance(std::integral_constant<int, 1>{}, false, true, stage ^ 1, 0);                 // (behind the last step: reads of a finished buffer, not used)
+            if constexpr (ST == 2) wait_steps<0>();
+            else if (s + ST - 1 < s1) wait_steps<(ST - 2) * (PA + PB)>();                         // (the ST - 2 steps behind the next one stay under way)
+            else wait_steps<0>();
+            if (s + ST < s1) issue(s + ST, stage);
+            advance(std::integral_constant<int, 1>{}, false, true, (stage + 1) & (ST - 1), 0);    // (behind the last step: reads of a finished buffer, not used)
         }
 
         // ---- epilogue.  A lane holds 4 columns of a row (8 bytes of a 16-bit row): the sums go through LDS, some rows of each row of wavefronts at a time, and come
@@ -660,13 +666,15 @@ __global__ __launch_bounds__(256) void pad_rows(const T* __restrict__ src, int64
 
 // ------------------------------------------------------------------------------------------ host side
 struct Plan {
-    int big = 0, tiles = 0, whole = 0, splits = 1;
+    int big = 0, tiles = 0, whole = 0, splits = 1, deep = 0;
     int grid() const { return whole + (tiles - whole) * splits; }
     int64_t part_bytes() const { return (int64_t)(tiles - whole) * splits * (big ? 256 * 256 : 128 * 128) * 4; }
 };
 
 // Tile: 256 x 256 (one workgroup of 8 wavefronts per CU) or 128 x 128 (4 wavefronts, two workgroups per CU).  A step of a large tile takes about 1.5 us on the
-// full chip, a step of two small ones 1.0 us for half the work (fp32: 7.8 and 4.2 us); filling the pipeline and storing costs about 6 and 3 us.  Whichever the sizes make cheaper by
+// full chip, a step of two small ones 1.0 us for half the work (fp32: 7.8 and 4.2 us); filling the pipeline and storing costs about 6 and 3 us.  Where no CU gets a second small
+// workgroup, its LDS holds four buffers and three steps of loads stay under way: bf16 1000 x 768 x 2048 forward 42.2 -> 37.1 us, 2048 x 2048 x 5632 gradients 376 -> 340 us (fp32
+// products wait for matrix instructions there: no gain, no loss).  Parts of a tile go down to 4 steps (fp32 500 x 384 x 1024 gradients with 8: 100 us, with 4: 90).  Whichever the sizes make cheaper by
 // that count, padding of the last tiles and the last round of workgroups included, is taken.
 // Shared tiles (products whose epilogue is linear): the tiles beyond the last full round are cut along k in equal parts, whose sums meet in a second launch in
 // the order of k, where the parts' way through memory costs less than the idle CUs.
@@ -683,11 +691,13 @@ inline Plan plan_gemm(int count, const int64_t (*mn)[2], int64_t steps, int es, 
         Plan q;
         q.big = big;
         q.tiles = q.whole = (int)tiles;
-        // (a last round with one small workgroup per CU runs faster than one with two)
-        double tail = rest == 0 ? 0. : (big || rest > slots / 2 ? full : 0.6 * full);
+        // (a last round with one small workgroup per CU runs faster than one with two, with four buffers and 16-bit operands twice as fast)
+        const double alone = es == 2 ? 0.5 : 0.6;
+        double tail = rest == 0 ? 0. : (big || rest > slots / 2 ? full : (tiles <= 256 ? alone : 0.6) * full);
         if (share)
-            for (int64_t z = 2; z <= 64 && rest > 0 && steps / z >= 8; ++z) {
-                const double us = (double)ceil_div(rest * z, slots) * ((double)ceil_div(steps, z) * step + ends) + 6. + (double)(rest * z) * (big ? 0.262 : 0.0655) * 2 / 4.;
+            for (int64_t z = 2; z <= 64 && rest > 0 && steps / z >= 4; ++z) {
+                const double speed = !big && tiles < slots && rest * z <= 256 ? alone : 1.;
+                const double us = (double)ceil_div(rest * z, slots) * ((double)ceil_div(steps, z) * step * speed + ends) + 6. + (double)(rest * z) * (big ? 0.262 : 0.0655) * 2 / 4.;
                 if (us < tail) {
                     tail = us;
                     q.whole = (int)(tiles - rest);
@@ -695,6 +705,7 @@ inline Plan plan_gemm(int count, const int64_t (*mn)[2], int64_t steps, int es, 
                 }
             }
         const double us = (double)(tiles / slots) * full + tail;
+        q.deep = !big && q.grid() <= 256;
         if (!big || us < best_us) {
             best = q;
             best_us = us;
@@ -738,7 +749,13 @@ int gemm_launch(GemmArgs a, int products, const Plan& q, hipStream_t st) {
         hipLaunchKernelGGL(k, grid, dim3(512), lds, st, a);
     } else {
         constexpr auto k = gemm_lowp<T, O, 4, 4, 2, 2, 128, 2, AKM, BKM, EPI>;
-        hipLaunchKernelGGL(k, grid, dim3(256), lds, st, a);
+        constexpr auto deep = gemm_lowp<T, O, 4, 4, 2, 2, 128, 4, AKM, BKM, EPI>;
+        if (q.deep) {
+            if (int rc = allow_lds<deep>(2 * lds)) return rc;
+            hipLaunchKernelGGL(deep, grid, dim3(256), 2 * lds, st, a);
+        } else {
+            hipLaunchKernelGGL(k, grid, dim3(256), lds, st, a);
+        }
     }
     if constexpr (EPI == EPI_STORE)
         if (q.whole < q.tiles) {
