@@ -379,6 +379,17 @@ int space_short(const char* who, const void* workspace, int64_t have, int64_t ne
     return SUHPE_EWORKSPACE;
 }
 
+// no byte of an output in another output or in an input (outputs first; a null pointer is no range): products of one launch write side by side
+struct Range { const void* p; int64_t bytes; };
+bool apart(const Range* r, int outputs, int count) {
+    for (int i = 0; i < outputs; ++i)
+        for (int j = i + 1; j < count; ++j) {
+            const uintptr_t a = reinterpret_cast<uintptr_t>(r[i].p), b = reinterpret_cast<uintptr_t>(r[j].p);
+            if (a && b && a < b + r[j].bytes && b < a + r[i].bytes) return false;
+        }
+    return true;
+}
+
 }  // namespace
 }  // namespace suhpe
 
@@ -436,6 +447,10 @@ int suhpe_gated_ffn_bwd(int dtype, int act, int64_t m, int k, int n, int o, cons
         SUHPE_REQUIRE((d.odd(k) || (aligned(x, 16) && aligned(wg, 16) && aligned(wu, 16))) && (d.odd(n) || (aligned(h, 16) && aligned(wd, 16))) && (d.odd(o) || aligned(dy, 16)),
                       "suhpe_gated_ffn_bwd: dy, x, wg, wu, wd and h start on 16-byte boundaries");
     if (int rc = space_short("suhpe_gated_ffn_bwd", workspace, workspace_bytes, suhpe_gated_ffn_bwd_workspace_bytes(dtype, m, k, n, o))) return rc;
+    const int64_t es = d.es, gs = dtype_size(grad_dtype), nk = (int64_t)n * k, on = (int64_t)o * n;
+    const Range r[] = {{dx, m * k * es}, {dwg, nk * gs}, {dwu, nk * gs}, {dwd, on * gs}, {dbg, n * gs}, {dbu, n * gs}, {dbd, o * gs},
+                       {dy, m * o * es}, {x, m * k * es}, {wg, nk * es}, {wu, nk * es}, {wd, on * es}, {kept, kept_bytes(d.es, m, n)}, {h, m * n * es}};
+    SUHPE_REQUIRE(apart(r, 7, 14), "suhpe_gated_ffn_bwd: the gradients share no memory with each other or with the inputs");
     hipStream_t st = as_stream(stream);
 #define FFN_BWD(T, O) ffn_bwd<T, O>(act, d, dy, x, wg, wu, wd, kept, h, dx, dwg, dwu, dwd, dbg, dbu, dbd, accumulate, workspace, st)
     if (dtype == SUHPE_F32) return FFN_BWD(float, float);

@@ -640,6 +640,7 @@ int suhpe_layernorm16_bwd(const void* x, const void* dy, int dtype, int64_t rows
             return SUHPE_EWORKSPACE;
         }
     }
+    SUHPE_REQUIRE(!dgamma || !dbeta || dgamma + c <= dbeta || dbeta + c <= dgamma, "suhpe_layernorm16_bwd: dgamma and dbeta share no memory");
     float* part = static_cast<float*>(workspace);
     if (dtype == SUHPE_BF16) return ln16_bwd<bf16>(x, dy, rows, c, mean, rstd, gamma, skip, dx, dgamma, dbeta, accumulate, part, as_stream(stream));
     return ln16_bwd<f16>(x, dy, rows, c, mean, rstd, gamma, skip, dx, dgamma, dbeta, accumulate, part, as_stream(stream));

@@ -103,3 +103,23 @@ def test_generator_in_integers():
     a = R.kept(1234, 10, 4000, 0.75)
     assert torch.equal(a[8:], R.kept(1234, 12, 3992, 0.75))
     assert abs(float(a.float().mean()) - 0.75) < 5 * (0.75 * 0.25 / 4000) ** 0.5
+
+
+def test_outputs_that_share_memory(lib):
+    """one buffer for two gradients, or a gradient over an input, is refused before anything runs: the products of a launch write side by side"""
+    need = lib.suhpe_gated_ffn_bwd_workspace_bytes(BF16, 8, 16, 24, 16)
+    # 8 x 16, 24 x 16 and 16 x 24 of 2 bytes fit 768 bytes; kept: 8 * 24 * 6 bytes
+    place = {name: 0x100000 + 0x1000 * i for i, name in enumerate(("dy", "x", "wg", "wu", "wd", "kept", "h", "dx", "dwg", "dwu", "dwd", "dbg", "dbu", "dbd"))}
+
+    def bwd(**moved):
+        at = dict(place, **moved)
+        return lib.suhpe_gated_ffn_bwd(BF16, 3, 8, 16, 24, 16, *(ctypes.c_void_p(p) for p in at.values()), BF16, 0, P, need, None)
+    for bad in (dict(dwu=place["dwg"]), dict(dwd=place["dwg"] + 766), dict(dbu=place["dbg"] + 46), dict(dx=place["x"]), dict(dx=place["dy"]), dict(dwg=place["wg"]),
+                dict(dwd=place["h"]), dict(dbd=place["kept"] + 8 * 24 * 6 - 2)):
+        assert bwd(**bad) == -1, bad
+        assert b"share no memory" in lib.suhpe_last_error()
+    need = lib.suhpe_layernorm16_bwd_workspace_bytes(64)
+    a, b = ctypes.c_void_p(0x100000), ctypes.c_void_p(0x100000 + 252)
+    for dg, db in ((a, a), (a, b), (b, a)):
+        assert lib.suhpe_layernorm16_bwd(P, P, BF16, 4, 64, P, P, None, None, P, dg, db, 0, P, need, None) == -1
+        assert b"share no memory" in lib.suhpe_last_error()
