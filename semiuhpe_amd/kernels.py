@@ -1872,7 +1872,8 @@ def gated_ffn_bwd(dy, x, wg, wu, wd, saved, act="silu", dwg=None, dwu=None, dwd=
         raise ValueError("saved: the forward ran with save=False")
     kept, h = saved
     _chk_tok(h, "saved h", x.dtype, dev, (m, n))
-    if kept.dtype is not torch.uint8 or kept.numel() != _lib.load().suhpe_gated_ffn_kept_bytes(_DTYPES[x.dtype], m, n) or kept.get_device() != dev:
+    if kept.dtype is not torch.uint8 or kept.numel() != _lib.load().suhpe_gated_ffn_kept_bytes(_DTYPES[x.dtype], m, n) or kept.get_device() != dev \
+            or not kept.is_contiguous():
         raise ValueError("saved: not what gated_ffn_fwd returned for rows of this number and type")
     if len({t is None for t in (dwg, dwu, dwd)}) != 1:
         raise ValueError("dwg, dwu, dwd: all three or none")

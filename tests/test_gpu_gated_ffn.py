@@ -103,6 +103,24 @@ def test_large_sizes(K, cfg):
             assert float(off) < (6 * R.half(x.dtype) if dtype != "fp32" else 1e-5), (key, float(off))
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+def test_more_small_tiles_than_compute_units(K, dtype):
+    """small tiles, two to a compute unit (sizes of some hundred small tiles in each product): the form with two buffers"""
+    x, w, b, dy = block(4000, 1496, 1520, 1504, dtype, True)
+    ref = R.gated_ffn(x, *w, *b, dy, "gelu", device="cuda")
+    got, _ = run(K, x, w, b, dy, "gelu")
+    for key, (value, bound) in ref.items():
+        R.within(got[key], value, bound, key)
+
+
+def test_saved_must_be_contiguous(K):
+    x, w, b, dy = block(40, 16, 24, 16, "bf16", True)
+    xs, ws = x.cuda(), cuda(w)
+    _, (kept, h) = K.gated_ffn_fwd(xs, *ws, *cuda(b))
+    with pytest.raises(ValueError, match="saved"):
+        K.gated_ffn_bwd(dy.cuda(), xs, *ws, (torch.zeros(2 * kept.numel(), dtype=torch.uint8, device="cuda")[::2], h))
+
+
 @pytest.mark.parametrize("act", ["silu", "gelu", "sigmoid", "none"])
 def test_activations(K, act):
     x, w, b, dy = block(40, 48, 56, 32, "fp32", True)
