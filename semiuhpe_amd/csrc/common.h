@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <stdio.h>
+#include <type_traits>
 
 #include "../../include/suhpe.h"
 
@@ -65,8 +66,9 @@ __device__ __forceinline__ float wave_max(float v) {
     return v;
 }
 
-// v^2 and q + v^2 with both roundings (no fused multiply-add, whatever the target's packed instructions make the compiler prefer): the kernels that emit BatchNorm's
-// statistics records all round alike, and as they did before the packed fp32 instructions were left out
+// Products and sums with both roundings (no fused multiply-add).  The library is built without packed fp32 instructions (build.py); where those had kept the compiler
+// from fusing a product into a sum, the scalar instructions would let it, and results would move in the last bit.  The places where that happened are written with
+// these (and with fmaf where the fused form was the old one), so that results are what they were and do not hang on which instructions the compiler has.
 __device__ __forceinline__ float square(float v) {
 #pragma clang fp contract(off)
     return v * v;
@@ -74,6 +76,18 @@ __device__ __forceinline__ float square(float v) {
 __device__ __forceinline__ float add_square(float q, float v) {
 #pragma clang fp contract(off)
     return q + v * v;
+}
+__device__ __forceinline__ float product(float a, float b) {            // (stays apart from a sum that takes it)
+#pragma clang fp contract(off)
+    return a * b;
+}
+__device__ __forceinline__ float add_product(float s, float a, float b) {
+#pragma clang fp contract(off)
+    return s + a * b;
+}
+__device__ __forceinline__ float sum_of_products(float a, float b, float c, float d) {
+#pragma clang fp contract(off)
+    return a * b + c * d;
 }
 
 // Predicated loads go through buffer descriptors: a lane that must read zero (padding tap, row beyond M, column beyond N)
@@ -128,6 +142,12 @@ __device__ __forceinline__ float act_apply(float u, int act) {
         case SUHPE_ACT_SIGMOID: return fast_sigmoid(u);
         default: return u;
     }
+}
+// d GELU / du with the half fused into the sum, (1 + erf) / 2 + [u exp(-u^2 / 2) / sqrt(2 pi)]: act_grad rounds the other way round
+__device__ __forceinline__ float gelu_grad_half(float u) {
+    float e;
+    const float q = 1.f + fast_erf(u * 0.70710678118654752f, &e);
+    return fmaf(0.5f, q, u * 0.3989422804014327f * e);
 }
 // d act(u) / du
 __device__ __forceinline__ float act_grad(float u, int act) {

@@ -284,7 +284,12 @@ __global__ __launch_bounds__(512) void gemm_nt_dma(const NtParams p, int total_v
 #pragma unroll
                             for (int i = 0; i < TM; ++i)
 #pragma unroll
-                                for (int e = 0; e < 16; ++e) { const float v = acc[i][j][e] - k; a += v; q = add_square(q, v); }
+                                for (int e = 0; e < 16; ++e) {      // (which squares are fused: see add_square)
+                                    const float v = acc[i][j][e] - k, v0 = acc[0][j][0] - k;
+                                    const int at = i * 16 + e;
+                                    a += v;
+                                    q = at == 0 ? square(v) : at == 1 ? fmaf(v0, v0, square(v)) : at < 16 * (TM - 1) + 3 ? fmaf(v, v, q) : add_square(q, v);
+                                }
                         } else {
 #pragma unroll
                             for (int i = 0; i < TM; ++i)

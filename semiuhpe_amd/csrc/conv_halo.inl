@@ -333,7 +333,11 @@ void igemm_nt3x3_kernel(const NtParams p, const HaloGeom hg) {
 #pragma unroll
                     for (int i = 0; i < TM; ++i)
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) { const float v = acc[i][j][e] - k; a += v; q = add_square(q, v); }
+                        for (int e = 0; e < 16; ++e) {                      // (which squares are fused: see add_square)
+                            const float v = acc[i][j][e] - k;
+                            a += v;
+                            q = TM >= 2 && i == 0 && e == 1 ? fmaf(v, v, q) : add_square(q, v);
+                        }
                 } else {
 #pragma unroll
                     for (int i = 0; i < TM; ++i)

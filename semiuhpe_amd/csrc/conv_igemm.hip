@@ -479,7 +479,11 @@ void igemm_nt_kernel(const NtParams p) {
 #pragma unroll
                     for (int i = 0; i < TM; ++i)
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) { const float v = acc[i][j][e] - k; a += v; q = add_square(q, v); }
+                        for (int e = 0; e < 16; ++e) {                      // (which squares are fused: see add_square)
+                            const float v = acc[i][j][e] - k;
+                            a += v;
+                            q = TM >= 2 && i == 0 && e == 1 ? fmaf(v, v, q) : add_square(q, v);
+                        }
                 } else {
 #pragma unroll
                     for (int i = 0; i < TM; ++i)
@@ -713,7 +717,11 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, (BM * BN >= 128 * 128) 
 #pragma unroll
                         for (int i = 0; i < TM; ++i)
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) { const float v = acc[i][j][e] - k; a += v; q = add_square(q, v); }
+                            for (int e = 0; e < 16; ++e) {                      // (which squares are fused: see add_square)
+                                const float v = acc[i][j][e] - k;
+                                a += v;
+                                q = TM >= 2 && i == 0 && e == 1 ? fmaf(v, v, q) : add_square(q, v);
+                            }
                     } else {
 #pragma unroll
                         for (int i = 0; i < TM; ++i)

@@ -163,7 +163,11 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void gemm_nt_resident(const NtPara
 #pragma unroll
                     for (int i = 0; i < TMU; ++i)
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) { const float v = acc[i][e] - k; a += v; q = add_square(q, v); }
+                        for (int e = 0; e < 16; ++e) {                  // (which squares are fused: see add_square)
+                            const float v = acc[i][e] - k;
+                            a += v;
+                            q = TMU >= 2 && i == 0 && e == 1 ? fmaf(v, v, q) : add_square(q, v);
+                        }
                 } else {
 #pragma unroll
                     for (int i = 0; i < TMU; ++i)

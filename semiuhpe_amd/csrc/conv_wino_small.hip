@@ -277,7 +277,7 @@ __global__ __launch_bounds__(256, 2) void wino_small_kernel(const NtParams p, co
             for (int e = 0; e < 4; ++e) {
                 ks[e] = __int_as_float(__builtin_amdgcn_ds_swizzle(__float_as_int(outp[0][e]), 0x0000));      // lane 0 of the 32-lane half: tile 0, row 0, this quad
                 const float v0 = outp[0][e] - ks[e], v1 = outp[1][e] - ks[e];
-                const float a = v0 + v1, qq = v0 * v0 + v1 * v1;
+                const float a = v0 + v1, qq = add_square(square(v0), v1);
                 as[e] = a + __int_as_float(__builtin_amdgcn_ds_swizzle(__float_as_int(a), 0x401F));           // + lane ^ 16: the tile's other output row
                 qs[e] = qq + __int_as_float(__builtin_amdgcn_ds_swizzle(__float_as_int(qq), 0x401F));
             }

@@ -126,7 +126,10 @@ __device__ __forceinline__ float4 ld4_or_zero(const float* __restrict__ base, bo
     return v;
 }
 __device__ __forceinline__ void fma4(float4& a, const float4& x, const float4& w) {
-    a.x += x.x * w.x; a.y += x.y * w.y; a.z += x.z * w.z; a.w += x.w * w.w;
+    a.x = fmaf(x.x, w.x, a.x); a.y = fmaf(x.y, w.y, a.y); a.z = fmaf(x.z, w.z, a.z); a.w = fmaf(x.w, w.w, a.w);
+}
+__device__ __forceinline__ void madd4(float4& a, const float4& x, const float4& w) {
+    a.x = add_product(a.x, x.x, w.x); a.y = add_product(a.y, x.y, w.y); a.z = add_product(a.z, x.z, w.z); a.w = add_product(a.w, x.w, w.w);
 }
 
 template <bool XF>
@@ -185,8 +188,13 @@ __device__ __forceinline__ void dw_stat_emit(const DwStat& a, bool active, int c
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
                 const float d = e[8 + v] - kb[v];
-                S[v] += e[v] + nt * d;
-                Q[v] += e[4 + v] + 2.f * d * e[v] + nt * d * d;
+                if (v < 2) {                                           // (which products are fused: see add_product)
+                    S[v] += fmaf(nt, d, e[v]);
+                    Q[v] += fmaf(nt * d, d, fmaf(2.f * d, e[v], e[4 + v]));
+                } else {
+                    S[v] += add_product(e[v], nt, d);
+                    Q[v] += add_product(add_product(e[4 + v], 2.f * d, e[v]), nt * d, d);
+                }
             }
             n += nt;
         }
@@ -234,7 +242,9 @@ __global__ __launch_bounds__(256) void dw3x3_row_kernel(const float* __restrict_
             x[r][1] = make_float4(0.f, 0.f, 0.f, 0.f);
             x[r][2] = ld4_xf<XF>(src, rok[r], rbase[r], xf);                      // iw = 0
         }
-        for (int ow = 0; ow < OW; ++ow) {
+        // one output.  With statistics some taps keep both roundings (see add_product): 2, 3, 6, 7 and 8 of every column but the first, with an input
+        // transform 1, 2 and 3
+        auto column = [&](int ow, auto first) __attribute__((always_inline)) {
             const int iw0 = ow * stride - 1;                                    // window columns iw0, iw0+1, iw0+2
             if (stride == 1) {
 #pragma unroll
@@ -255,10 +265,17 @@ __global__ __launch_bounds__(256) void dw3x3_row_kernel(const float* __restrict_
 #pragma unroll
             for (int r = 0; r < 3; ++r)
 #pragma unroll
-                for (int c = 0; c < 3; ++c) fma4(acc, x[r][c], wv[r * 3 + c]);
+                for (int c = 0; c < 3; ++c) {
+                    constexpr int plain = !STATS ? 0 : XF ? 0x00e : decltype(first)::value ? 0 : 0x1cc;
+                    if (plain >> (r * 3 + c) & 1) madd4(acc, x[r][c], wv[r * 3 + c]);
+                    else fma4(acc, x[r][c], wv[r * 3 + c]);
+                }
             *reinterpret_cast<float4*>(dst + ((int64_t)row * OW + ow) * C + coff) = acc;
             if (STATS) { const float o[4] = {acc.x, acc.y, acc.z, acc.w}; dw_stat_add(st, o); }
-        }
+        };
+        constexpr bool own_first = STATS && !XF;
+        if constexpr (own_first) column(0, std::true_type{});
+        for (int ow = own_first ? 1 : 0; ow < OW; ++ow) column(ow, std::false_type{});
     }
     if (STATS) {
         // rows of the first segment: st_a when the thread crossed the boundary, else st if it never left the first segment
@@ -399,9 +416,9 @@ __global__ __launch_bounds__(256) void dw3x3_s1_kernel(const float* __restrict__
 #pragma unroll
                     for (int v = 0; v < 4; ++v) {
                         const float xh = (xv[v] - b_mu[v]) * b_rs[v];
-                        const float g = acc[v] * act_grad(xh * b_ga[v] + b_be[v], bnb.act);
+                        const float g = product(acc[v], act_grad(xh * b_ga[v] + b_be[v], bnb.act));
                         b_s0[v] += g;
-                        b_s1[v] += g * xh;
+                        b_s1[v] = add_product(b_s1[v], g, xh);
                     }
                 }
             }
@@ -588,9 +605,9 @@ __global__ __launch_bounds__(256, (HW == 14 || BNB || (XF && STATS)) ? 2 : 3) vo
 #pragma unroll
                     for (int v = 0; v < 4; ++v) {
                         const float xh = (xv[v] - b_mu[v]) * b_rs[v];
-                        const float gg = o[v] * act_grad(xh * b_ga[v] + b_be[v], bact);
+                        const float da = act_grad(xh * b_ga[v] + b_be[v], bact), gg = ACTC < 0 ? product(o[v], da) : o[v] * da;
                         b_s0[v] += gg;
-                        b_s1[v] += gg * xh;
+                        b_s1[v] = ACTC < 0 ? add_product(b_s1[v], gg, xh) : b_s1[v] + gg * xh;
                     }
                 }
 #pragma unroll
@@ -942,9 +959,9 @@ __global__ __launch_bounds__(256, 2) void dw3x3_bwd_tile_kernel(const float* __r
                         zc[v] = act_apply(u, bact);
                         ag = act_grad(u, bact);
                     }
-                    const float gg = o[v] * ag;
+                    const float gg = ACTC < 0 ? product(o[v], ag) : o[v] * ag;
                     b_s0[v] += gg;
-                    b_s1[v] += gg * xh;
+                    b_s1[v] = ACTC < 0 ? add_product(b_s1[v], gg, xh) : b_s1[v] + gg * xh;
                 }
                 const float4 z4 = make_float4(zc[0], zc[1], zc[2], zc[3]);
 #pragma unroll
@@ -1027,7 +1044,7 @@ __global__ __launch_bounds__(256) void dw3x3_wgrad_row_kernel(const float* __res
             float4 x[3][3];
 #pragma unroll
             for (int r = 0; r < 3; ++r) { x[r][1] = make_float4(0.f, 0.f, 0.f, 0.f); x[r][2] = ld4_xf<XF>(x_, rok[r], rbase[r], xf); }
-            for (int ow = 0; ow < OW; ++ow) {
+            auto column = [&](int ow, auto first) __attribute__((always_inline)) {
                 const int iw0 = ow * stride - 1;
                 if (stride == 1) {
 #pragma unroll
@@ -1048,8 +1065,20 @@ __global__ __launch_bounds__(256) void dw3x3_wgrad_row_kernel(const float* __res
 #pragma unroll
                 for (int r = 0; r < 3; ++r)
 #pragma unroll
-                    for (int c = 0; c < 3; ++c) fma4(acc[r * 3 + c], x[r][c], dv);
-            }
+                    for (int c = 0; c < 3; ++c) {
+                        float4 &a = acc[r * 3 + c], &v = x[r][c];
+                        if (XF && c < 2) {                                 // (which products are fused: see add_product)
+                            a.x = c == 0 ? fmaf(v.x, dv.x, a.x) : add_product(a.x, v.x, dv.x); a.y = c == 0 ? fmaf(v.y, dv.y, a.y) : add_product(a.y, v.y, dv.y);
+                            a.z = c == 1 ? fmaf(v.z, dv.z, a.z) : add_product(a.z, v.z, dv.z); a.w = c == 1 ? fmaf(v.w, dv.w, a.w) : add_product(a.w, v.w, dv.w);
+                        } else if (decltype(first)::value && r > 0 && c == 1) {
+                            madd4(a, v, dv);
+                        } else {
+                            fma4(a, v, dv);
+                        }
+                    }
+            };
+            if constexpr (!XF) column(0, std::true_type{});
+            for (int ow = XF ? 0 : 1; ow < OW; ++ow) column(ow, std::false_type{});
         }
     }
 #pragma unroll

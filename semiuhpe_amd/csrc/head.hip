@@ -94,6 +94,12 @@ __global__ __launch_bounds__(256) void head_ce_kernel(const float* __restrict__ 
     if (dA2 && lane < 9) dA2[9 * (int64_t)b + lane] = (float)da[lane];
 }
 
+// p0 q0 + p1 q1 + p2 q2: the first product fused into the second or the second into the first, the third fused or not (which: see add_product in common.h)
+__device__ __forceinline__ float dot3(float p0, float q0, float p1, float q1, float p2, float q2, bool second, bool plain) {
+    const float t = second ? fmaf(p1, q1, p0 * q0) : fmaf(p0, q0, p1 * q1);
+    return plain ? add_product(t, p2, q2) : fmaf(p2, q2, t);
+}
+
 // one thread per sample: tiny 3x3 products
 __global__ void rot_adjust_kernel(const float* __restrict__ A, const float* __restrict__ aug, int n, int mode,
                                   float* __restrict__ out) {
@@ -103,16 +109,22 @@ __global__ void rot_adjust_kernel(const float* __restrict__ A, const float* __re
 #pragma unroll
     for (int i = 0; i < 9; ++i) { a[i] = A[9 * (int64_t)b + i]; g[i] = aug[9 * (int64_t)b + i]; }
     if (mode == 0) {   // DAD3DHeads: aug * A   (agent.py:113-114)
+#pragma unroll
         for (int i = 0; i < 3; ++i)
-            for (int j = 0; j < 3; ++j) o[3 * i + j] = g[3 * i] * a[j] + g[3 * i + 1] * a[3 + j] + g[3 * i + 2] * a[6 + j];
+#pragma unroll
+            for (int j = 0; j < 3; ++j)
+                o[3 * i + j] = dot3(g[3 * i], a[j], g[3 * i + 1], a[3 + j], g[3 * i + 2], a[6 + j], 0x023 >> (3 * i + j) & 1, 0x100 >> (3 * i + j) & 1);
     } else {           // 300WLP: (D aug D A^T)^T, D = diag(1,-1,-1)   (agent.py:115-120)
         const float dsg[3] = {1.f, -1.f, -1.f};
         float m[9];    // m = D * aug * D
         for (int i = 0; i < 3; ++i)
             for (int j = 0; j < 3; ++j) m[3 * i + j] = dsg[i] * g[3 * i + j] * dsg[j];
         // out = (m A^T)^T = A m^T
+#pragma unroll
         for (int i = 0; i < 3; ++i)
-            for (int j = 0; j < 3; ++j) o[3 * i + j] = a[3 * i] * m[3 * j] + a[3 * i + 1] * m[3 * j + 1] + a[3 * i + 2] * m[3 * j + 2];
+#pragma unroll
+            for (int j = 0; j < 3; ++j)
+                o[3 * i + j] = dot3(a[3 * i], m[3 * j], a[3 * i + 1], m[3 * j + 1], a[3 * i + 2], m[3 * j + 2], 0x0b5 >> (3 * i + j) & 1, 0x145 >> (3 * i + j) & 1);
     }
 #pragma unroll
     for (int i = 0; i < 9; ++i) out[9 * (int64_t)b + i] = o[i];

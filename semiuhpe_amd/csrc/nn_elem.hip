@@ -204,7 +204,11 @@ __global__ __launch_bounds__(256) void bn_stats_partial(const float* __restrict_
             for (int u = 0; u < 8; ++u) {
                 const bool ok = r + u * (int64_t)rp < r1;
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) { const float a = ok ? xv[u][v] - k[v] : 0.f; s0[v] += a; s1[v] += a * a; }
+                for (int v = 0; v < VEC; ++v) {                          // (which squares are fused: see add_square)
+                    const float a = ok ? xv[u][v] - k[v] : 0.f;
+                    s0[v] += a;
+                    s1[v] = VEC == 1 || (u < 2 && v >= 2) ? add_square(s1[v], a) : fmaf(a, a, s1[v]);
+                }
             }
         }
     }
@@ -377,8 +381,8 @@ __global__ void syncbn_finish_kernel(const float* __restrict__ moments, int c, f
     const float var = fmaxf(moments[c + ch] - m * m, 0.f);
     mean[ch] = m;
     rstd[ch] = 1.f / sqrtf(var + eps);
-    if (running_mean) running_mean[ch] = (1.f - momentum) * running_mean[ch] + momentum * m;
-    if (running_var) running_var[ch] = (1.f - momentum) * running_var[ch] + momentum * unbias * var;
+    if (running_mean) running_mean[ch] = sum_of_products(1.f - momentum, running_mean[ch], momentum, m);
+    if (running_var) running_var[ch] = sum_of_products(1.f - momentum, running_var[ch], momentum * unbias, var);
 }
 
 // eval-mode BatchNorm as a per-channel affine map: scale = gamma*rstd, shift = beta - mean*scale
@@ -616,10 +620,10 @@ __global__ __launch_bounds__(256) void bn_bwd_partial(const float* __restrict__ 
                     const float xh = (xv[u][v] - mu[v]) * rs[v];
                     float g;
                     if (yout) g = yv[u][v] > 0.f ? dv[u][v] : 0.f;       // ReLU applied after a pre-activation residual
-                    else g = dv[u][v] * rsc * act_grad(xh * ga[v] + be[v], act);
+                    else g = dv[u][v] * rsc * (ACTC == SUHPE_ACT_GELU ? gelu_grad_half(xh * ga[v] + be[v]) : act_grad(xh * ga[v] + be[v], act));
                     g = ok ? g : 0.f;
                     s0[v] += g;
-                    s1[v] += g * xh;
+                    s1[v] = VEC == 1 ? add_product(s1[v], g, xh) : s1[v] + g * xh;
                 }
             }
         }
@@ -710,7 +714,7 @@ __global__ __launch_bounds__(256) void bn_bwd_apply(const float* __restrict__ x,
                 const float xh = (xv[u][v] - mu[v]) * rs[v];
                 float g;
                 if (yout) g = yv[u][v] > 0.f ? dv[u][v] : 0.f;
-                else g = dv[u][v] * rsc * act_grad(xh * ga[v] + be[v], act);
+                else g = dv[u][v] * rsc * (ACTC == SUHPE_ACT_GELU ? gelu_grad_half(xh * ga[v] + be[v]) : act_grad(xh * ga[v] + be[v], act));
                 g = g - m0[v] - xh * m1[v];
                 o[v] = ga[v] * rs[v] * g;
             }
@@ -819,7 +823,7 @@ __global__ __launch_bounds__(256) void bn3_act_fwd_kernel(Bn3 b, int rows, int c
             for (int v = 0; v < VEC; ++v) {
                 const float a = bn3_pre(b.nb, xv[0][u][v], xv[1][u][v], b.nb == 3 ? xv[2][u][v] : 0.f, sc[0][v], sc[1][v], sc[2][v], sh[v]);
                 o[v] = a > 0.f ? a : 0.f;
-                if (STATS) { const float d = o[v] - k[v]; s0[v] += d; s1[v] += d * d; }
+                if (STATS) { const float d = o[v] - k[v]; s0[v] += d; s1[v] = VEC == 1 ? add_square(s1[v], d) : s1[v] + d * d; }
             }
             vstore<VEC>(y + ((int64_t)rr * cv + vc) * VEC, o);
         }
@@ -882,7 +886,10 @@ __global__ __launch_bounds__(256) void bn3_bwd_partial(Bn3 b, const float* __res
                     s[0][v] += g;
 #pragma unroll
                     for (int j = 0; j < 3; ++j)
-                        if (j < b.nb) s[j + 1][v] += g * (xv[j][u][v] - mu[j][v]) * rs[j][v];
+                        if (j < b.nb) {                                 // (which products are fused: see add_product)
+                            const float t = g * (xv[j][u][v] - mu[j][v]);
+                            s[j + 1][v] = !REMASK && VEC == 4 && j == 0 && u < 2 && v >= 2 ? add_product(s[j + 1][v], t, rs[j][v]) : fmaf(t, rs[j][v], s[j + 1][v]);
+                        }
                 }
             }
         }
@@ -1060,7 +1067,7 @@ __global__ __launch_bounds__(256) void layernorm_fwd_v4(const float* __restrict_
     for (int k = 0; k < NV; ++k)
         if (lane + 64 * k < cv) {
             const float a = v[k].x - m, b = v[k].y - m, cc = v[k].z - m, d = v[k].w - m;
-            q += (a * a + b * b) + (cc * cc + d * d);
+            q += NV == 1 ? add_square(square(a), b) + add_square(square(cc), d) : (a * a + b * b) + (cc * cc + d * d);
         }
     const float rs = 1.f / sqrtf(wave_sum(q) / c + eps);
 #pragma unroll
@@ -1100,7 +1107,7 @@ __global__ __launch_bounds__(256) void layernorm_bwd_dx_v4(const float* __restri
         sk[k][0] = sv.x; sk[k][1] = sv.y; sk[k][2] = sv.z; sk[k][3] = sv.w;
         if (ok) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) { s0 += g[k][e]; s1 += g[k][e] * xh[k][e]; }
+            for (int e = 0; e < 4; ++e) { s0 += g[k][e]; s1 = add_product(s1, g[k][e], xh[k][e]); }
         }
     }
     s0 = wave_sum(s0) / c;
@@ -1128,7 +1135,7 @@ __global__ __launch_bounds__(256) void layernorm_bwd_dx_kernel(const float* __re
         const float g = dy[row * c + j] * (gamma ? gamma[j] : 1.f);
         const float xh = (x[row * c + j] - m) * rs;
         s0 += g;
-        s1 += g * xh;
+        s1 = add_product(s1, g, xh);
     }
     s0 = wave_sum(s0) / c;
     s1 = wave_sum(s1) / c;
@@ -1162,7 +1169,10 @@ __global__ __launch_bounds__(256) void layernorm_bwd_partial(const float* __rest
             vload<VEC>(dy + off, dv);
             const float m = mean[r], rs = rstd[r];
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) { s0[v] += dv[v]; s1[v] += dv[v] * (xv[v] - m) * rs; }
+            for (int v = 0; v < VEC; ++v) {
+                s0[v] += dv[v];
+                s1[v] = VEC == 1 ? add_product(s1[v], dv[v] * (xv[v] - m), rs) : s1[v] + dv[v] * (xv[v] - m) * rs;
+            }
         }
     }
     block_combine<VEC>(s0, s1, cw, rp, col0, c, blockIdx.x, part, lds);
@@ -1475,7 +1485,7 @@ __global__ __launch_bounds__(256) void se_bn_bwd_reduce_kernel(const float* __re
                         ap = act_grad(uu, act);
                     }
                     ap = ok ? ap : 0.f;                              // rows past the sample: no contribution (d = 0 silences z)
-                    const float d = ok ? dv[u][v] : 0.f, dap = d * ap;
+                    const float d = ok ? dv[u][v] : 0.f, dap = ACTC < 0 ? product(d, ap) : d * ap;
                     a[0][v] += d * z;
                     a[1][v] += dap;
                     a[2][v] += dap * xh;
@@ -1614,8 +1624,8 @@ __global__ __launch_bounds__(256) void add_rowscale_kernel(const float* __restri
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             if (i + u * stride >= per_vec) break;
-            float4 o = make_float4(bv[u].x * sc, bv[u].y * sc, bv[u].z * sc, bv[u].w * sc);
-            if (a) { o.x += av[u].x; o.y += av[u].y; o.z += av[u].z; o.w += av[u].w; }
+            const float4 o = a ? make_float4(fmaf(bv[u].x, sc, av[u].x), fmaf(bv[u].y, sc, av[u].y), fmaf(bv[u].z, sc, av[u].z), fmaf(bv[u].w, sc, av[u].w))
+                               : make_float4(bv[u].x * sc, bv[u].y * sc, bv[u].z * sc, bv[u].w * sc);
             reinterpret_cast<float4*>(y)[base + i + u * stride] = o;
         }
     }
@@ -1807,8 +1817,8 @@ __global__ __launch_bounds__(256) void adam_kernel(float* __restrict__ p, const 
         float gi = g[i];
         const float pi = p[i];
         if (wd != 0.f) gi += wd * pi;
-        const float mi = b1 * m[i] + (1.f - b1) * gi;
-        const float vi = b2 * v[i] + (1.f - b2) * gi * gi;
+        const float mi = sum_of_products(b1, m[i], 1.f - b1, gi);
+        const float vi = sum_of_products(b2, v[i], (1.f - b2) * gi, gi);
         m[i] = mi;
         v[i] = vi;
         p[i] = pi - step_size * mi / (sqrtf(vi) / bc2_sqrt + eps);
@@ -1816,7 +1826,7 @@ __global__ __launch_bounds__(256) void adam_kernel(float* __restrict__ p, const 
 }
 __global__ __launch_bounds__(256) void ema_kernel(float* __restrict__ e, const float* __restrict__ p, int64_t count, float alpha) {
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < count; i += (int64_t)gridDim.x * blockDim.x)
-        e[i] = e[i] * alpha + (1.f - alpha) * p[i];
+        e[i] = sum_of_products(e[i], alpha, 1.f - alpha, p[i]);
 }
 __global__ __launch_bounds__(256) void fill_kernel(float* __restrict__ p, int64_t count, float value) {
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < count; i += (int64_t)gridDim.x * blockDim.x) p[i] = value;

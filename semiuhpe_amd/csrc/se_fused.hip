@@ -43,7 +43,9 @@ __global__ __launch_bounds__(kSeThreads) void se_mlp_fwd_kernel(const float* __r
                 const float4 pv = *reinterpret_cast<const float4*>(pl + (ok ? i0 + u * 256 : 0));
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const float d = wv[u][q].x * pv.x + wv[u][q].y * pv.y + wv[u][q].z * pv.z + wv[u][q].w * pv.w;
+                    // (which of the first two products is fused: see add_product)
+                    const float xy = q & 1 ? fmaf(wv[u][q].x, pv.x, wv[u][q].y * pv.y) : fmaf(wv[u][q].y, pv.y, wv[u][q].x * pv.x);
+                    const float d = fmaf(wv[u][q].w, pv.w, fmaf(wv[u][q].z, pv.z, xy));
                     acc[q] += ok ? d : 0.f;
                 }
             }
