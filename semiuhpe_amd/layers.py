@@ -583,7 +583,9 @@ class ResidualDropout(Layer):
         if not self.active():
             if tape is not None:
                 tape.append(None)
-            return K.add(skip, branch)
+            if branch.dtype == torch.float32:
+                return K.add(skip, branch)
+            return K.dropout_apply(branch, 1.0, K.rng_counter(branch.device), 0, skip=skip)     # (16 bits: every element kept, one rounding of the sum)
         if _mask_hook is not None:                          # host-made masks
             mask = draw_mask("dropout", branch.shape, 1.0 - self.p, branch.device)
             if tape is not None:
