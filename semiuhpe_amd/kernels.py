@@ -1742,6 +1742,38 @@ class RopeAxes:
         self.axis = torch.tensor([a for a, w in enumerate(axes) for _ in range(w // 2)], dtype=torch.int32, device=device)
 
 
+_ROPE_PLANS, _ROPE_GRIDS = {}, {}
+
+
+def _made_outside_capture(device, what):
+    if torch.device(device).type == "cuda" and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{what}: not made yet, and a table made inside a graph capture would hold nothing until a replay; run the same sizes once before the capture")
+
+
+def rope_plan(dh, axes, device):
+    """RopeAxes of these axes, made once per device and kept: a captured graph may go on reading its tables"""
+    key = (torch.device(device), int(dh), tuple(axes))
+    plan = _ROPE_PLANS.get(key)
+    if plan is None:
+        _made_outside_capture(device, f"rotary plan {tuple(axes)}")
+        plan = _ROPE_PLANS[key] = RopeAxes(dh, axes, device=device)
+    return plan
+
+
+def rope_grid(images, height, width, device):
+    """positions (row, column) of the tokens of `images` feature maps, int32 (images * height * width, 2).  Tables are kept and never dropped (a captured graph, or
+    another stream, may go on reading one); fewer images than a table holds are the front of it, so a change of batch size costs nothing once the largest has been seen."""
+    rows = images * height * width
+    tables = _ROPE_GRIDS.setdefault((torch.device(device), height, width), [])
+    for t in tables:
+        if t.shape[0] >= rows:
+            return t[:rows]
+    _made_outside_capture(device, f"positions of {images} x {height} x {width} tokens")
+    pos = torch.cartesian_prod(torch.arange(height), torch.arange(width)).to(torch.int32).repeat(images, 1)
+    tables.append(pos.to(device))                           # (pageable memory: the copy has ended when this returns, so any stream may read the table)
+    return tables[-1]
+
+
 _POS_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 
 

@@ -148,7 +148,6 @@ class Attention(Layer):
     def __init__(self, dim, key_dim, num_heads, window, rope=False):
         super().__init__()
         self.rope = rope
-        self._plan, self._grid = None, None
         self.dim, self.key_dim, self.num_heads, self.window = dim, key_dim, num_heads, window
         self.scale = key_dim ** -0.5
         self.norm = LayerNorm(dim)
@@ -178,12 +177,8 @@ class Attention(Layer):
 
     def _turn(self, qkv, B, H, W, inverse):
         """q and k of the packed rows turned in place (qkv is this block's own: the backward works on the turned ones, and its gradient is turned back)"""
-        if self._plan is None or self._plan.freq.device != qkv.device:
-            self._plan = K.RopeAxes(self.key_dim, (self.key_dim // 2, self.key_dim // 2), device=qkv.device)
-        if self._grid is None or self._grid[0] != (B, H, W) or self._grid[1].device != qkv.device:
-            pos = torch.cartesian_prod(torch.arange(H), torch.arange(W)).to(torch.int32).repeat(B, 1)
-            self._grid = ((B, H, W), pos.to(qkv.device))
-        return K.rope_axes(qkv, self._grid[1], self._plan, self.num_heads, parts=3, rotated=2, inverse=inverse, out=qkv)
+        plan = K.rope_plan(self.key_dim, (self.key_dim // 2, self.key_dim // 2), qkv.device)
+        return K.rope_axes(qkv, K.rope_grid(B, H, W, qkv.device), plan, self.num_heads, parts=3, rotated=2, inverse=inverse, out=qkv)
 
     def fwd(self, x, tape, residual=None):
         """residual = (skip, keep scale per sample or None): x + drop_path(attn(x)) closed by the proj GEMM's epilogue (src/tiny_vit.py:366)"""

@@ -24,3 +24,75 @@ def test_residual_dropout_that_drops_nothing(L, dtype, training, p):
     assert torch.equal(layer.fwd2(branch, skip, None), y)
     d_branch, d_skip = layer.bwd2(dy, tape)
     assert torch.equal(d_branch, dy) and torch.equal(d_skip, dy) and not tape
+
+
+def test_captured_block_keeps_its_positions(L):
+    """a captured block with rotary positions, replayed while the same block runs eagerly at other batch sizes and other tensors take and leave memory"""
+    from semiuhpe_amd import kernels as K
+    from semiuhpe_amd.src import tiny_vit
+    torch.manual_seed(5)
+    blk = tiny_vit.TinyViTBlock(96, (14, 14), 3, 7, 4.0, 0.0, mlp="gated", rope=True).cuda().eval()
+    x = torch.randn(4, 14, 14, 96, device="cuda")
+    other = torch.randn(9, 14, 14, 96, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            want = blk.fwd(x, None).clone()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        y = blk.fwd(x, None)
+    table = K.rope_grid(4, 14, 14, x.device).data_ptr()
+    for i in range(3):
+        eager = blk.fwd(other, None)
+        churn = [torch.full((1 << (8 + i), 96), -7, dtype=torch.int32, device="cuda") for i in range(6)]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want), i
+        assert torch.equal(eager, blk.fwd(other, None))
+        del churn
+    assert K.rope_grid(4, 14, 14, x.device).data_ptr() == table
+
+
+def test_rotary_positions_captured_and_replayed(L):
+    """in place and out of place, forward and back, on new contents of the captured tensors"""
+    from semiuhpe_amd import kernels as K
+    plan = K.RopeAxes(32, (16, 16), device="cuda")
+    pos = K.rope_grid(2, 7, 7, torch.device("cuda", torch.cuda.current_device()))
+    x = torch.randn(98, 4 * 3 * 32, device="cuda").to(torch.bfloat16)
+    K.rope_axes(x, pos, plan, 4, parts=3, rotated=2)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        turned = K.rope_axes(x, pos, plan, 4, parts=3, rotated=2)
+        back = K.rope_axes(turned, pos, plan, 4, parts=3, rotated=2, inverse=True)
+    for i in range(3):
+        x.copy_(torch.randn(x.shape, device="cuda") + i)
+        want = K.rope_axes(x, pos, plan, 4, parts=3, rotated=2)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(turned, want) and torch.equal(back, K.rope_axes(want, pos, plan, 4, parts=3, rotated=2, inverse=True))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,c", [(37, 100), (300, 1357)])
+def test_sixteen_bit_layernorm_captured_and_replayed(L, dtype, rows, c):
+    from semiuhpe_amd import kernels as K
+    gamma, beta = torch.rand(c, device="cuda") + 0.5, torch.randn(c, device="cuda")
+    x, dy = (torch.randn(rows, c, device="cuda").to(dtype) for _ in range(2))
+    dgamma, dbeta = torch.zeros(c, device="cuda"), torch.zeros(c, device="cuda")
+
+    def both(dg, db):
+        y, mean, rstd = K.layernorm_fwd(x, c, 1e-5, gamma, beta)
+        return y, K.layernorm_bwd(x, dy, c, mean, rstd, gamma, dg, db)
+    both(dgamma, dbeta)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, dx = both(dgamma, dbeta)
+    for i in range(3):
+        x.copy_(torch.randn(rows, c, device="cuda") * (i + 1)); dy.copy_(torch.randn(rows, c, device="cuda"))
+        dg, db = torch.empty(c, device="cuda"), torch.empty(c, device="cuda")
+        wy, wdx = both(dg, db)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, wy) and torch.equal(dx, wdx) and torch.equal(dgamma, dg) and torch.equal(dbeta, db), i
