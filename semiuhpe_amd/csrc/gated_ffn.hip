@@ -22,7 +22,8 @@ namespace {
 //
 // A 16-byte load from an address that is not a multiple of 4 takes several times as long (13 x 1001 x 2727 fp16, the whole block: 22 us against 10 us for
 // 13 x 1002 x 2726).  ODD: a chunk that starts on an odd element is read as the 16 bytes one element further (at a row's end: one element before) and the element
-// that is missing there, and shifted into place.
+// that is missing there, and shifted into place.  A row of one chunk (last == 0) has no neighbour on either side and is read where it lies.
+template <typename T> __device__ __forceinline__ bool shifted(const T* chunk, int last) { return last > 0 && (reinterpret_cast<uintptr_t>(chunk) & 2); }
 struct Chunk { i32x4 d; unsigned short e; };
 template <typename T, bool ODD> __device__ __forceinline__ Chunk load_k(const T* row, int k, int last) {
     Chunk c;
@@ -31,7 +32,7 @@ template <typename T, bool ODD> __device__ __forceinline__ Chunk load_k(const T*
         __builtin_memcpy(&c.d, row + at, 16);
         c.e = 0;
     } else {
-        const bool odd = reinterpret_cast<uintptr_t>(row + at) & 2;
+        const bool odd = shifted(row + at, last);
         __builtin_memcpy(&c.d, row + at + (odd ? (at < last ? 1 : -1) : 0), 16);
         __builtin_memcpy(&c.e, row + at + (odd && at == last ? 7 : 0), 2);
     }
@@ -42,7 +43,7 @@ template <typename T, bool ODD> __device__ __forceinline__ i32x4 chunk_of(const 
         return c.d;
     } else {
         const int at = k < last ? k : last;
-        const bool odd = reinterpret_cast<uintptr_t>(row + at) & 2, behind = at < last;
+        const bool odd = shifted(row + at, last), behind = at < last;
         const unsigned w[5] = {behind ? (unsigned)c.e << 16 : (unsigned)c.d[0], (unsigned)(behind ? c.d[0] : c.d[1]), (unsigned)(behind ? c.d[1] : c.d[2]),
                                (unsigned)(behind ? c.d[2] : c.d[3]), behind ? (unsigned)c.d[3] : (unsigned)c.e};
         i32x4 v;

@@ -1,0 +1,43 @@
+"""The feed-forward block's few-row (serving) form: operands at any address, against the 64-bit form (tests/token_ops_ref.py)."""
+import pytest
+import torch
+
+import token_ops_ref as R
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def K():
+    from semiuhpe_amd import kernels
+    return kernels
+
+
+def normal(shape, dtype, seed, scale=1.0):
+    return (torch.randn(shape, generator=torch.Generator().manual_seed(seed)) * scale).to(R.TYPES[dtype])
+
+
+def shifted(t, by):
+    """the tensor `by` elements into a buffer of NaN on the device"""
+    buf = torch.full((t.numel() + 32,), float("nan"), dtype=t.dtype, device="cuda")
+    out = buf[by:by + t.numel()].view(t.shape)
+    out.copy_(t)
+    return out
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("m", [1, 3, 16])
+@pytest.mark.parametrize("k,n,o", [(8, 8, 8), (8, 8, 3), (8, 21, 5), (9, 8, 8), (16, 24, 8)])
+def test_operands_off_every_boundary(K, dtype, m, k, n, o):
+    """rows of one chunk and more, every operand one element into a buffer (nothing before or behind a row is taken into it)"""
+    from semiuhpe_amd import _lib
+    x, wg, wu, wd = normal((m, k), dtype, 1), normal((n, k), dtype, 2, k ** -0.5), normal((n, k), dtype, 3, k ** -0.5), normal((o, n), dtype, 4, n ** -0.5)
+    dx, dg, du, dd = (shifted(t, 1) for t in (x, wg, wu, wd))
+    h, y = torch.empty((m, n), dtype=x.dtype, device="cuda"), torch.empty((m, o), dtype=x.dtype, device="cuda")
+    code = K._DTYPES[x.dtype]
+    need = _lib.load().suhpe_gated_ffn_fwd_workspace_bytes(code, m, k, n, o)
+    ws = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda")
+    _lib.call("suhpe_gated_ffn_fwd", code, K.ACT["silu"], m, k, n, o, dx.data_ptr(), dg.data_ptr(), du.data_ptr(), dd.data_ptr(), None, None, None, None,
+              h.data_ptr(), y.data_ptr(), ws.data_ptr() if need else None, need)
+    ref = R.gated_ffn(x, wg, wu, wd, None, None, None, torch.zeros((m, o), dtype=x.dtype), "silu")
+    R.within(y, *ref["y"], "y")
