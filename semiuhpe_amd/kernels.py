@@ -1688,8 +1688,9 @@ def _scratch(nbytes, device):
 
 
 def _on_16_bytes(t):
-    """the tensor, or a copy of one that starts off a 16-byte boundary (a view into another tensor)"""
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    """the tensor, or a copy of one that starts off a 16-byte boundary (a view into another tensor) although its rows are whole 16-byte pieces: rows that are not are
+    copied to padded ones by the call itself"""
+    return t if t.data_ptr() % 16 == 0 or t.shape[-1] * t.element_size() % 16 else t.clone()
 
 
 def _layernorm16_fwd(x, c, eps, gamma, beta):
@@ -1879,7 +1880,8 @@ def gated_ffn_fwd(x, wg, wu, wd, bg=None, bu=None, bd=None, act="silu", save=Tru
     """The gated feed-forward block y = (act(x wg^T + bg) * (x wu^T + bu)) wd^T + bd: x (..., k), wg and wu (n, k), wd (o, n) -> y (..., o) and, with save=True, what
     gated_ffn_bwd needs (both projections, in 24 bits where x has 16, and h, their product, in x's type), else None."""
     dev, m, k, n, o = _ffn_sizes(x, wg, wu, wd, act)
-    if (x.data_ptr() | wg.data_ptr() | wu.data_ptr() | wd.data_ptr()) & 15:
+    few = m <= 32 and min(k, n) * x.element_size() >= 16                # (Dims::few in csrc/gated_ffn.hip: that kernel takes any address)
+    if not few and (x.data_ptr() | wg.data_ptr() | wu.data_ptr() | wd.data_ptr()) & 15:
         x, wg, wu, wd = (_on_16_bytes(t) for t in (x, wg, wu, wd))
     for t, name, c in ((bg, "bg", n), (bu, "bu", n), (bd, "bd", o)):
         _chk_tok(t, name, x.dtype, dev, (c,))

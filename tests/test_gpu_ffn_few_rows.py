@@ -41,3 +41,19 @@ def test_operands_off_every_boundary(K, dtype, m, k, n, o):
               h.data_ptr(), y.data_ptr(), ws.data_ptr() if need else None, need)
     ref = R.gated_ffn(x, wg, wu, wd, None, None, None, torch.zeros((m, o), dtype=x.dtype), "silu")
     R.within(y, *ref["y"], "y")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("m,k,n,o,copies", [(1, 128, 136, 64, 0), (32, 72, 40, 9, 0), (2, 33, 57, 33, 0), (40, 64, 72, 24, 4), (40, 33, 57, 19, 0), (3, 2, 8, 8, 1), (40, 64, 33, 24, 3)])
+def test_operands_are_copied_only_where_the_kernel_asks(K, monkeypatch, dtype, m, k, n, o, copies):
+    """views into a larger buffer: none is copied for few rows (of 16 bytes and more: with k = 2 the tile kernel runs, and wd is copied), nor where the rows are copied to padded ones anyway; the same bits as with operands of their own"""
+    x, wg, wu, wd = normal((m, k), dtype, 1), normal((n, k), dtype, 2, k ** -0.5), normal((n, k), dtype, 3, k ** -0.5), normal((o, n), dtype, 4, n ** -0.5)
+    want, _ = K.gated_ffn_fwd(*(t.cuda() for t in (x, wg, wu, wd)), save=False)
+    views = [shifted(t, 1) for t in (x, wg, wu, wd)]
+    made = []
+    clone = torch.Tensor.clone
+    monkeypatch.setattr(torch.Tensor, "clone", lambda t, *a, **kw: made.append(t) or clone(t, *a, **kw))
+    y, _ = K.gated_ffn_fwd(*views, save=False)
+    monkeypatch.undo()
+    assert len(made) == copies
+    assert torch.equal(y, want)
