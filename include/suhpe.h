@@ -591,7 +591,8 @@ int suhpe_dropout_apply(const void* x, int dtype, int64_t count, float keep, con
 /* counter[1] += by on the device: the last launch of a captured graph that draws, so that its next replay draws fresh numbers */
 int suhpe_dropout_advance(uint64_t* counter, uint64_t by, suhpe_stream_t stream);
 /* LayerNorm of bf16 / fp16 rows with fp32 statistics, parameters and parameter gradients; skip as in suhpe_layernorm_bwd_skip (NULL: none);
- * dgamma / dbeta may be NULL.  workspace: suhpe_layernorm16_bwd_workspace_bytes(c). */
+ * dgamma / dbeta may be NULL.  workspace: suhpe_layernorm16_bwd_workspace_bytes(c).  Forward: y may be x itself; no other output shares memory with an input or
+ * another output (backward: none at all).  rows < 2^31. */
 int suhpe_layernorm16_fwd(const void* x, int dtype, int64_t rows, int c, float eps, const float* gamma, const float* beta, void* y, float* mean, float* rstd,
                           suhpe_stream_t stream);
 int64_t suhpe_layernorm16_bwd_workspace_bytes(int c);

@@ -380,17 +380,6 @@ int space_short(const char* who, const void* workspace, int64_t have, int64_t ne
     return SUHPE_EWORKSPACE;
 }
 
-// no byte of an output in another output or in an input (outputs first; a null pointer is no range): products of one launch write side by side
-struct Range { const void* p; int64_t bytes; };
-bool apart(const Range* r, int outputs, int count) {
-    for (int i = 0; i < outputs; ++i)
-        for (int j = i + 1; j < count; ++j) {
-            const uintptr_t a = reinterpret_cast<uintptr_t>(r[i].p), b = reinterpret_cast<uintptr_t>(r[j].p);
-            if (a && b && a < b + r[j].bytes && b < a + r[i].bytes) return false;
-        }
-    return true;
-}
-
 }  // namespace
 }  // namespace suhpe
 

@@ -36,6 +36,17 @@ inline int dtype_size(int dtype) { return dtype == SUHPE_F32 ? 4 : 2; }
 inline bool dtype_ok(int dtype) { return dtype == SUHPE_F32 || dtype == SUHPE_BF16 || dtype == SUHPE_F16; }
 inline bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
+// no byte of an output in another output or in an input (outputs first; a null pointer is no range): products of one launch write side by side
+struct Range { const void* p; int64_t bytes; };
+inline bool apart(const Range* r, int outputs, int count) {
+    for (int i = 0; i < outputs; ++i)
+        for (int j = i + 1; j < count; ++j) {
+            const uintptr_t a = reinterpret_cast<uintptr_t>(r[i].p), b = reinterpret_cast<uintptr_t>(r[j].p);
+            if (a && b && a < b + r[j].bytes && b < a + r[i].bytes) return false;
+        }
+    return true;
+}
+
 // Philox4x32-10, the generator of suhpe_dropout_mask: the four words of call number `ctr` under key `seed`
 __device__ __forceinline__ void philox_words(uint64_t seed, uint64_t ctr, uint32_t (&w)[4]) {
     uint32_t c0 = (uint32_t)ctr, c1 = (uint32_t)(ctr >> 32), c2 = 0x5355u, c3 = 0x4850u;

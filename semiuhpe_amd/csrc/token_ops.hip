@@ -408,22 +408,23 @@ __global__ __launch_bounds__(256) void layernorm16_bwd_kernel(const T* __restric
     }
 }
 
-// Widths under 8 and over 8192: one wavefront per row, element by element
+// Widths under 8 and over 8192: one wavefront per row at a time, element by element (at most kAnyBlocks workgroups: a launch holds less than 2^32 threads)
+constexpr int64_t kAnyBlocks = 1 << 20;
 template <typename T>
 __global__ __launch_bounds__(256) void layernorm16_fwd_any(const T* __restrict__ x, int64_t rows, int c, float eps, const float* __restrict__ gamma,
                                                            const float* __restrict__ beta, T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
     const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= rows) return;
-    const T* xr = x + row * c;
-    float s = 0.f;
-    for (int j = lane; j < c; j += 64) s += (float)xr[j];
-    const float m = wave_sum(s) / c;
-    float q = 0.f;
-    for (int j = lane; j < c; j += 64) { const float d = (float)xr[j] - m; q += d * d; }
-    const float rs = 1.f / sqrtf(wave_sum(q) / c + eps);
-    for (int j = lane; j < c; j += 64) y[row * c + j] = (T)(((float)xr[j] - m) * rs * (gamma ? gamma[j] : 1.f) + (beta ? beta[j] : 0.f));
-    if (lane == 0) { mean[row] = m; rstd[row] = rs; }
+    for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < rows; row += (int64_t)gridDim.x * 4) {
+        const T* xr = x + row * c;
+        float s = 0.f;
+        for (int j = lane; j < c; j += 64) s += (float)xr[j];
+        const float m = wave_sum(s) / c;
+        float q = 0.f;
+        for (int j = lane; j < c; j += 64) { const float d = (float)xr[j] - m; q += d * d; }
+        const float rs = 1.f / sqrtf(wave_sum(q) / c + eps);
+        for (int j = lane; j < c; j += 64) y[row * c + j] = (T)(((float)xr[j] - m) * rs * (gamma ? gamma[j] : 1.f) + (beta ? beta[j] : 0.f));
+        if (lane == 0) { mean[row] = m; rstd[row] = rs; }
+    }
 }
 
 // dx = rstd (g - mean(g) - xhat mean(g xhat)) [+ skip], g = dy gamma
@@ -432,21 +433,21 @@ __global__ __launch_bounds__(256) void layernorm16_bwd_dx_any(const T* __restric
                                                               const float* __restrict__ mean, const float* __restrict__ rstd, const float* __restrict__ gamma,
                                                               const T* __restrict__ skip, T* __restrict__ dx) {
     const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= rows) return;
-    const float m = mean[row], rs = rstd[row];
-    const int64_t at = row * c;
-    float s0 = 0.f, s1 = 0.f;
-    for (int j = lane; j < c; j += 64) {
-        const float g = (float)dy[at + j] * (gamma ? gamma[j] : 1.f);
-        s0 += g;
-        s1 += g * (((float)x[at + j] - m) * rs);
-    }
-    s0 = wave_sum(s0) / c;
-    s1 = wave_sum(s1) / c;
-    for (int j = lane; j < c; j += 64) {
-        const float g = (float)dy[at + j] * (gamma ? gamma[j] : 1.f), xh = ((float)x[at + j] - m) * rs;
-        dx[at + j] = (T)(rs * (g - s0 - xh * s1) + (skip ? (float)skip[at + j] : 0.f));
+    for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < rows; row += (int64_t)gridDim.x * 4) {
+        const float m = mean[row], rs = rstd[row];
+        const int64_t at = row * c;
+        float s0 = 0.f, s1 = 0.f;
+        for (int j = lane; j < c; j += 64) {
+            const float g = (float)dy[at + j] * (gamma ? gamma[j] : 1.f);
+            s0 += g;
+            s1 += g * (((float)x[at + j] - m) * rs);
+        }
+        s0 = wave_sum(s0) / c;
+        s1 = wave_sum(s1) / c;
+        for (int j = lane; j < c; j += 64) {
+            const float g = (float)dy[at + j] * (gamma ? gamma[j] : 1.f), xh = ((float)x[at + j] - m) * rs;
+            dx[at + j] = (T)(rs * (g - s0 - xh * s1) + (skip ? (float)skip[at + j] : 0.f));
+        }
     }
 }
 
@@ -499,6 +500,7 @@ __global__ __launch_bounds__(1024) void layernorm16_bwd_finish(const float* __re
 }
 
 constexpr int kLnBlocks = 512;
+inline unsigned any_blocks(int64_t rows) { return (unsigned)(ceil_div(rows, 4) < kAnyBlocks ? ceil_div(rows, 4) : kAnyBlocks); }
 
 // lanes per row and vectors per lane for a width: as few lanes as hold the row in at most 3 vectors each (the sums cross few lanes and the parameters' registers
 // stay few), then the whole block
@@ -522,7 +524,7 @@ int ln16_fwd(const void* x, int64_t rows, int c, float eps, const float* gamma, 
     const T* xt = static_cast<const T*>(x);
     T* yt = static_cast<T*>(y);
     if (c < 8 || c > 8192) {
-        hipLaunchKernelGGL((layernorm16_fwd_any<T>), dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, st, xt, rows, c, eps, gamma, beta, yt, mean, rstd);
+        hipLaunchKernelGGL((layernorm16_fwd_any<T>), dim3(any_blocks(rows)), dim3(256), 0, st, xt, rows, c, eps, gamma, beta, yt, mean, rstd);
     } else {
 #define LN16_FWD(L, V)                                                                                                                                           \
     do {                                                                                                                                                         \
@@ -543,7 +545,7 @@ int ln16_bwd(const void* x, const void* dy, int64_t rows, int c, const float* me
     const bool want = dgamma || dbeta;
     int blocks = 0;
     if (rows > 0 && (c < 8 || c > 8192)) {
-        hipLaunchKernelGGL((layernorm16_bwd_dx_any<T>), dim3((unsigned)ceil_div(rows, 4)), dim3(256), 0, st, xt, dt, rows, c, mean, rstd, gamma, kt, ot);
+        hipLaunchKernelGGL((layernorm16_bwd_dx_any<T>), dim3(any_blocks(rows)), dim3(256), 0, st, xt, dt, rows, c, mean, rstd, gamma, kt, ot);
         if (want) {
             blocks = (int)(ceil_div(rows, 16) < kLnBlocks ? ceil_div(rows, 16) : kLnBlocks);
             const int64_t per = ceil_div(rows, blocks);
@@ -622,6 +624,10 @@ int suhpe_layernorm16_fwd(const void* x, int dtype, int64_t rows, int c, float e
     SUHPE_REQUIRE(rows >= 0 && c > 0 && rows <= 0x7fffffffll, "suhpe_layernorm16_fwd: bad sizes");
     if (rows == 0) return SUHPE_OK;
     SUHPE_REQUIRE(x && y && mean && rstd, "suhpe_layernorm16_fwd: null pointer");
+    // (a wavefront holds its row in registers between reading and writing: y may be x itself)
+    const int64_t row_bytes = rows * c * 2;
+    const Range r[] = {{y, row_bytes}, {mean, rows * 4}, {rstd, rows * 4}, {x == y ? nullptr : x, row_bytes}, {gamma, (int64_t)c * 4}, {beta, (int64_t)c * 4}};
+    SUHPE_REQUIRE(apart(r, 3, 6), "suhpe_layernorm16_fwd: y (unless it is x), mean and rstd share no memory with each other or with the inputs");
     if (dtype == SUHPE_BF16) return ln16_fwd<bf16>(x, rows, c, eps, gamma, beta, y, mean, rstd, as_stream(stream));
     return ln16_fwd<f16>(x, rows, c, eps, gamma, beta, y, mean, rstd, as_stream(stream));
 }
@@ -640,7 +646,10 @@ int suhpe_layernorm16_bwd(const void* x, const void* dy, int dtype, int64_t rows
             return SUHPE_EWORKSPACE;
         }
     }
-    SUHPE_REQUIRE(!dgamma || !dbeta || dgamma + c <= dbeta || dbeta + c <= dgamma, "suhpe_layernorm16_bwd: dgamma and dbeta share no memory");
+    const int64_t row_bytes = rows * c * 2;
+    const Range r[] = {{rows ? dx : nullptr, row_bytes}, {dgamma, (int64_t)c * 4}, {dbeta, (int64_t)c * 4}, {dgamma || dbeta ? workspace : nullptr, suhpe_layernorm16_bwd_workspace_bytes(c)},
+                       {x, row_bytes}, {dy, row_bytes}, {skip, row_bytes}, {mean, rows * 4}, {rstd, rows * 4}, {gamma, (int64_t)c * 4}};
+    SUHPE_REQUIRE(apart(r, 4, 10), "suhpe_layernorm16_bwd: dx, dgamma, dbeta and the workspace share no memory with each other or with the inputs");
     float* part = static_cast<float*>(workspace);
     if (dtype == SUHPE_BF16) return ln16_bwd<bf16>(x, dy, rows, c, mean, rstd, gamma, skip, dx, dgamma, dbeta, accumulate, part, as_stream(stream));
     return ln16_bwd<f16>(x, dy, rows, c, mean, rstd, gamma, skip, dx, dgamma, dbeta, accumulate, part, as_stream(stream));

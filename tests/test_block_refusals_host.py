@@ -1,0 +1,42 @@
+"""What the C entry points of the transformer-block operators refuse about memory: decided on the host, nothing is launched."""
+import ctypes
+
+import pytest
+
+BF16 = 1
+AT = 1 << 30
+
+
+def P(offset=0):
+    return ctypes.c_void_p(AT + offset)
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from semiuhpe_amd import _lib
+    return _lib.load()
+
+
+ROWS, C = 100, 60                                           # 12 000 bytes a tensor of rows, 240 a parameter
+PLACES = dict(x=0, dy=1 << 16, dx=2 << 16, skip=3 << 16, mean=4 << 16, rstd=5 << 16, gamma=6 << 16, dgamma=7 << 16, dbeta=8 << 16, ws=1 << 24)
+
+
+def backward(lib, **moved):
+    at = {k: P(moved.get(k, v)) for k, v in PLACES.items()}
+    need = lib.suhpe_layernorm16_bwd_workspace_bytes(C)
+    return lib.suhpe_layernorm16_bwd(at["x"], at["dy"], BF16, ROWS, C, at["mean"], at["rstd"], at["gamma"], at["skip"], at["dx"], at["dgamma"], at["dbeta"], 0, at["ws"], need, None)
+
+
+@pytest.mark.parametrize("moved", [dict(dx=PLACES["x"]), dict(dx=PLACES["dy"]), dict(dx=PLACES["skip"]), dict(dx=PLACES["skip"] + 11998), dict(dx=PLACES["dy"] - 11998),
+                                   dict(dgamma=PLACES["gamma"]), dict(dgamma=PLACES["dbeta"] - 236), dict(dbeta=PLACES["x"] + 4), dict(dgamma=PLACES["mean"] + 396),
+                                   dict(dx=PLACES["rstd"]), dict(ws=PLACES["dx"]), dict(ws=PLACES["gamma"] - 1024), dict(dgamma=PLACES["ws"] + 64)])
+def test_layernorm16_backward_refuses_shared_memory(lib, moved):
+    assert backward(lib, **moved) == -1, moved
+    assert b"suhpe_layernorm16_bwd" in lib.suhpe_last_error() and b"share no memory" in lib.suhpe_last_error()
+
+
+@pytest.mark.parametrize("moved", [dict(y=2), dict(y=-11998), dict(mean=PLACES["x"]), dict(rstd=PLACES["mean"] + 396), dict(mean=PLACES["gamma"] - 396), dict(y=PLACES["rstd"])])
+def test_layernorm16_forward_refuses_shared_memory(lib, moved):
+    at = {k: P(moved.get(k, v)) for k, v in dict(PLACES, y=2 << 16, beta=9 << 16).items()}
+    assert lib.suhpe_layernorm16_fwd(at["x"], BF16, ROWS, C, ctypes.c_float(1e-5), at["gamma"], at["beta"], at["y"], at["mean"], at["rstd"], None) == -1, moved
+    assert b"share no memory" in lib.suhpe_last_error()

@@ -96,3 +96,22 @@ def test_sixteen_bit_layernorm_captured_and_replayed(L, dtype, rows, c):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, wy) and torch.equal(dx, wdx) and torch.equal(dgamma, dg) and torch.equal(dbeta, db), i
+
+
+def test_sixteen_bit_layernorm_of_very_many_short_rows(L):
+    """more rows than one launch has wavefronts (2^26 + 5 rows of 4): the same bits as in two halves, gradients too"""
+    from semiuhpe_amd import kernels as K
+    rows, c = (1 << 26) + 5, 4
+    x = torch.randn(rows, c, device="cuda", dtype=torch.bfloat16)
+    dy = torch.randn(rows, c, device="cuda", dtype=torch.bfloat16)
+    gamma, beta = torch.rand(c, device="cuda") + 0.5, torch.randn(c, device="cuda")
+    y, mean, rstd = K.layernorm_fwd(x, c, 1e-5, gamma, beta)
+    dx = K.layernorm_bwd(x, dy, c, mean, rstd, gamma)
+    cut = 1 << 25
+    for part in (slice(0, cut), slice(cut, rows)):
+        py, pm, pr = K.layernorm_fwd(x[part], c, 1e-5, gamma, beta)
+        assert torch.equal(y[part], py) and torch.equal(mean[part], pm) and torch.equal(rstd[part], pr)
+        assert torch.equal(dx[part], K.layernorm_bwd(x[part], dy[part], c, pm, pr, gamma))
+    last = x[-7:].double()
+    want = (last - last.mean(1, keepdim=True)) / torch.sqrt(last.var(1, unbiased=False, keepdim=True) + 1e-5) * gamma.double() + beta.double()
+    assert float((y[-7:].double() - want).abs().max()) < 2.0 ** -8 * float(want.abs().max()) * 1.01 + 1e-5       # (half a step of bf16, fp32 sums of four)
