@@ -113,7 +113,8 @@ int rope_launch(const T* x, T* y, const P* pos, RopeArgs a, hipStream_t st) {
     if (r < 1) r = 1;
     if (r > a.rows) r = a.rows;
     a.rows_per_block = (int)r;
-    const dim3 grid((unsigned)ceil_div(a.rows, r));
+    SUHPE_REQUIRE(ceil_div(a.rows, r) < (1 << 24), "suhpe_rope_axes: %lld rows of %lld elements are more than one launch holds", (long long)a.rows, (long long)width);
+    const dim3 grid((unsigned)ceil_div(a.rows, r));                    // (2^24 workgroups of 256: some 2^36 elements)
     const size_t lds = (size_t)r * a.pairs * sizeof(float2);
     if (fits(FULL)) hipLaunchKernelGGL((rope_axes_kernel<T, P, FULL>), grid, dim3(256), lds, st, x, y, pos, a);
     else if (fits(FULL / 2)) hipLaunchKernelGGL((rope_axes_kernel<T, P, FULL / 2>), grid, dim3(256), lds, st, x, y, pos, a);

@@ -40,3 +40,9 @@ def test_layernorm16_forward_refuses_shared_memory(lib, moved):
     at = {k: P(moved.get(k, v)) for k, v in dict(PLACES, y=2 << 16, beta=9 << 16).items()}
     assert lib.suhpe_layernorm16_fwd(at["x"], BF16, ROWS, C, ctypes.c_float(1e-5), at["gamma"], at["beta"], at["y"], at["mean"], at["rstd"], None) == -1, moved
     assert b"share no memory" in lib.suhpe_last_error()
+
+
+def test_rope_axes_refuses_more_than_one_launch_holds(lib):
+    """2^31 - 1 rows of 64 fp32 elements: 64 rows a workgroup of 256 threads would be 2^33 threads"""
+    assert lib.suhpe_rope_axes(P(), 0, (1 << 31) - 1, 1, 1, 1, 64, P(1 << 20), 0, 1, P(2 << 20), P(3 << 20), 32, 1, 0, P(), None) == -1
+    assert b"one launch" in lib.suhpe_last_error()
