@@ -3,7 +3,7 @@
     python -m semiuhpe_amd.build          # or semiuhpe_amd.build.build()
 
 hipcc cross-compiles without a GPU; the .so stays next to the sources (semiuhpe_amd/csrc/libsuhpe.so) so that it
-travels with the repo snapshot to the GPU box.  Objects are rebuilt only when a source or header is newer.
+travels with a copy of the tree.  An object is rebuilt when a source or header is newer, or when it was compiled with another compiler or other flags (build/flags.txt).
 """
 import os
 import subprocess
@@ -15,9 +15,9 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(CSRC, "libsuhpe.so")
 SOURCES = ["common.hip", "head.hip", "nn_elem.hip", "layout_aug.hip", "conv_igemm.hip", "conv_wino.hip", "conv_wino_small.hip", "dwconv.hip", "attention.hip", "se_fused.hip", "augment.hip", "comm.hip", "raster.hip",
            "token_ops.hip", "gated_ffn.hip"]
-# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 (some of their forms have given wrong results on MI355X; hipcc -O3 forms them from ordinary float
-# code by itself).  Where a packed add kept a product from being fused into it the scalar one may fuse it, so sums can round differently than with them (add_square in
-# common.h).  hipcc's host pass warns that it does not know the feature: harmless.
+# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32, which hipcc -O3 forms from ordinary float code by itself.  The library is built without them as a precaution for the cards it
+# runs on (no case of a wrong result is known from this code); EfficientNetV2-S pays 2 % of its step for it (46.7 -> 47.5 ms).  Which products are fused into sums is
+# written in the kernels (add_product in common.h), so results do not hang on the flag.  hipcc's host pass warns that it does not know the feature: harmless.
 FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
@@ -41,6 +41,11 @@ def build(force=False, verbose=True):
     os.makedirs(objdir, exist_ok=True)
     hdr_time = _newest_header()
     srcs = [s for s in SOURCES if os.path.exists(os.path.join(CSRC, s))]
+    stamp, used = os.path.join(objdir, "flags.txt"), " ".join([hipcc] + FLAGS)
+    if not os.path.exists(stamp) or open(stamp).read() != used:
+        force = True                                        # objects of other flags (or of unknown ones) are not linked with these
+        if os.path.exists(stamp):
+            os.remove(stamp)                                # (written again when every object has been compiled)
     jobs = []
     for s in srcs:
         src = os.path.join(CSRC, s)
@@ -58,6 +63,8 @@ def build(force=False, verbose=True):
     if jobs:
         with ThreadPoolExecutor(max_workers=8) as ex:
             list(ex.map(compile_one, jobs))
+    with open(stamp, "w") as f:
+        f.write(used)
     objs = [os.path.join(objdir, s.replace(".hip", ".o")) for s in srcs]
     if jobs or not os.path.exists(LIB) or os.path.getmtime(LIB) < max(os.path.getmtime(o) for o in objs):
         cmd = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs + ["-ldl"]
