@@ -439,8 +439,12 @@ class SSLAgent:
         opt = {"state": {i: {k: (v.detach().cpu().contiguous().clone() if torch.is_tensor(v) else v) for k, v in st.items()}
                          for i, st in sd["state"].items()},
                "param_groups": [dict(g) for g in sd["param_groups"]]}
-        torch.save({"clock": self.clock.make_checkpoint(), "model_state_dict": host(self.net.state_dict()),
-                    "model_state_dict_ema": host(self.ema_net.state_dict()), "optimizer_state_dict": opt}, save_path)
+        checkpoint = {"clock": self.clock.make_checkpoint(), "model_state_dict": host(self.net.state_dict()),
+                      "model_state_dict_ema": host(self.ema_net.state_dict()), "optimizer_state_dict": opt}
+        options = getattr(self.net, "options", {})
+        if options:                                         # (the reference's networks have none: the reference's four keys)
+            checkpoint["network_options"] = dict(options)
+        torch.save(checkpoint, save_path)
 
     def load_ckpt(self, name=None):
         """reference :333-354"""
@@ -449,6 +453,11 @@ class SSLAgent:
             raise ValueError("Checkpoint {} not exists.".format(load_path))
         checkpoint = torch.load(load_path, map_location=torch.device("cpu"))
         print("Loading checkpoint from {} ...".format(load_path))
+        # options that no parameter shows (rotary positions): with others than it was trained with, the checkpoint would load and be a different network
+        trained, mine = checkpoint.get("network_options", {}), getattr(self.net, "options", {})
+        if trained != mine:
+            raise ValueError(f"Checkpoint {load_path} holds a network with options {trained or 'none'}, this one was built with {mine or 'none'}: "
+                             "give the same --vit_mlp / --vit_rope")
         self.net.load_state_dict(checkpoint["model_state_dict"])
         if "model_state_dict_ema" in checkpoint.keys():
             self.ema_net.load_state_dict(checkpoint["model_state_dict_ema"])

@@ -372,6 +372,8 @@ class TinyViT21M(Network):
 
     def __init__(self, num_classes=9, drop_path_rate=0.2, mlp="gelu", rope=False, drop=0.0):
         super().__init__()
+        # what a checkpoint has to say of the network it holds: options that change its outputs and that the parameters' names and shapes may not show
+        self.options = {k: v for k, v in (("vit_mlp", mlp), ("vit_rope", bool(rope))) if v not in ("gelu", False)}
         d = self.DIMS
         self.patch_embed = PatchEmbed(3, d[0])
         dpr = [v.item() for v in torch.linspace(0, drop_path_rate, sum(self.DEPTHS))]
