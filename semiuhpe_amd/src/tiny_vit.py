@@ -273,7 +273,7 @@ class GatedMlp(Layer):
         self.norm = LayerNorm(in_features)
         self.ffn = GatedFeedForward(in_features, hidden_features // 3 * 2)
 
-    def fwd(self, x, tape, residual=None):
+    def fwd(self, x, tape):                                 # (no residual: the block joins it, TinyViTBlock._join)
         return self.ffn.fwd(self.norm.fwd(x, tape), tape)
 
     def bwd(self, dy, tape, skip=None):
