@@ -5,7 +5,8 @@
 // Forward, two products: [g | u] with the activation and the product in the epilogue (a tile takes the SAME columns of Wg and Wu, so both factors of an
 // output element meet in one lane's registers), then y.  Backward, four: dh whose epilogue turns it into dg and du at once (dh itself is never stored),
 // dx as one product over two ranges of n, and the three weight gradients in one launch.  h, dg and du are rounded to the tensors' type once on their way to memory
-// (they are operands of 16-bit matrix instructions next), g and u keep 24 bits; every sum runs in fp32.
+// (they are operands of 16-bit matrix instructions next; few rows, where the weights are the traffic, multiply what h's rounding left as well), g and u keep 24 bits;
+// every sum runs in fp32.
 #include "lowp.h"
 #include "gemm_lowp.inl"
 
@@ -18,6 +19,8 @@ namespace {
 // P > 1 (at most 16 / P rows of x): the 16 x 16 matrix instruction takes P stretches of k at once -- weight row r and x row m of stretch p in its rows and columns
 // 16 / P * p + r, + m -- and the blocks on its diagonal are summed: P times as many workgroups, and P * 64 bytes of a weight row side by side in one load.
 // 1 x 2048 x 5632 bf16 (69 MB of weights): 15.3 us = 4.5 TB/s with P = 4, 22 us with P = 1.
+// LO: x comes in two parts, rounded and what the rounding left (h between the two products), and each weight fragment is multiplied with both: y is then as exact as with h in
+// 16 + 8 bits (bf16: 2^-16 of h is left out, rounding h alone 2^-8; fp16: 2^-22 or 2^-25), for m more 16-bit rows out of L2 beside the weights out of memory.
 // Rows may start at any element (16-byte loads from any address); the last chunk of a row starts at K - CH, with what the chunk before it holds set to zero.
 //
 // A 16-byte load from an address that is not a multiple of 4 takes several times as long (13 x 1001 x 2727 fp16, the whole block: 22 us against 10 us for
@@ -61,27 +64,28 @@ template <typename T> __device__ __forceinline__ i32x4 drop_first(i32x4 v, int g
     return __builtin_bit_cast(i32x4, e);
 }
 
-template <typename T, int P, int MT, int W, bool GATE, bool ODD>
-__global__ __launch_bounds__(64 * W) void ffn_few_rows(const T* __restrict__ x, int M, int64_t K, const T* __restrict__ w, const T* __restrict__ w2, int N, const T* __restrict__ bias,
-                                                       const T* __restrict__ bias2, int act, void* kept, T* __restrict__ out) {
-    static_assert(P == 1 || MT == 1, "");
+template <typename T, int P, int MT, int W, bool GATE, bool LO, bool ODD>
+__global__ __launch_bounds__(64 * W) void ffn_few_rows(const T* __restrict__ x, const T* __restrict__ xlo, int M, int64_t K, const T* __restrict__ w, const T* __restrict__ w2, int N,
+                                                       const T* __restrict__ bias, const T* __restrict__ bias2, int act, void* kept, T* __restrict__ out, T* __restrict__ lo_out) {
+    static_assert((P == 1 || MT == 1) && !(GATE && LO), "");
     constexpr int CH = 16 / (int)sizeof(T), KE = 4 * CH * P, S = GATE ? 2 : 1, R = 16 / P;      // KE: k of one matrix step
     __shared__ float sums[W * P][S][MT][16 * R];
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, t = lane & 15, g = lane >> 4;
     const int n0 = blockIdx.x * R, part = t / R, rt = t % R, nr = n0 + rt < N ? n0 + rt : N - 1;
     const T *r1 = w + nr * K, *r2 = GATE ? w2 + nr * K : nullptr;
-    const T* xr[MT];
+    constexpr int MX = LO ? 2 * MT : MT;                                    // fragments of x: MT of its rows, then MT of what their rounding left
+    const T* xr[MX];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) xr[i] = x + (int64_t)(16 * i + rt < M ? 16 * i + rt : M - 1) * K;
+    for (int i = 0; i < MX; ++i) xr[i] = (i < MT ? x : xlo) + (int64_t)(16 * (i % MT) + rt < M ? 16 * (i % MT) + rt : M - 1) * K;
     const int steps = (int)((K + KE - 1) / KE), lo = steps * wave / W, hi = steps * (wave + 1) / W, last = (int)K - CH;
     f32x4 acc[S][MT];
 #pragma unroll
     for (int s = 0; s < S; ++s)
 #pragma unroll
         for (int i = 0; i < MT; ++i) acc[s][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    constexpr int U = GATE || MT > 1 ? 4 : 8;                              // steps whose loads are in flight together
+    constexpr int U = MX > 2 && ODD ? 2 : GATE || MX > 1 ? 4 : 8;          // steps whose loads are in flight together (128 registers a lane hold no more)
     for (int q = lo; q < hi; q += U) {
-        Chunk ca[U][S], cb[U][MT];
+        Chunk ca[U][S], cb[U][MX];
 #pragma unroll
         for (int v = 0; v < U; ++v) {
             if (q + v >= hi) break;
@@ -89,29 +93,29 @@ __global__ __launch_bounds__(64 * W) void ffn_few_rows(const T* __restrict__ x, 
             ca[v][0] = load_k<T, ODD>(r1, k, last);
             if constexpr (GATE) ca[v][1] = load_k<T, ODD>(r2, k, last);
 #pragma unroll
-            for (int i = 0; i < MT; ++i) cb[v][i] = load_k<T, ODD>(xr[i], k, last);
+            for (int i = 0; i < MX; ++i) cb[v][i] = load_k<T, ODD>(xr[i], k, last);
         }
 #pragma unroll
         for (int v = 0; v < U; ++v) {
             if (q + v >= hi) break;
             const int k = (q + v) * KE + (part * 4 + g) * CH;
-            i32x4 a[S], b[MT];
+            i32x4 a[S], b[MX];
             a[0] = chunk_of<T, ODD>(ca[v][0], r1, k, last);
             if constexpr (GATE) a[1] = chunk_of<T, ODD>(ca[v][1], r2, k, last);
 #pragma unroll
-            for (int i = 0; i < MT; ++i) b[i] = chunk_of<T, ODD>(cb[v][i], xr[i], k, last);
+            for (int i = 0; i < MX; ++i) b[i] = chunk_of<T, ODD>(cb[v][i], xr[i], k, last);
             if ((q + v + 1) * KE > K) {                                // the row ends in this step
                 const int over = k - last;
                 const int gone = over < 0 ? 0 : over > CH ? CH : over;
 #pragma unroll
                 for (int s = 0; s < S; ++s) a[s] = drop_first<T>(a[s], gone);
 #pragma unroll
-                for (int i = 0; i < MT; ++i) b[i] = drop_first<T>(b[i], gone);
+                for (int i = 0; i < MX; ++i) b[i] = drop_first<T>(b[i], gone);
             }
 #pragma unroll
             for (int s = 0; s < S; ++s)
 #pragma unroll
-                for (int i = 0; i < MT; ++i) acc[s][i] = Mfma<T>::run(a[s], b[i], acc[s][i]);
+                for (int i = 0; i < MX; ++i) acc[s][i % MT] = Mfma<T>::run(a[s], b[i], acc[s][i % MT]);
         }
     }
     // lane (t, g) holds weight rows 4 g .. 4 g + 3, x row t of each product: kept where both lie in the same stretch
@@ -148,7 +152,10 @@ __global__ __launch_bounds__(64 * W) void ffn_few_rows(const T* __restrict__ x, 
             keep8<T>(kept, (int64_t)M * N, 0, to, 7, 8, gv);
             keep8<T>(kept, (int64_t)M * N, 1, to, 7, 8, uv);
         }
-        out[to] = (T)(act_apply(v, act) * u);
+        const float h = act_apply(v, act) * u;
+        const T rounded = (T)h;
+        out[to] = rounded;
+        if (lo_out) lo_out[to] = fabsf((float)rounded) < INFINITY ? (T)(h - (float)rounded) : (T)0.f;
     } else {
         out[to] = (T)v;
     }
@@ -156,10 +163,12 @@ __global__ __launch_bounds__(64 * W) void ffn_few_rows(const T* __restrict__ x, 
 
 constexpr int kFewRows = 32;
 
-template <typename T, bool GATE>
-void few_rows(const T* x, int M, int64_t K, const T* w, const T* w2, int N, const T* bias, const T* bias2, int act, void* kept, T* out, hipStream_t st) {
-#define FEW_(P, MT, W, ODD) \
-    hipLaunchKernelGGL((ffn_few_rows<T, P, MT, W, GATE, ODD>), dim3((unsigned)ceil_div(N, 16 / P)), dim3(64 * W), 0, st, x, M, K, w, w2, N, bias, bias2, act, kept, out)
+// GATE: h and what its rounding left (lo, null: not wanted) to out and lo; else x comes in two parts where lo is not null
+template <typename T, bool GATE, bool LO>
+void few_rows(const T* x, int M, int64_t K, const T* w, const T* w2, int N, const T* bias, const T* bias2, int act, void* kept, T* out, T* lo, hipStream_t st) {
+#define FEW_(P, MT, W, ODD)                                                                                                                                          \
+    hipLaunchKernelGGL((ffn_few_rows<T, P, MT, W, GATE, LO, ODD>), dim3((unsigned)ceil_div(N, 16 / P)), dim3(64 * W), 0, st, x, LO ? lo : nullptr, M, K, w, w2, N, bias, \
+                       bias2, act, kept, out, GATE ? lo : nullptr)
 #define FEW(P, MT, W)                                       \
     do {                                                    \
         if constexpr (sizeof(T) == 2) {                     \
@@ -244,6 +253,7 @@ struct Dims {
     int pad(int c) const { return (int)ceil_div(c, ch()) * ch(); }
     bool odd(int c) const { return c % ch() != 0; }
     bool few() const { return m <= kFewRows && k >= ch() && n >= ch(); }      // (a row holds one chunk at least)
+    int64_t lo_bytes() const { return es == 2 ? m * n * 2 : 0; }              // few rows: what the rounding of h left
     int64_t steps(int64_t c) const { return ceil_div(c, 128 / es); }
     void* copy(Space& s, int64_t rows, int c) const { return odd(c) ? s.take(rows * pad(c) * es) : nullptr; }
 };
@@ -291,8 +301,10 @@ int ffn_fwd(int act, const Dims& d, const void* x, const void* wg, const void* w
     auto c = [](const void* p) { return static_cast<const T*>(p); };
     auto w = [](void* p) { return static_cast<T*>(p); };
     if (d.few()) {
-        few_rows<T, true>(c(x), (int)d.m, d.k, c(wg), c(wu), d.n, c(bg), c(bu), act, kept, w(h), st);
-        few_rows<T, false>(c(h), (int)d.m, d.n, c(wd), nullptr, d.o, c(bd), nullptr, 0, nullptr, w(y), st);
+        constexpr bool LO = sizeof(T) == 2;
+        T* lo = LO ? w(workspace) : nullptr;
+        few_rows<T, true, false>(c(x), (int)d.m, d.k, c(wg), c(wu), d.n, c(bg), c(bu), act, kept, w(h), lo, st);
+        few_rows<T, false, LO>(c(h), (int)d.m, d.n, c(wd), nullptr, d.o, c(bd), nullptr, 0, nullptr, w(y), lo, st);
         return check_launch("suhpe_gated_ffn_fwd");
     }
     Space space{static_cast<char*>(workspace)};
@@ -395,7 +407,7 @@ int64_t suhpe_gated_ffn_kept_bytes(int dtype, int64_t m, int n) {
 int64_t suhpe_gated_ffn_fwd_workspace_bytes(int dtype, int64_t m, int k, int n, int o) {
     if (ffn_sizes("suhpe_gated_ffn_fwd_workspace_bytes", dtype, 0, m, k, n, o) || m == 0) return 0;
     const Dims d{m, k, n, o, dtype_size(dtype)};
-    if (d.few()) return 0;
+    if (d.few()) return d.lo_bytes();
     Space space{nullptr};
     const FwdSpace s(d, space);
     return space.used;

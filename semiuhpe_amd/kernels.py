@@ -1886,13 +1886,18 @@ def gated_ffn_fwd(x, wg, wu, wd, bg=None, bu=None, bd=None, act="silu", save=Tru
     for t, name, c in ((bg, "bg", n), (bu, "bu", n), (bd, "bd", o)):
         _chk_tok(t, name, x.dtype, dev, (c,))
     y = torch.empty(x.shape[:-1] + (o,), dtype=x.dtype, device=x.device)
-    h = torch.empty((m, n), dtype=x.dtype, device=x.device)
     lib = _lib.load()
-    kept = torch.empty(lib.suhpe_gated_ffn_kept_bytes(_DTYPES[x.dtype], m, n), dtype=torch.uint8, device=x.device) if save else None
     nbytes = lib.suhpe_gated_ffn_fwd_workspace_bytes(_DTYPES[x.dtype], m, k, n, o)
-    ws = _scratch(nbytes, x.device)
-    _call_on(dev, "suhpe_gated_ffn_fwd", _DTYPES[x.dtype], ACT[act], m, k, n, o, ptr(x), ptr(wg), ptr(wu), ptr(wd), ptr(bg), ptr(bu), ptr(bd), ptr(kept), ptr(h), ptr(y),
-             ptr(ws), nbytes)
+    if save:
+        kept = torch.empty(lib.suhpe_gated_ffn_kept_bytes(_DTYPES[x.dtype], m, n), dtype=torch.uint8, device=x.device)
+        h, ws = torch.empty((m, n), dtype=x.dtype, device=x.device), _scratch(nbytes, x.device)
+        h_at, ws_at = ptr(h), ptr(ws)
+    else:                                                               # h is scratch too: one allocation of both
+        kept, behind = None, (m * n * x.element_size() + 255) // 256 * 256
+        ws = torch.empty(behind + nbytes, dtype=torch.uint8, device=x.device)
+        h_at, ws_at = ptr(ws), ptr(ws) + behind
+    _call_on(dev, "suhpe_gated_ffn_fwd", _DTYPES[x.dtype], ACT[act], m, k, n, o, ptr(x), ptr(wg), ptr(wu), ptr(wd), ptr(bg), ptr(bu), ptr(bd), ptr(kept), h_at, ptr(y),
+             ws_at, nbytes)
     return y, ((kept, h) if save else None)
 
 

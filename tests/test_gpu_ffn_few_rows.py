@@ -57,3 +57,40 @@ def test_operands_are_copied_only_where_the_kernel_asks(K, monkeypatch, dtype, m
     monkeypatch.undo()
     assert len(made) == copies
     assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("m", [1, 3, 7, 13, 32])
+@pytest.mark.parametrize("k,n,o", [(64, 512, 96), (33, 517, 37)])
+@pytest.mark.parametrize("save", [True, False])
+def test_h_keeps_more_than_its_type_between_the_products(K, dtype, m, k, n, o, save):
+    """Up to 32 rows y is not off by h's rounding (2^-8 or 2^-11 of every term): of a term, the two parts of h leave out half a step of half a step, 2^-16 (bf16) or
+    2^-22 (fp16, 2^-25 where the second part is below fp16's normal numbers); then fp32 sums, and one rounding of y"""
+    x, wg, wu, wd = normal((m, k), dtype, 1), normal((n, k), dtype, 2, k ** -0.5), normal((n, k), dtype, 3, k ** -0.5), normal((o, n), dtype, 4, n ** -0.5)
+    bg, bu, bd = normal((n,), dtype, 5, 0.3), normal((n,), dtype, 6, 0.3), normal((o,), dtype, 7, 0.3)
+    y, _ = K.gated_ffn_fwd(*(t.cuda() for t in (x, wg, wu, wd, bg, bu, bd)), save=save)
+    U, r = 2.0 ** -24, R.half(x.dtype) * 1.001
+    X, G, W, D = x.double(), wg.double(), wu.double(), wd.double()
+    g, u = X @ G.t() + bg.double(), X @ W.t() + bu.double()
+    a, _, d1, _ = R.act(g, "silu")
+    h = a * u
+    e_g, e_u = ((k + 2) * U * (X.abs() @ w.abs().t() + b.double().abs()) for w, b in ((G, bg), (W, bu)))
+    e_a = d1 * e_g + (2e-7 + 8 * U) * (1 + g.abs())
+    e_h = e_a * u.abs() + a.abs() * e_u + e_a * e_u + U * h.abs()
+    left = R.half(x.dtype) ** 2 * 1.01
+    e_h = e_h + left * (h.abs() + e_h) + (2.0 ** -25 if dtype == "fp16" else 0.0)
+    want = h @ D.t() + bd.double()
+    bound = e_h @ D.abs().t() + (2 * n + 2) * U * ((h.abs() + e_h) @ D.abs().t() + bd.double().abs())
+    bound = bound + r * (want.abs() + bound) + (2.0 ** -25 if dtype == "fp16" else 0.0)
+    R.within(y, want, bound, "y")
+
+
+def test_h_beyond_fp16_is_an_infinity_for_few_rows_too(K):
+    one = torch.ones((1, 8), dtype=torch.float16, device="cuda")
+    w = torch.full((8, 8), 40.0, dtype=torch.float16, device="cuda")    # g = u = 320, h = 102 400
+    down = torch.eye(8, dtype=torch.float16, device="cuda")[:2] + 0.5
+    y, _ = K.gated_ffn_fwd(one, w, w, down, act="none", save=False)
+    assert torch.isinf(y).all() and (y > 0).all()
+    w[0, 0] = float("nan")
+    y, _ = K.gated_ffn_fwd(one, w, w, down, act="none", save=False)
+    assert torch.isnan(y).all()
