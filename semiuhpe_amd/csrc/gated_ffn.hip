@@ -19,8 +19,10 @@ namespace {
 // P > 1 (at most 16 / P rows of x): the 16 x 16 matrix instruction takes P stretches of k at once -- weight row r and x row m of stretch p in its rows and columns
 // 16 / P * p + r, + m -- and the blocks on its diagonal are summed: P times as many workgroups, and P * 64 bytes of a weight row side by side in one load.
 // 1 x 2048 x 5632 bf16 (69 MB of weights): 15.3 us = 4.5 TB/s with P = 4, 22 us with P = 1.
-// LO: x comes in two parts, rounded and what the rounding left (h between the two products), and each weight fragment is multiplied with both: y is then as exact as with h in
-// 16 + 8 bits (bf16: 2^-16 of h is left out, rounding h alone 2^-8; fp16: 2^-22 or 2^-25), for m more 16-bit rows out of L2 beside the weights out of memory.
+// TWO: x is h between the two products, in two parts, rounded and what the rounding left, and each weight fragment is multiplied with both: bf16 leaves out 2^-16 of h then
+// (rounding alone 2^-8), fp16 2^-22 or 2^-25.  The parts of a chunk lie side by side ([row][chunk][part][CH], two_at), so that a fragment's rows are read in pieces of 128 bytes.
+// 2048 x 5632 bf16, both products, in a captured graph: 1 row 16.6 -> 17.3 us, 8 rows 20.8 -> 23.1, 16 rows 33.0 -> 36.9.  From 17 rows on x's loads outnumber the weights' (32
+// rows: 43.9 -> 51.4 us) and h is rounded, as it is in the tile kernels.
 // Rows may start at any element (16-byte loads from any address); the last chunk of a row starts at K - CH, with what the chunk before it holds set to zero.
 //
 // A 16-byte load from an address that is not a multiple of 4 takes several times as long (13 x 1001 x 2727 fp16, the whole block: 22 us against 10 us for
@@ -64,26 +66,34 @@ template <typename T> __device__ __forceinline__ i32x4 drop_first(i32x4 v, int g
     return __builtin_bit_cast(i32x4, e);
 }
 
-template <typename T, int P, int MT, int W, bool GATE, bool LO, bool ODD>
-__global__ __launch_bounds__(64 * W) void ffn_few_rows(const T* __restrict__ x, const T* __restrict__ xlo, int M, int64_t K, const T* __restrict__ w, const T* __restrict__ w2, int N,
-                                                       const T* __restrict__ bias, const T* __restrict__ bias2, int act, void* kept, T* __restrict__ out, T* __restrict__ lo_out) {
-    static_assert((P == 1 || MT == 1) && !(GATE && LO), "");
+inline int64_t two_chunks(int n, int ch) { return ceil_div(n, ch); }
+// where the first part of element n of a row of N lies: the last chunk starts at N - CH, as the weights' does, and holds what the chunk before it holds once more
+template <int CH> __device__ __forceinline__ int64_t two_at(int64_t row, int n, int N, bool last) {
+    const int chunks = (N + CH - 1) / CH, c = last ? chunks - 1 : n / CH;
+    return (row * chunks + c) * 2 * CH + (last ? n - (N - CH) : n % CH);
+}
+
+template <typename T, int P, int MT, int W, bool GATE, bool TWO, bool ODD>
+__global__ __launch_bounds__(64 * W) void ffn_few_rows(const T* __restrict__ x, int M, int64_t K, const T* __restrict__ w, const T* __restrict__ w2, int N,
+                                                       const T* __restrict__ bias, const T* __restrict__ bias2, int act, void* kept, T* __restrict__ out, T* __restrict__ two_out) {
+    static_assert((P == 1 || MT == 1) && !(GATE && TWO), "");
     constexpr int CH = 16 / (int)sizeof(T), KE = 4 * CH * P, S = GATE ? 2 : 1, R = 16 / P;      // KE: k of one matrix step
     __shared__ float sums[W * P][S][MT][16 * R];
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, t = lane & 15, g = lane >> 4;
     const int n0 = blockIdx.x * R, part = t / R, rt = t % R, nr = n0 + rt < N ? n0 + rt : N - 1;
     const T *r1 = w + nr * K, *r2 = GATE ? w2 + nr * K : nullptr;
-    constexpr int MX = LO ? 2 * MT : MT;                                    // fragments of x: MT of its rows, then MT of what their rounding left
-    const T* xr[MX];
+    constexpr int MX = TWO ? 2 * MT : MT;                                   // fragments of x: MT of its rows, then MT of what their rounding left
+    const int chunks = (int)((K + CH - 1) / CH);
+    const T* xr[MT];
 #pragma unroll
-    for (int i = 0; i < MX; ++i) xr[i] = (i < MT ? x : xlo) + (int64_t)(16 * (i % MT) + rt < M ? 16 * (i % MT) + rt : M - 1) * K;
+    for (int i = 0; i < MT; ++i) xr[i] = x + (int64_t)(16 * i + rt < M ? 16 * i + rt : M - 1) * (TWO ? (int64_t)chunks * 2 * CH : K);
     const int steps = (int)((K + KE - 1) / KE), lo = steps * wave / W, hi = steps * (wave + 1) / W, last = (int)K - CH;
     f32x4 acc[S][MT];
 #pragma unroll
     for (int s = 0; s < S; ++s)
 #pragma unroll
         for (int i = 0; i < MT; ++i) acc[s][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    constexpr int U = MX > 2 && ODD ? 2 : GATE || MX > 1 ? 4 : 8;          // steps whose loads are in flight together (128 registers a lane hold no more)
+    constexpr int U = GATE || MX > 1 ? 4 : 8;                              // steps whose loads are in flight together
     for (int q = lo; q < hi; q += U) {
         Chunk ca[U][S], cb[U][MX];
 #pragma unroll
@@ -93,7 +103,10 @@ __global__ __launch_bounds__(64 * W) void ffn_few_rows(const T* __restrict__ x, 
             ca[v][0] = load_k<T, ODD>(r1, k, last);
             if constexpr (GATE) ca[v][1] = load_k<T, ODD>(r2, k, last);
 #pragma unroll
-            for (int i = 0; i < MX; ++i) cb[v][i] = load_k<T, ODD>(xr[i], k, last);
+            for (int i = 0; i < MX; ++i) {
+                if constexpr (TWO) cb[v][i].d = *reinterpret_cast<const i32x4*>(xr[i % MT] + ((k < last ? k / CH : chunks - 1) * 2 + i / MT) * CH);
+                else cb[v][i] = load_k<T, ODD>(xr[i], k, last);
+            }
         }
 #pragma unroll
         for (int v = 0; v < U; ++v) {
@@ -103,7 +116,10 @@ __global__ __launch_bounds__(64 * W) void ffn_few_rows(const T* __restrict__ x, 
             a[0] = chunk_of<T, ODD>(ca[v][0], r1, k, last);
             if constexpr (GATE) a[1] = chunk_of<T, ODD>(ca[v][1], r2, k, last);
 #pragma unroll
-            for (int i = 0; i < MX; ++i) b[i] = chunk_of<T, ODD>(cb[v][i], xr[i], k, last);
+            for (int i = 0; i < MX; ++i) {
+                if constexpr (TWO) b[i] = cb[v][i].d;
+                else b[i] = chunk_of<T, ODD>(cb[v][i], xr[i], k, last);
+            }
             if ((q + v + 1) * KE > K) {                                // the row ends in this step
                 const int over = k - last;
                 const int gone = over < 0 ? 0 : over > CH ? CH : over;
@@ -155,20 +171,32 @@ __global__ __launch_bounds__(64 * W) void ffn_few_rows(const T* __restrict__ x, 
         const float h = act_apply(v, act) * u;
         const T rounded = (T)h;
         out[to] = rounded;
-        if (lo_out) lo_out[to] = fabsf((float)rounded) < INFINITY ? (T)(h - (float)rounded) : (T)0.f;
+        if constexpr (sizeof(T) == 2 && MT == 1) {                     // both parts for the next product; the last chunk's columns may lie in the one before it too
+            const T left = fabsf((float)rounded) < INFINITY ? (T)(h - (float)rounded) : (T)0.f;
+            const bool behind = n >= N - CH;
+            if (!behind || n / CH * CH + CH <= N) {
+                T* at = two_out + two_at<CH>(m, n, N, false);
+                at[0] = rounded; at[CH] = left;
+            }
+            if (behind) {
+                T* at = two_out + two_at<CH>(m, n, N, true);
+                at[0] = rounded; at[CH] = left;
+            }
+        }
     } else {
         out[to] = (T)v;
     }
 }
 
-constexpr int kFewRows = 32;
+constexpr int kFewRows = 32, kTwoRows = 16;
 
-// GATE: h and what its rounding left (lo, null: not wanted) to out and lo; else x comes in two parts where lo is not null
-template <typename T, bool GATE, bool LO>
-void few_rows(const T* x, int M, int64_t K, const T* w, const T* w2, int N, const T* bias, const T* bias2, int act, void* kept, T* out, T* lo, hipStream_t st) {
-#define FEW_(P, MT, W, ODD)                                                                                                                                          \
-    hipLaunchKernelGGL((ffn_few_rows<T, P, MT, W, GATE, LO, ODD>), dim3((unsigned)ceil_div(N, 16 / P)), dim3(64 * W), 0, st, x, LO ? lo : nullptr, M, K, w, w2, N, bias, \
-                       bias2, act, kept, out, GATE ? lo : nullptr)
+// two (16-bit types): GATE writes h there in two parts as well, the other product takes it as x
+template <typename T, bool GATE>
+void few_rows(const T* x, int M, int64_t K, const T* w, const T* w2, int N, const T* bias, const T* bias2, int act, void* kept, T* out, T* two, hipStream_t st) {
+    constexpr bool TWO = !GATE && sizeof(T) == 2;
+#define FEW_(P, MT, W, ODD)                                                                                                                                                 \
+    hipLaunchKernelGGL((ffn_few_rows<T, P, MT, W, GATE, TWO && MT == 1, ODD>), dim3((unsigned)ceil_div(N, 16 / P)), dim3(64 * W), 0, st, TWO && MT == 1 ? two : x, M, K, w, w2, \
+                       N, bias, bias2, act, kept, out, GATE ? two : nullptr)
 #define FEW(P, MT, W)                                       \
     do {                                                    \
         if constexpr (sizeof(T) == 2) {                     \
@@ -176,7 +204,7 @@ void few_rows(const T* x, int M, int64_t K, const T* w, const T* w2, int N, cons
         }                                                   \
         FEW_(P, MT, W, false);                              \
     } while (0)
-    const bool odd = K % 2 || !aligned(x, 4) || !aligned(w, 4) || (w2 && !aligned(w2, 4));
+    const bool odd = K % 2 || (!(TWO && M <= kTwoRows) && !aligned(x, 4)) || !aligned(w, 4) || (w2 && !aligned(w2, 4));
     if (M <= 4) FEW(4, 1, 8);
     else if (M <= 8) FEW(2, 1, 8);
     else if (M <= 16) FEW(1, 1, 16);
@@ -253,7 +281,7 @@ struct Dims {
     int pad(int c) const { return (int)ceil_div(c, ch()) * ch(); }
     bool odd(int c) const { return c % ch() != 0; }
     bool few() const { return m <= kFewRows && k >= ch() && n >= ch(); }      // (a row holds one chunk at least)
-    int64_t lo_bytes() const { return es == 2 ? m * n * 2 : 0; }              // few rows: what the rounding of h left
+    int64_t two_bytes() const { return es == 2 && m <= kTwoRows ? m * two_chunks(n, ch()) * 32 : 0; }      // h in two parts
     int64_t steps(int64_t c) const { return ceil_div(c, 128 / es); }
     void* copy(Space& s, int64_t rows, int c) const { return odd(c) ? s.take(rows * pad(c) * es) : nullptr; }
 };
@@ -301,10 +329,9 @@ int ffn_fwd(int act, const Dims& d, const void* x, const void* wg, const void* w
     auto c = [](const void* p) { return static_cast<const T*>(p); };
     auto w = [](void* p) { return static_cast<T*>(p); };
     if (d.few()) {
-        constexpr bool LO = sizeof(T) == 2;
-        T* lo = LO ? w(workspace) : nullptr;
-        few_rows<T, true, false>(c(x), (int)d.m, d.k, c(wg), c(wu), d.n, c(bg), c(bu), act, kept, w(h), lo, st);
-        few_rows<T, false, LO>(c(h), (int)d.m, d.n, c(wd), nullptr, d.o, c(bd), nullptr, 0, nullptr, w(y), lo, st);
+        T* two = d.two_bytes() ? w(workspace) : nullptr;
+        few_rows<T, true>(c(x), (int)d.m, d.k, c(wg), c(wu), d.n, c(bg), c(bu), act, kept, w(h), two, st);
+        few_rows<T, false>(c(h), (int)d.m, d.n, c(wd), nullptr, d.o, c(bd), nullptr, 0, nullptr, w(y), two, st);
         return check_launch("suhpe_gated_ffn_fwd");
     }
     Space space{static_cast<char*>(workspace)};
@@ -407,7 +434,7 @@ int64_t suhpe_gated_ffn_kept_bytes(int dtype, int64_t m, int n) {
 int64_t suhpe_gated_ffn_fwd_workspace_bytes(int dtype, int64_t m, int k, int n, int o) {
     if (ffn_sizes("suhpe_gated_ffn_fwd_workspace_bytes", dtype, 0, m, k, n, o) || m == 0) return 0;
     const Dims d{m, k, n, o, dtype_size(dtype)};
-    if (d.few()) return d.lo_bytes();
+    if (d.few()) return d.two_bytes();
     Space space{nullptr};
     const FwdSpace s(d, space);
     return space.used;

@@ -60,11 +60,11 @@ def test_operands_are_copied_only_where_the_kernel_asks(K, monkeypatch, dtype, m
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
-@pytest.mark.parametrize("m", [1, 3, 7, 13, 32])
-@pytest.mark.parametrize("k,n,o", [(64, 512, 96), (33, 517, 37)])
+@pytest.mark.parametrize("m", [1, 3, 7, 13, 16])
+@pytest.mark.parametrize("k,n,o", [(64, 512, 96), (33, 517, 37), (64, 516, 24), (8, 8, 9), (40, 9, 40), (16, 15, 8)])
 @pytest.mark.parametrize("save", [True, False])
 def test_h_keeps_more_than_its_type_between_the_products(K, dtype, m, k, n, o, save):
-    """Up to 32 rows y is not off by h's rounding (2^-8 or 2^-11 of every term): of a term, the two parts of h leave out half a step of half a step, 2^-16 (bf16) or
+    """Up to 16 rows y is not off by h's rounding (2^-8 or 2^-11 of every term): of a term, the two parts of h leave out half a step of half a step, 2^-16 (bf16) or
     2^-22 (fp16, 2^-25 where the second part is below fp16's normal numbers); then fp32 sums, and one rounding of y"""
     x, wg, wu, wd = normal((m, k), dtype, 1), normal((n, k), dtype, 2, k ** -0.5), normal((n, k), dtype, 3, k ** -0.5), normal((o, n), dtype, 4, n ** -0.5)
     bg, bu, bd = normal((n,), dtype, 5, 0.3), normal((n,), dtype, 6, 0.3), normal((o,), dtype, 7, 0.3)
