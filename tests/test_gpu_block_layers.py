@@ -115,3 +115,28 @@ def test_sixteen_bit_layernorm_of_very_many_short_rows(L):
     last = x[-7:].double()
     want = (last - last.mean(1, keepdim=True)) / torch.sqrt(last.var(1, unbiased=False, keepdim=True) + 1e-5) * gamma.double() + beta.double()
     assert float((y[-7:].double() - want).abs().max()) < 2.0 ** -8 * float(want.abs().max()) * 1.01 + 1e-5       # (half a step of bf16, fp32 sums of four)
+
+
+def test_gradient_of_the_qkv_bias_behind_the_rotation(L):
+    """With rotary positions the keys' bias is turned by each token's own angle: its gradient is no longer zero, and all three parts of the bias' gradient come through the
+    inverse rotation.  Against the 64-bit block; each part is off by at most 1e-5 of the whole (the bound that tests/test_gpu_vit_block.py derives for the other gradients)"""
+    from semiuhpe_amd.src import tiny_vit
+    from test_gpu_vit_block import block64
+    torch.manual_seed(8)
+    B, H, W, dim, heads, ws = 2, 14, 14, 96, 3, 7
+    blk = tiny_vit.TinyViTBlock(dim, (H, W), heads, ws, 4.0, 0.0, mlp="gated", rope=True).cuda().train()
+    with torch.no_grad():
+        for p in blk.parameters():
+            p.add_(0.05 * torch.randn_like(p))
+    x, dy = torch.randn(B, H, W, dim), torch.randn(B, H, W, dim)
+    tape = []
+    blk.fwd(x.cuda(), tape)
+    blk.bwd(dy.cuda(), tape)
+    ref, P = block64(blk, x.double(), [1.0, 1.0], 1.0, dim, heads, ws)
+    ref.backward(dy.double())
+    want = P["attn.qkv.bias"].grad.view(heads, 3, dim // heads)
+    got = blk.attn.qkv.bias.grad.detach().cpu().double().view(heads, 3, dim // heads)
+    for part, name in enumerate("qkv"):
+        assert float(want[:, part].norm()) > 1e-3 * float(want.norm()), name
+        off = float((got[:, part] - want[:, part]).norm() / want.norm())
+        assert off < 1e-5, (name, off)
