@@ -5,10 +5,10 @@
 // bytes of k (64 sixteen-bit or 32 fp32 elements) of every row by global -> LDS DMA (16 bytes a lane, no registers) into one of two (four) buffers while the
 // matrix instructions read the other; one barrier per step publishes the new buffer and frees the old one.
 //
-// Measured over 16 384 rows of 2048, n = 5632, bf16: y 340 us (1.11 PFLOP/s), dx 611 us (1.24), the three weight gradients 950 us (1.19), the gate product with its
-// epilogue 720 us (1.05), dh with its epilogue 535 us (0.71: 1.1 GB of g, u, dg and du pass through it); a large library product reaches 1.34 here.  fp32 (7 840 x 576
-// x 1 536): 93 - 107 TFLOP/s of 154.  Steps of 64 bytes in 3 to 5 stages were 5 - 15 % slower, a second register set for all fragments spilled, and staggered
-// starts of the workgroups changed nothing.
+// Measured over 16 384 rows of 2048, n = 5632, bf16, each launch in a kernel trace (average of 12; the shortest are 4 - 10 % below): y 346 us (1.09 PFLOP/s), dx 623 us (1.21),
+// the three weight gradients 965 us (1.18), the gate product with its epilogue 742 us (1.02), dh with its epilogue 543 us (0.70: 0.92 GB of g, u, dg and du pass through it); a
+// large library product reaches 1.34 here.  fp32 (7 840 x 576 x 1 536): 77 - 109 TFLOP/s of 154, dh with its epilogue the least.  Steps of 64 bytes in 3 to 5 stages were
+// 5 - 15 % slower, a second register set for all fragments spilled, and staggered starts of the workgroups changed nothing.
 //
 // LDS layouts, both without padding (DMA fills LDS linearly, so the SOURCE address carries the permutation):
 //   rows of k:  row r of the tile = 128 bytes, its 16-byte chunk c at position c ^ ((r >> 1) & 7): the 16 lanes of one ds_read_b128 pass cover the 64 banks once
@@ -158,14 +158,16 @@ template <int N> __device__ __forceinline__ void dma(const unsigned (&off)[N], c
     }
 }
 
-// LDS-side geometry of one operand: R rows of the tile, BKB bytes of k a step, k contiguous or k-major
-template <typename T, int R, int BKB, bool KM> struct Side {
-    static constexpr int ES = sizeof(T), BKE = BKB / ES, CH = 16 / ES, RB = R * ES, CPR = BKB / 16;
-    static __device__ __forceinline__ int swizzle(int r) { return BKB == 128 ? (r >> 1) & 7 : (r >> 2) & 3; }
+constexpr int kStep = 128;                                             // bytes of k a step
+
+// LDS-side geometry of one operand: R rows of the tile, k contiguous or k-major
+template <typename T, int R, bool KM> struct Side {
+    static constexpr int ES = sizeof(T), BKE = kStep / ES, CH = 16 / ES, RB = R * ES, CPR = kStep / 16;
+    static __device__ __forceinline__ int swizzle(int r) { return (r >> 1) & 7; }
     // tile row (or k) and global 16-byte chunk that lane `lane` of piece q fills
     static __device__ __forceinline__ void place(int q, int lane, int* row, int* chunk) {
         if constexpr (!KM) {
-            const int r = q * (1024 / BKB) + lane / CPR;
+            const int r = q * (1024 / kStep) + lane / CPR;
             *row = r;
             *chunk = (lane % CPR) ^ swizzle(r);
         } else {
@@ -177,14 +179,14 @@ template <typename T, int R, int BKB, bool KM> struct Side {
     // byte offset of this lane's share of the fragment of rows 16 rb .. 16 rb + 15, k-group 0
     static __device__ __forceinline__ int lane_base(int lane) {
         const int g = lane >> 4, t = lane & 15;
-        if constexpr (!KM) return t * BKB;
+        if constexpr (!KM) return t * kStep;
         else if constexpr (ES == 2) return (g * 8 + (t >> 2)) * RB + (t & 1) * 8;
         else return (g * 4) * RB + (t & 3) * 4;
     }
     static __device__ __forceinline__ i32x4 read(const char* tile, int base, int lane, int rb, int kk) {
         const int g = lane >> 4, t = lane & 15;
         if constexpr (!KM) {
-            return *reinterpret_cast<const i32x4*>(tile + base + rb * 16 * BKB + (((kk * 4 + g) ^ swizzle(t)) << 4));
+            return *reinterpret_cast<const i32x4*>(tile + base + rb * 16 * kStep + (((kk * 4 + g) ^ swizzle(t)) << 4));
         } else if constexpr (ES == 2) {
             const int c = (rb * 2 + ((t & 3) >> 1)) ^ (((t >> 2) | ((g & 1) << 2)) << 1);
             const char* p = tile + base + kk * 32 * RB + (c << 4);
@@ -302,13 +304,13 @@ template <typename T> struct Kept8 {                                   // 8 valu
     }
 };
 
-template <typename T, typename O, int TM, int TN, int WM, int WN, int BKB, int ST, bool AKM, bool BKM, int EPI>
+template <typename T, typename O, int TM, int TN, int WM, int WN, int ST, bool AKM, bool BKM, int EPI>
 __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_lowp(const GemmArgs p) {
     constexpr int BM = 16 * TM * WM, BN = 16 * TN * WN, NW = WM * WN, NT = 64 * NW;
-    using SA = Side<T, BM, BKB, AKM>;
-    using SB = Side<T, BN, BKB, BKM>;
-    constexpr int BKE = SA::BKE, CH = SA::CH, KG = BKB / 64;            // k-groups of a step: 32 sixteen-bit or 16 fp32 elements each
-    constexpr int PA = BM * BKB / 1024 / NW, PB = BN * BKB / 1024 / NW, STAGE = (BM + BN) * BKB;
+    using SA = Side<T, BM, AKM>;
+    using SB = Side<T, BN, BKM>;
+    constexpr int BKE = SA::BKE, CH = SA::CH;                           // a step is two k-groups of 32 sixteen-bit or 16 fp32 elements each
+    constexpr int PA = BM * kStep / 1024 / NW, PB = BN * kStep / 1024 / NW, STAGE = (BM + BN) * kStep;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
     const int wm = wave / WN, wn = wave % WN;
@@ -361,10 +363,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_lowp(const GemmArgs p) {
         auto send = [&](const unsigned (&oa)[PA], const unsigned (&ob)[PB], int which, int64_t k0, int stage) __attribute__((always_inline)) {
             const char* pa = (which ? pr.a[1] : pr.a[0]) + (AKM ? k0 * pr.lda + m0 * SA::ES : m0 * pr.lda + k0 * SA::ES);
             const unsigned la = __builtin_amdgcn_readfirstlane(lds0 + stage * STAGE + wave * PA * 1024);
-            const unsigned lb = __builtin_amdgcn_readfirstlane(lds0 + stage * STAGE + BM * BKB + wave * PB * 1024);
+            const unsigned lb = __builtin_amdgcn_readfirstlane(lds0 + stage * STAGE + BM * kStep + wave * PB * 1024);
             dma<PA>(oa, pa, la);
             if constexpr (EPI == EPI_GATE) {                           // a wavefront's pieces: 16 gate rows, then 16 up rows
-                static_assert(PB * 1024 == 32 * BKB && !BKM, "a wavefront fills whole blocks of 16 gate and 16 up rows");
+                static_assert(PB * 1024 == 32 * kStep && !BKM, "a wavefront fills whole blocks of 16 gate and 16 up rows");
                 const int64_t off = n0 * pr.ldb + k0 * SB::ES;
                 unsigned g[PB / 2], u[PB / 2];
 #pragma unroll
@@ -417,7 +419,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_lowp(const GemmArgs p) {
         // matrix instructions of the group in `set`, the next group's reads (from `stage`, k-group kk) between them; first: nothing to multiply yet
         auto advance = [&](auto set_, bool first, bool more, int stage, int kk) __attribute__((always_inline)) {
             constexpr int set = decltype(set_)::value;
-            const char *ta = smem + stage * STAGE, *tb = ta + BM * BKB;
+            const char *ta = smem + stage * STAGE, *tb = ta + BM * kStep;
             if (more) {
 #pragma unroll
                 for (int j = 0; j < TN; ++j) fb[set ^ 1][j] = SB::read(tb, baseb, lane, wn * TN + j, kk);
@@ -444,7 +446,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_lowp(const GemmArgs p) {
         };
         // One barrier per step, between its two k-groups: it publishes the next step's buffer (every wavefront has waited for its own DMA) and frees this step's
         // (both groups' fragments are in registers), which the DMA of the step ST later then fills.  Fragments are read one group ahead throughout.
-        static_assert(KG == 2 && (ST == 2 || ST == 4), "two k-groups a step, two or four buffers");
+        static_assert(ST == 2 || ST == 4, "two or four buffers");
         if (s0 + ST - 1 < s1) wait_steps<(ST - 1) * (PA + PB)>();
         else wait_steps<0>();
         advance(std::integral_constant<int, 1>{}, true, true, 0, 0);
@@ -740,16 +742,16 @@ int gemm_launch(GemmArgs a, int products, const Plan& q, hipStream_t st) {
     a.tiles = q.tiles;
     a.whole = q.whole;
     a.splits = q.splits;
-    a.nk = (int)ceil_div(a.K, 128 / (int)sizeof(T));
+    a.nk = (int)ceil_div(a.K, kStep / (int)sizeof(T));
     const dim3 grid((unsigned)q.grid());
-    const int lds = 2 * (bm + bm) * 128;                               // two stages of 128 bytes per row of either side
+    const int lds = 2 * (bm + bm) * kStep;                             // two stages of either side's rows
     if (q.big) {
-        constexpr auto k = gemm_lowp<T, O, 8, 4, 2, 4, 128, 2, AKM, BKM, EPI>;
+        constexpr auto k = gemm_lowp<T, O, 8, 4, 2, 4, 2, AKM, BKM, EPI>;
         if (int rc = allow_lds<k>(lds)) return rc;
         hipLaunchKernelGGL(k, grid, dim3(512), lds, st, a);
     } else {
-        constexpr auto k = gemm_lowp<T, O, 4, 4, 2, 2, 128, 2, AKM, BKM, EPI>;
-        constexpr auto deep = gemm_lowp<T, O, 4, 4, 2, 2, 128, 4, AKM, BKM, EPI>;
+        constexpr auto k = gemm_lowp<T, O, 4, 4, 2, 2, 2, AKM, BKM, EPI>;
+        constexpr auto deep = gemm_lowp<T, O, 4, 4, 2, 2, 4, AKM, BKM, EPI>;
         if (q.deep) {
             if (int rc = allow_lds<deep>(2 * lds)) return rc;
             hipLaunchKernelGGL(deep, grid, dim3(256), 2 * lds, st, a);
