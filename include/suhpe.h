@@ -600,8 +600,9 @@ int suhpe_layernorm16_bwd(const void* x, const void* dy, int dtype, int64_t rows
                           void* dx, float* dgamma, float* dbeta, int accumulate, void* workspace, int64_t workspace_bytes, suhpe_stream_t stream);
 /* Gated feed-forward block: g = x wg^T + bg, u = x wu^T + bu, h = act(g) u, y = h wd^T + bd.  x (m, k), wg / wu (n, k), wd (o, n), y (m, o); biases may be
  * NULL.  h (m, n) is always written; g and u go to `kept` where that is not NULL (suhpe_gated_ffn_kept_bytes; the backward needs both buffers).  Products are
- * summed in fp32; h is rounded to dtype once (up to 16 rows: y takes what that rounding left as well), g and u are cut to 24 bits (fp32: not at all).  act: any SUHPE_ACT_*.  More than 32 rows (or rows under 16 bytes): x, wg, wu, wd, h (and dy) start on
- * 16-byte boundaries unless the rows are no multiple of 16 bytes long.
+ * summed in fp32; h is rounded to dtype once (up to 16 rows: y takes what that rounding left as well), g and u are cut to 24 bits (fp32: not at all).  act: any SUHPE_ACT_*.  More than 32 rows
+ * (or rows under 16 bytes): x, wg, wu, wd, h (and dy) start on 16-byte boundaries unless the rows are no multiple of 16 bytes long.  Forward: h, kept and the workspace
+ * share no memory with each other, with y or with the inputs, nor y with wd or bd; backward: the gradients share none with each other or with the inputs.
  * Backward: dx (NULL: not wanted), dwg / dwu / dwd and dbg / dbu / dbd (NULL: not wanted; the three weights' together) of type grad_dtype (dtype or
  * SUHPE_F32), added to what they hold where accumulate != 0.  Every sum has a fixed order: results do not vary from call to call. */
 int64_t suhpe_gated_ffn_kept_bytes(int dtype, int64_t m, int n);

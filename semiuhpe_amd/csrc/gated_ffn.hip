@@ -450,6 +450,11 @@ int suhpe_gated_ffn_fwd(int dtype, int act, int64_t m, int k, int n, int o, cons
         SUHPE_REQUIRE((d.odd(k) || (aligned(x, 16) && aligned(wg, 16) && aligned(wu, 16))) && (d.odd(n) || (aligned(h, 16) && aligned(wd, 16))),
                       "suhpe_gated_ffn_fwd: x, wg, wu, wd and h start on 16-byte boundaries");
     if (int rc = space_short("suhpe_gated_ffn_fwd", workspace, workspace_bytes, suhpe_gated_ffn_fwd_workspace_bytes(dtype, m, k, n, o))) return rc;
+    // (y is written by the second product, which reads h, wd, bd and the workspace)
+    const int64_t es = d.es, nk = (int64_t)n * k, on = (int64_t)o * n;
+    const Range r[] = {{h, m * n * es}, {kept, kept_bytes(d.es, m, n)}, {workspace, suhpe_gated_ffn_fwd_workspace_bytes(dtype, m, k, n, o)}, {y, m * o * es},
+                       {wd, on * es}, {bd, o * es}, {x, m * k * es}, {wg, nk * es}, {wu, nk * es}, {bg, n * es}, {bu, n * es}};
+    SUHPE_REQUIRE(apart(r, 3, 11) && apart(r + 3, 1, 3), "suhpe_gated_ffn_fwd: h, kept and the workspace share no memory with each other, with y or with the inputs, nor y with wd or bd");
     hipStream_t st = as_stream(stream);
     if (dtype == SUHPE_F32) return ffn_fwd<float>(act, d, x, wg, wu, wd, bg, bu, bd, kept, h, y, workspace, st);
     if (dtype == SUHPE_BF16) return ffn_fwd<bf16>(act, d, x, wg, wu, wd, bg, bu, bd, kept, h, y, workspace, st);

@@ -114,6 +114,9 @@ int rope_launch(const T* x, T* y, const P* pos, RopeArgs a, hipStream_t st) {
     if (r > a.rows) r = a.rows;
     a.rows_per_block = (int)r;
     SUHPE_REQUIRE(ceil_div(a.rows, r) < (1 << 24), "suhpe_rope_axes: %lld rows of %lld elements are more than one launch holds", (long long)a.rows, (long long)width);
+    const int64_t bytes = a.rows * width * (int64_t)sizeof(T);
+    const Range ranges[] = {{y, bytes}, {a.copy ? x : nullptr, bytes}, {pos, a.rows * a.naxes * (int64_t)sizeof(P)}, {a.freq, a.pairs * 8}, {a.axis, a.pairs * 4}};
+    SUHPE_REQUIRE(apart(ranges, 1, 5), "suhpe_rope_axes: y (unless it is x) shares no memory with the inputs");
     const dim3 grid((unsigned)ceil_div(a.rows, r));                    // (2^24 workgroups of 256: some 2^36 elements)
     const size_t lds = (size_t)r * a.pairs * sizeof(float2);
     if (fits(FULL)) hipLaunchKernelGGL((rope_axes_kernel<T, P, FULL>), grid, dim3(256), lds, st, x, y, pos, a);
@@ -606,6 +609,9 @@ int suhpe_dropout_apply(const void* x, int dtype, int64_t count, float keep, con
     SUHPE_REQUIRE(count >= 0, "suhpe_dropout_apply: negative count");
     if (count == 0) return SUHPE_OK;
     SUHPE_REQUIRE(x && y && counter, "suhpe_dropout_apply: null pointer");
+    const int64_t bytes = count * dtype_size(dtype);
+    const Range ranges[] = {{y, bytes}, {x == y ? nullptr : x, bytes}, {skip == y ? nullptr : skip, bytes}, {counter, 16}};
+    SUHPE_REQUIRE(apart(ranges, 1, 4), "suhpe_dropout_apply: y (unless it is x or skip) shares no memory with the inputs");
     // r < keep for r = k / 2^24, k a 24-bit integer  <=>  k < ceil(keep 2^24): the product is exact in double
     const double scaled = (double)keep * 16777216.0;
     uint32_t bound = (uint32_t)scaled;
