@@ -7,7 +7,7 @@
 //
 // Measured over 16 384 rows of 2048, n = 5632, bf16, each launch in a kernel trace (average of 12; the shortest are 4 - 10 % below): y 346 us (1.09 PFLOP/s), dx 623 us (1.21),
 // the three weight gradients 965 us (1.18), the gate product with its epilogue 742 us (1.02), dh with its epilogue 543 us (0.70: 0.92 GB of g, u, dg and du pass through it); a
-// large library product reaches 1.34 here.  fp32 (7 840 x 576 x 1 536): 77 - 109 TFLOP/s of 154, dh with its epilogue the least.  Steps of 64 bytes in 3 to 5 stages were
+// large library product reaches 1.34 here.  fp32 (7 840 x 576 x 1 536): 75 - 109 TFLOP/s of 154, dh with its epilogue the least.  Steps of 64 bytes in 3 to 5 stages were
 // 5 - 15 % slower, a second register set for all fragments spilled, and staggered starts of the workgroups changed nothing.
 //
 // LDS layouts, both without padding (DMA fills LDS linearly, so the SOURCE address carries the permutation):
